@@ -58,12 +58,17 @@ typedef int stade_status;
 #define STADE_EREPLICA   6  /* check_replicas: buffers differ across ranks   */
 
 #define STADE_HOST_SCALARS  0x1u  /* scalar adjoint out-params are host pointers */
+/* Reverse sweeps of the token-model operators (embed_b, layer_norm_b,
+ * act_tape8_b, expert_mm_b) only: */
+#define STADE_ADJ_STORE     0x2u  /* store adjoint outputs instead of adding to them:
+                                     what they hold on entry is not read            */
+#define STADE_SEED_KEEP     0x4u  /* leave the consumed seed (yb) as it is          */
 
 typedef struct stade_opts {
   void*    stream;          /* cudaStream_t; NULL = the legacy default stream     */
   void*    workspace;       /* device scratch; NULL = library-managed cache       */
   size_t   workspace_bytes; /* size of `workspace` in bytes                       */
-  uint32_t flags;           /* STADE_HOST_SCALARS                                 */
+  uint32_t flags;           /* STADE_HOST_SCALARS, STADE_ADJ_STORE, STADE_SEED_KEEP */
 } stade_opts;
 
 /* Library state ------------------------------------------------------------ */
@@ -79,9 +84,10 @@ size_t      stade_workspace_cached_bytes(void);
  * with CUDA events on their stream; stade_profile_read waits for them and
  * sums device milliseconds per phase name (names: max entries of name_len
  * bytes each). Returns the number of distinct phases recorded. */
-/* Sticky device-side error word of the kernels with bounded waits (the
- * tensor-core pipeline): 0 = none; nonzero = a wait ran out and the results of
- * that call are invalid. Reading it waits for the device and clears it. */
+/* Sticky device-side error word: 0 = none; nonzero = a bounded wait of a
+ * tensor-core kernel ran out and the results of that call are invalid, or
+ * embed / expert_mm met an id or a group bound out of range. Reading it waits
+ * for the device and clears it. */
 int         stade_device_error(void);
 /* Check of the device-side wait guard (no counterpart in the reference, whose
  * kernels have no bounded waits): one kernel waits on an mbarrier nothing
@@ -297,6 +303,9 @@ typedef struct stade_comm stade_comm;
 
 #define STADE_F32 0
 #define STADE_F64 1
+/* 16-bit element types, of the token-model operators only */
+#define STADE_BF16 2
+#define STADE_F16  3
 
 /* 128 opaque bytes made on one rank and broadcast by the caller (MPI, a
  * torch.distributed store, a file) before stade_comm_init on every rank. */
@@ -438,6 +447,92 @@ stade_status stade_heat2d_b_f64_slab(double* loss, const double* lossb,
                                      int64_t n, int64_t n_step,
                                      double* u_stack, int64_t rows,
                                      stade_comm* comm, const stade_opts* opts);
+
+/* ---------------------------------------------------------------------------
+ * Operators of a token model's training step, each a forward and the reverse
+ * sweep of it (no counterpart in the reference, whose generated sweeps are
+ * loops over Float64 arrays; the forward of the reference's own
+ * test/val-corpus/transformer_b.jl sample spells such layers out).
+ *
+ * dtype: STADE_F32, STADE_F64, STADE_BF16 or STADE_F16, the element type T of
+ * the arrays that hold activations. Sums are held in P, and parameters of
+ * layer_norm, the statistics on its tape and every parameter adjoint (wb, bb)
+ * are arrays of P: Float64 for STADE_F64, Float32 otherwise, so that several
+ * micro-batches add up without rounding to 16 bits in between.
+ *
+ * The reverse sweeps follow the conventions above: xb, wb and bb are added to
+ * and the seed yb ends at zero. STADE_ADJ_STORE stores instead of adding (no
+ * reset before, no read of the old value), STADE_SEED_KEEP leaves yb. They
+ * take only what they read: what the forward left on its tape (`*_stack`),
+ * not y. Arrays must not overlap, except xb and yb of act_tape8_b, which may
+ * be the same array with both flags set. Sums run in a fixed order.
+ * ------------------------------------------------------------------------- */
+
+/* embed: y[s] = scale w[ids[s] - base] (rows of n_d), s = 0 .. n_s - 1; base 0
+ * or 1 as the caller counts. An id below base is padding: a zero row of y, no
+ * gradient. An id of n_v + base or more is treated the same and sets the
+ * device error word (stade_device_error). scale is a constant of the program.
+ * w, y: T; wb: P. Also gathers rows by any index list (w: any n_v x n_d
+ * array), with embed_b the matching scatter-add. */
+stade_status stade_embed(int dtype, const void* w, const int64_t* ids, void* y, double scale,
+                         int64_t base, int64_t n_s, int64_t n_v, int64_t n_d,
+                         const stade_opts* opts);
+size_t stade_embed_b_workspace(int64_t n_s, int64_t n_v, int64_t n_d);
+stade_status stade_embed_b(int dtype, void* wb, const int64_t* ids, void* yb, double scale,
+                           int64_t base, int64_t n_s, int64_t n_v, int64_t n_d,
+                           const stade_opts* opts);
+
+/* layer_norm: h = (x - mean) rstd, y = h w + b over rows of n_d, rstd =
+ * 1 / sqrt(var + eps). w == NULL counts as ones, b == NULL as zeros. m_stack
+ * and r_stack (n_s of P) receive mean and rstd. layer_norm_b: any of xb, wb,
+ * bb may be NULL (not wanted). x, y, xb, yb: T; the rest P. */
+stade_status stade_layer_norm(int dtype, const void* x, const void* w, const void* b, void* y,
+                              void* m_stack, void* r_stack, double eps, int64_t n_s, int64_t n_d,
+                              const stade_opts* opts);
+size_t stade_layer_norm_b_workspace(int dtype, int64_t n_s, int64_t n_d);
+stade_status stade_layer_norm_b(int dtype, const void* x, void* xb, const void* w, void* wb,
+                                void* bb, void* yb, const void* m_stack, const void* r_stack,
+                                int64_t n_s, int64_t n_d, const stade_opts* opts);
+
+/* The 8-bit tape (T: Float32 or 16 bits): q_stack holds n_s n_d int8 codes,
+ * e_stack stade_initstacks_tape8(n_s, n_d) scale bytes, one per 32 values of
+ * a row (the last group of a row may be shorter). A group's values read back
+ * as q 2^e, within 2^e / 2 of what was written (2^e in the top 1/128 of the
+ * group's binade), 2^e = 1/64 of the power of two at or below the group's
+ * largest magnitude; a group that held an infinity or NaN reads back as NaN.
+ * push writes the tape, pop restores x from it. act_tape8 also computes
+ * y = f(x); act_tape8_b adds yb f'(x^) to xb, x^ from the tape. relu'(0) =
+ * 1/2, as in the generated sweeps. */
+#define STADE_ACT_NONE 0
+#define STADE_ACT_RELU 1
+#define STADE_ACT_TANH 2
+#define STADE_ACT_SILU 3  /* x / (1 + exp(-x))              */
+#define STADE_ACT_GELU 4  /* x (1 + erf(x / sqrt 2)) / 2    */
+int64_t stade_initstacks_tape8(int64_t n_s, int64_t n_d);
+stade_status stade_tape8_push(int dtype, const void* x, int8_t* q_stack, uint8_t* e_stack,
+                              int64_t n_s, int64_t n_d, const stade_opts* opts);
+stade_status stade_tape8_pop(int dtype, void* x, const int8_t* q_stack, const uint8_t* e_stack,
+                             int64_t n_s, int64_t n_d, const stade_opts* opts);
+stade_status stade_act_tape8(int dtype, int act, const void* x, void* y, int8_t* q_stack,
+                             uint8_t* e_stack, int64_t n_s, int64_t n_d, const stade_opts* opts);
+stade_status stade_act_tape8_b(int dtype, int act, void* xb, void* yb, const int8_t* q_stack,
+                               const uint8_t* e_stack, int64_t n_s, int64_t n_d,
+                               const stade_opts* opts);
+
+/* expert_mm: rows grouped by expert. Rows off[e] .. off[e + 1] - 1 (0-based,
+ * off: n_e + 1 rising bounds on the device) belong to expert e; groups may be
+ * empty; rows in no group get y = 0 and no gradient. y[s] = x[s] w[e], w[e]:
+ * n_i x n_o input-major. Bounds that fall or leave 0 .. n_s are clamped and
+ * set the device error word. expert_mm_b: xb or wb may be NULL (not wanted).
+ * x, w, y, xb, yb: T; wb: P. Supported: n_e < 65534. */
+size_t stade_expert_mm_workspace(int dtype, int64_t n_s, int64_t n_e, int64_t n_i, int64_t n_o);
+stade_status stade_expert_mm(int dtype, const void* x, const void* w, void* y, const int64_t* off,
+                             int64_t n_s, int64_t n_e, int64_t n_i, int64_t n_o,
+                             const stade_opts* opts);
+size_t stade_expert_mm_b_workspace(int dtype, int64_t n_s, int64_t n_e, int64_t n_i, int64_t n_o);
+stade_status stade_expert_mm_b(int dtype, const void* x, void* xb, const void* w, void* wb,
+                               void* yb, const int64_t* off, int64_t n_s, int64_t n_e,
+                               int64_t n_i, int64_t n_o, const stade_opts* opts);
 
 /* ---------------------------------------------------------------------------
  * Synthetic inputs (host side). Seed = FNV-1a-64 of a name, the scheme of

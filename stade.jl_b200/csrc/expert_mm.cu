@@ -1,0 +1,302 @@
+// expert_mm and expert_mm_b: matrix products grouped by expert, with ragged
+// groups whose bounds are on the device.
+//
+//   rows off[e] .. off[e + 1] - 1 belong to expert e (off has n_e + 1 entries)
+//   y[s, :] = x[s, :] W[e]                    W: n_e x n_i x n_o
+//   xb[s, :] += yb[s, :] W[e]^T
+//   wb[e] += sum over the expert's rows of x[s, :]^T yb[s, :]
+//
+// Rows in no group get y = 0 and add nothing. The bounds are read on the
+// device, so a router's counts never visit the host: one small kernel cuts
+// every group into row tiles, and the product kernels walk that list. Bounds
+// that fall or leave 0 .. n_s are clamped and set the device error word.
+
+#include <initializer_list>
+
+#include "token_ops.cuh"
+
+namespace stade {
+namespace {
+
+__device__ int g_expert_error = 0;
+
+struct Tile {
+  int expert, row, rows, pad;   // expert < 0: rows of no group
+};
+
+constexpr int kTile = 64;       // rows and columns of a CUDA-core tile
+constexpr int kStep = 16;
+
+// One block. bounds[0 .. n_e]: the clamped, rising bounds; tiles of at most
+// `tile` rows of every group, then of the rows in no group; count[0]: how many.
+__global__ void __launch_bounds__(1024)
+plan_kernel(const int64_t* __restrict__ off, int64_t n_s, int64_t n_e, int tile,
+            int64_t* __restrict__ bounds, Tile* __restrict__ tiles, int* __restrict__ count) {
+  __shared__ long long scan[1024];
+  __shared__ long long carry_bound;
+  __shared__ int carry_tiles;
+  const int t = threadIdx.x;
+  if (t == 0) {
+    carry_bound = 0;
+    carry_tiles = 0;
+  }
+  __syncthreads();
+  // rising bounds: a running maximum of the clamped entries
+  for (int64_t e0 = 0; e0 <= n_e; e0 += 1024) {
+    const int64_t e = e0 + t;
+    long long v = 0;
+    if (e <= n_e) {
+      const long long raw = off[e];
+      if (raw < 0 || raw > n_s || (e > 0 && raw < off[e - 1])) g_expert_error = 1;
+      v = min(max(raw, 0ll), (long long)n_s);
+    }
+    scan[t] = v;
+    __syncthreads();
+    for (int o = 1; o < 1024; o <<= 1) {
+      const long long u = t >= o ? scan[t - o] : 0;
+      __syncthreads();
+      scan[t] = max(scan[t], u);
+      __syncthreads();
+    }
+    if (e <= n_e) bounds[e] = max(scan[t], carry_bound);
+    __syncthreads();
+    if (t == 1023) carry_bound = max(scan[t], carry_bound);
+    __syncthreads();
+  }
+  // group n_e: the rows before the first bound, group n_e + 1: those after the last
+  for (int64_t e0 = 0; e0 < n_e + 2; e0 += 1024) {
+    const int64_t e = e0 + t;
+    int64_t a = 0, b = 0;
+    if (e < n_e) a = bounds[e], b = bounds[e + 1];
+    else if (e == n_e) b = bounds[0];
+    else if (e == n_e + 1) a = bounds[n_e], b = n_s;
+    const int mine = (int)((b - a + tile - 1) / tile);
+    scan[t] = mine;
+    __syncthreads();
+    for (int o = 1; o < 1024; o <<= 1) {
+      const long long u = t >= o ? scan[t - o] : 0;
+      __syncthreads();
+      scan[t] += u;
+      __syncthreads();
+    }
+    int at = carry_tiles + (int)scan[t] - mine;
+    for (int i = 0; i < mine; ++i, ++at)
+      tiles[at] = Tile{e < n_e ? (int)e : -1, (int)(a + (int64_t)i * tile),
+                       (int)min((int64_t)tile, b - a - (int64_t)i * tile), 0};
+    __syncthreads();
+    if (t == 1023) carry_tiles += (int)scan[t];
+    __syncthreads();
+  }
+  if (t == 0) count[0] = carry_tiles;
+}
+
+// C[m][n] (+)= sum_k A(m, k) B(k, n) of one 64 x 64 tile, A(m, k) =
+// a[m am + k ak], B(k, n) = b[k bk + n bn], C[m][n] = c[m ldc + n].
+template <class T, class O>
+__device__ __forceinline__ void simt_tile(const T* __restrict__ a, int64_t am, int64_t ak,
+                                          const T* __restrict__ b, int64_t bk, int64_t bn,
+                                          O* __restrict__ c, int64_t ldc, int M, int N, int64_t K,
+                                          bool add) {
+  using A = acc_t<T>;
+  __shared__ A as[kStep][kTile + 1], bs[kStep][kTile + 1];
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  A acc[4][4] = {};
+  for (int64_t k0 = 0; k0 < K; k0 += kStep) {
+    for (int i = tid; i < kStep * kTile; i += 256) {
+      const int ka = ak == 1 ? i % kStep : i / kTile, ma = ak == 1 ? i / kStep : i % kTile;
+      as[ka][ma] = ma < M && k0 + ka < K ? load_acc<T>(a[ma * am + (k0 + ka) * ak]) : A(0);
+      const int kb = bk == 1 ? i % kStep : i / kTile, nb = bk == 1 ? i / kStep : i % kTile;
+      bs[kb][nb] = nb < N && k0 + kb < K ? load_acc<T>(b[(k0 + kb) * bk + nb * bn]) : A(0);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kStep; ++k) {
+      A ra[4], rb[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ra[i] = as[k][ty + 16 * i], rb[i] = bs[k][tx + 16 * i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] += ra[i] * rb[j];
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int m = ty + 16 * i, n = tx + 16 * j;
+      if (m < M && n < N) {
+        O* p = c + m * ldc + n;
+        *p = round_to<O>(add ? load_acc<O>(*p) + acc[i][j] : acc[i][j]);
+      }
+    }
+}
+
+// rows x width: y = x W (trans false) or xb = yb W^T (trans true)
+template <class T>
+__global__ void __launch_bounds__(256)
+expert_rows_kernel(const T* __restrict__ in, const T* __restrict__ w, T* __restrict__ out,
+                   const Tile* __restrict__ tiles, const int* __restrict__ count, int64_t n_i,
+                   int64_t n_o, bool trans, bool add) {
+  if ((int)blockIdx.x >= *count) return;
+  const Tile t = tiles[blockIdx.x];
+  const int64_t width = trans ? n_i : n_o, depth = trans ? n_o : n_i;
+  const int64_t n0 = (int64_t)blockIdx.y * kTile;
+  const T* wt = w + (int64_t)max(t.expert, 0) * n_i * n_o + (trans ? n0 * n_o : n0);
+  simt_tile<T, T>(in + (int64_t)t.row * depth, depth, 1, wt, trans ? 1 : n_o, trans ? n_o : 1,
+                  out + (int64_t)t.row * width + n0, width, t.rows,
+                  (int)min((int64_t)kTile, width - n0), t.expert < 0 ? 0 : depth, add);
+}
+
+template <class T>
+__global__ void __launch_bounds__(256)
+expert_wgrad_kernel(const T* __restrict__ x, const T* __restrict__ yb, acc_t<T>* __restrict__ wb,
+                    const int64_t* __restrict__ bounds, int64_t n_i, int64_t n_o, bool add) {
+  const int64_t e = blockIdx.z, i0 = (int64_t)blockIdx.y * kTile, o0 = (int64_t)blockIdx.x * kTile;
+  const int64_t a = bounds[e], b = bounds[e + 1];
+  simt_tile<T, acc_t<T>>(x + a * n_i + i0, 1, n_i, yb + a * n_o + o0, n_o, 1,
+                         wb + (e * n_i + i0) * n_o + o0, n_o, (int)min((int64_t)kTile, n_i - i0),
+                         (int)min((int64_t)kTile, n_o - o0), b - a, add);
+}
+
+int64_t max_tiles(int64_t n_s, int64_t n_e, int tile) { return n_s / tile + n_e + 2; }
+
+struct Plan {
+  int64_t* bounds;
+  Tile* tiles;
+  int* count;
+};
+size_t plan_bytes(int64_t n_s, int64_t n_e) {
+  Sizer z;
+  z.take<int64_t>(n_e + 1);
+  z.take<Tile>(max_tiles(n_s, n_e, kTile));
+  z.take<int>(1);
+  return z.bytes();
+}
+stade_status make_plan(const int64_t* off, int64_t n_s, int64_t n_e, void* ws, Plan* p,
+                       cudaStream_t s) {
+  Carver c(ws);
+  p->bounds = c.take<int64_t>(n_e + 1);
+  p->tiles = c.take<Tile>(max_tiles(n_s, n_e, kTile));
+  p->count = c.take<int>(1);
+  plan_kernel<<<1, 1024, 0, s>>>(off, n_s, n_e, kTile, p->bounds, p->tiles, p->count);
+  STADE_CHECK_LAUNCH();
+  return STADE_OK;
+}
+
+stade_status check_sizes(const char* who, int dtype, int64_t n_s, int64_t n_e, int64_t n_i,
+                         int64_t n_o) {
+  STADE_REQUIRE(known_dtype(dtype), "%s: bad dtype %d", who, dtype);
+  STADE_REQUIRE(n_s >= 0 && n_e >= 0 && n_i >= 0 && n_o >= 0, "%s: negative size", who);
+  int64_t t;
+  STADE_REQUIRE(n_s < (int64_t(1) << 30) && n_e < (int64_t(1) << 16) - 2 &&
+                    n_i < (int64_t(1) << 21) && n_o < (int64_t(1) << 21) &&
+                    mul_ok(n_s, n_i + n_o, &t) && mul_ok(n_e, n_i * n_o, &t),
+                "%s: size overflow", who);
+  return STADE_OK;
+}
+
+}  // namespace
+
+int expert_take_error() {
+  int host = 0;
+  const int zero = 0;
+  if (cudaMemcpyFromSymbol(&host, g_expert_error, sizeof(int)) != cudaSuccess) return -1;
+  if (host) cudaMemcpyToSymbol(g_expert_error, &zero, sizeof(int));
+  return host;
+}
+
+}  // namespace stade
+
+using namespace stade;
+
+extern "C" size_t stade_expert_mm_workspace(int dtype, int64_t n_s, int64_t n_e, int64_t n_i,
+                                            int64_t n_o) {
+  (void)dtype;
+  if (n_s <= 0 || n_e < 0 || n_i < 0 || n_o < 0) return 0;
+  return plan_bytes(n_s, n_e);
+}
+
+extern "C" stade_status stade_expert_mm(int dtype, const void* x, const void* w, void* y,
+                                        const int64_t* off, int64_t n_s, int64_t n_e, int64_t n_i,
+                                        int64_t n_o, const stade_opts* opts) {
+  stade_status st = check_sizes("expert_mm", dtype, n_s, n_e, n_i, n_o);
+  if (st != STADE_OK) return st;
+  if (n_s == 0 || n_o == 0) return STADE_OK;
+  cudaStream_t s = stream_of(opts);
+  STADE_REQUIRE(y, "expert_mm: null array argument");
+  if (n_i == 0 || n_e == 0) {   // empty sums
+    STADE_CUDA(cudaMemsetAsync(y, 0, (size_t)n_s * n_o * dtype_size(dtype), s));
+    return STADE_OK;
+  }
+  STADE_REQUIRE(x && w && off, "expert_mm: null array argument");
+  void* ws = nullptr;
+  st = get_workspace(opts, stade_expert_mm_workspace(dtype, n_s, n_e, n_i, n_o), &ws);
+  if (st != STADE_OK) return st;
+  PhaseScope ph("expert_mm", s);
+  Plan p;
+  st = make_plan(off, n_s, n_e, ws, &p, s);
+  if (st != STADE_OK) return st;
+  return with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    const dim3 grid((unsigned)max_tiles(n_s, n_e, kTile), ceil_div_u(n_o, kTile));
+    expert_rows_kernel<T><<<grid, 256, 0, s>>>((const T*)x, (const T*)w, (T*)y, p.tiles, p.count,
+                                               n_i, n_o, false, false);
+    STADE_CHECK_LAUNCH();
+    return (stade_status)STADE_OK;
+  });
+}
+
+extern "C" size_t stade_expert_mm_b_workspace(int dtype, int64_t n_s, int64_t n_e, int64_t n_i,
+                                              int64_t n_o) {
+  return stade_expert_mm_workspace(dtype, n_s, n_e, n_i, n_o);
+}
+
+extern "C" stade_status stade_expert_mm_b(int dtype, const void* x, void* xb, const void* w,
+                                          void* wb, void* yb, const int64_t* off, int64_t n_s,
+                                          int64_t n_e, int64_t n_i, int64_t n_o,
+                                          const stade_opts* opts) {
+  stade_status st = check_sizes("expert_mm_b", dtype, n_s, n_e, n_i, n_o);
+  if (st != STADE_OK) return st;
+  cudaStream_t s = stream_of(opts);
+  const bool add = accumulates(opts);
+  const size_t wsize = dtype == STADE_F64 ? 8 : 4;
+  if (n_s == 0 || n_e == 0 || n_i == 0 || n_o == 0) {   // empty sums
+    if (!add && wb && n_e * n_i * n_o > 0)
+      STADE_CUDA(cudaMemsetAsync(wb, 0, (size_t)(n_e * n_i * n_o) * wsize, s));
+    if (!add && xb && n_s * n_i > 0)
+      STADE_CUDA(cudaMemsetAsync(xb, 0, (size_t)(n_s * n_i) * dtype_size(dtype), s));
+    if (consumes(opts) && yb && n_s * n_o > 0)
+      STADE_CUDA(cudaMemsetAsync(yb, 0, (size_t)(n_s * n_o) * dtype_size(dtype), s));
+    return STADE_OK;
+  }
+  STADE_REQUIRE(yb && off && (!xb || w) && (!wb || x), "expert_mm_b: null array argument");
+  void* ws = nullptr;
+  st = get_workspace(opts, stade_expert_mm_b_workspace(dtype, n_s, n_e, n_i, n_o), &ws);
+  if (st != STADE_OK) return st;
+  PhaseScope ph("expert_mm_b", s);
+  Plan p;
+  st = make_plan(off, n_s, n_e, ws, &p, s);
+  if (st != STADE_OK) return st;
+  st = with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (xb) {
+      const dim3 grid((unsigned)max_tiles(n_s, n_e, kTile), ceil_div_u(n_i, kTile));
+      expert_rows_kernel<T><<<grid, 256, 0, s>>>((const T*)yb, (const T*)w, (T*)xb, p.tiles,
+                                                 p.count, n_i, n_o, true, add);
+      STADE_CHECK_LAUNCH();
+    }
+    if (wb) {
+      const dim3 grid(ceil_div_u(n_o, kTile), ceil_div_u(n_i, kTile), (unsigned)n_e);
+      expert_wgrad_kernel<T><<<grid, 256, 0, s>>>((const T*)x, (const T*)yb, (acc_t<T>*)wb,
+                                                  p.bounds, n_i, n_o, add);
+      STADE_CHECK_LAUNCH();
+    }
+    return (stade_status)STADE_OK;
+  });
+  if (st != STADE_OK) return st;
+  if (consumes(opts))
+    STADE_CUDA(cudaMemsetAsync(yb, 0, (size_t)n_s * n_o * dtype_size(dtype), s));
+  return STADE_OK;
+}

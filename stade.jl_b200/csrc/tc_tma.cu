@@ -1169,6 +1169,8 @@ int tma_take_error() {
 namespace stade {
 int conv_tc_take_error();
 int heat_take_error();
+int embed_take_error();
+int expert_take_error();
 
 namespace {
 __device__ int g_wait_check_out = 0;
@@ -1204,11 +1206,14 @@ extern "C" stade_status stade_check_bounded_wait(int64_t wait_cycles, const stad
 
 // The library's device error word: set when a bounded wait inside a
 // tensor-core kernel ran out (the kernel then skipped its remaining work and
-// returned). Reading clears it.
+// returned), or when a token-model operator met an id or a group bound that
+// is out of range. Reading clears it.
 extern "C" int stade_device_error(void) {
   const int t = stade::tma_take_error();
   const int c = stade::conv_tc_take_error();
   const int h = stade::heat_take_error();
-  if (t < 0 || c < 0 || h < 0) return -1;
-  return t | c | h;
+  const int e = stade::embed_take_error();
+  const int x = stade::expert_take_error();
+  if (t < 0 || c < 0 || h < 0 || e < 0 || x < 0) return -1;
+  return t | c | h | e | x;
 }

@@ -10,3 +10,8 @@ from .kernels import (  # noqa: F401
     affine_ls_d_cuda, mlp2_ce_d_cuda, heat2d_d_cuda, conv1d_relu_mse_d_cuda,
     kernel_launches, reset_kernel_launches,
 )
+from .token_ops import (  # noqa: F401
+    embed_cuda, embed_b_cuda, layer_norm_cuda, layer_norm_b_cuda,
+    tape8_push_cuda, tape8_pop_cuda, act_tape8_cuda, act_tape8_b_cuda, initstacks_tape8_cuda,
+    expert_mm_cuda, expert_mm_b_cuda,
+)

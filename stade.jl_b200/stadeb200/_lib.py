@@ -19,8 +19,12 @@ STADE_ETIMEDOUT = 4
 STADE_ENOTSUP = 5
 STADE_EREPLICA = 6
 STADE_HOST_SCALARS = 0x1
+STADE_ADJ_STORE = 0x2
+STADE_SEED_KEEP = 0x4
 STADE_F32 = 0
 STADE_F64 = 1
+STADE_BF16 = 2
+STADE_F16 = 3
 
 _STATUS_NAMES = {
     0: "STADE_OK", 1: "STADE_EINVAL", 2: "STADE_ECUDA", 3: "STADE_ENCCL",
@@ -118,6 +122,21 @@ SIGNATURES = {
     "stade_mlp2_ce_hv_allreduce_reduced_f64": (ST, [P, P, C.c_void_p, OPTS]),
     "stade_mlp2_ce_hv_check_replicas_f64": (ST, [P] * 10 + [I64] * 3 + [
         C.c_void_p, C.POINTER(C.c_uint64), OPTS]),
+    "stade_embed": (ST, [C.c_int, P, P, P, D] + [I64] * 4 + [OPTS]),
+    "stade_embed_b_workspace": (C.c_size_t, [I64] * 3),
+    "stade_embed_b": (ST, [C.c_int, P, P, P, D] + [I64] * 4 + [OPTS]),
+    "stade_layer_norm": (ST, [C.c_int] + [P] * 6 + [D, I64, I64, OPTS]),
+    "stade_layer_norm_b_workspace": (C.c_size_t, [C.c_int, I64, I64]),
+    "stade_layer_norm_b": (ST, [C.c_int] + [P] * 8 + [I64, I64, OPTS]),
+    "stade_initstacks_tape8": (I64, [I64, I64]),
+    "stade_tape8_push": (ST, [C.c_int] + [P] * 3 + [I64, I64, OPTS]),
+    "stade_tape8_pop": (ST, [C.c_int] + [P] * 3 + [I64, I64, OPTS]),
+    "stade_act_tape8": (ST, [C.c_int, C.c_int] + [P] * 4 + [I64, I64, OPTS]),
+    "stade_act_tape8_b": (ST, [C.c_int, C.c_int] + [P] * 4 + [I64, I64, OPTS]),
+    "stade_expert_mm_workspace": (C.c_size_t, [C.c_int] + [I64] * 4),
+    "stade_expert_mm": (ST, [C.c_int] + [P] * 4 + [I64] * 4 + [OPTS]),
+    "stade_expert_mm_b_workspace": (C.c_size_t, [C.c_int] + [I64] * 4),
+    "stade_expert_mm_b": (ST, [C.c_int] + [P] * 6 + [I64] * 4 + [OPTS]),
     "stade_fnv1a64": (C.c_uint64, [C.c_char_p]),
     "stade_fill_normal_f64": (None, [P, I64, C.c_uint64, D, D]),
     "stade_fill_normal_f32": (None, [P, I64, C.c_uint64, D, D]),
