@@ -13,6 +13,7 @@
 
 #include <initializer_list>
 
+#include "expert_tc.cuh"
 #include "token_ops.cuh"
 
 namespace stade {
@@ -20,9 +21,7 @@ namespace {
 
 __device__ int g_expert_error = 0;
 
-struct Tile {
-  int expert, row, rows, pad;   // expert < 0: rows of no group
-};
+using Tile = ExpertTile;
 
 constexpr int kTile = 64;       // rows and columns of a CUDA-core tile
 constexpr int kStep = 16;
@@ -162,27 +161,69 @@ expert_wgrad_kernel(const T* __restrict__ x, const T* __restrict__ yb, acc_t<T>*
 
 int64_t max_tiles(int64_t n_s, int64_t n_e, int tile) { return n_s / tile + n_e + 2; }
 
+// Which path a call takes. The tensor cores read 16-bit operands whose rows
+// start on 16-byte boundaries: arrays of a 16-bit type with widths that are
+// multiples of 8 as they stand, other widths and Float32 from planes that
+// expert_pack writes into the workspace. Float64, and 16-bit arrays that do
+// not start on such a boundary, go to the CUDA cores.
+bool packs(int dtype, int64_t n_i, int64_t n_o) {
+  return dtype == STADE_F32 || n_i % 8 || n_o % 8;
+}
+bool on_tensor_cores(int dtype, int64_t n_i, int64_t n_o, std::initializer_list<const void*> ptrs) {
+  if (dtype == STADE_F64) return false;
+  return packs(dtype, n_i, n_o) || row_align(16, ptrs) == 16;
+}
+int64_t pitch8(int64_t n) { return (n + 7) / 8 * 8; }
+
 struct Plan {
   int64_t* bounds;
   Tile* tiles;
   int* count;
+  uint16_t *x, *w, *yb;      // packed planes, where needed
 };
-size_t plan_bytes(int64_t n_s, int64_t n_e) {
+// S: Sizer or Carver
+template <class S>
+Plan layout(S& z, int dtype, int64_t n_s, int64_t n_e, int64_t n_i, int64_t n_o, bool reverse) {
+  Plan p{};
+  auto take = [&](auto** to, size_t n) {
+    using E = std::remove_pointer_t<std::remove_pointer_t<decltype(to)>>;
+    if constexpr (std::is_same<S, Sizer>::value) z.template take<E>(n);
+    else *to = z.template take<E>(n);
+  };
+  take(&p.bounds, n_e + 1);
+  take(&p.tiles, max_tiles(n_s, n_e, kTile));
+  take(&p.count, 1);
+  if (dtype != STADE_F64 && packs(dtype, n_i, n_o)) {
+    const int64_t np = expert_planes(dtype);
+    take(&p.x, np * n_s * pitch8(n_i));
+    take(&p.w, np * n_e * n_i * pitch8(n_o));
+    if (reverse) take(&p.yb, np * n_s * pitch8(n_o));
+  }
+  return p;
+}
+size_t plan_bytes(int dtype, int64_t n_s, int64_t n_e, int64_t n_i, int64_t n_o, bool reverse) {
+  if (n_s <= 0 || n_e < 0 || n_i < 0 || n_o < 0) return 0;
   Sizer z;
-  z.take<int64_t>(n_e + 1);
-  z.take<Tile>(max_tiles(n_s, n_e, kTile));
-  z.take<int>(1);
+  layout(z, dtype, n_s, n_e, n_i, n_o, reverse);
   return z.bytes();
 }
-stade_status make_plan(const int64_t* off, int64_t n_s, int64_t n_e, void* ws, Plan* p,
+stade_status make_plan(const Plan& p, const int64_t* off, int64_t n_s, int64_t n_e, int tile,
                        cudaStream_t s) {
-  Carver c(ws);
-  p->bounds = c.take<int64_t>(n_e + 1);
-  p->tiles = c.take<Tile>(max_tiles(n_s, n_e, kTile));
-  p->count = c.take<int>(1);
-  plan_kernel<<<1, 1024, 0, s>>>(off, n_s, n_e, kTile, p->bounds, p->tiles, p->count);
+  plan_kernel<<<1, 1024, 0, s>>>(off, n_s, n_e, tile, p.bounds, p.tiles, p.count);
   STADE_CHECK_LAUNCH();
   return STADE_OK;
+}
+
+// An operand for the tensor cores: d2 x d1 rows of d0 values, packed into
+// `planes` first where the call packs.
+stade_status operand(int dtype, const void* a, uint16_t* planes, int64_t d0, int64_t d1, int64_t d2,
+                     ExpertOperand* out, cudaStream_t s) {
+  if (!planes) {
+    *out = ExpertOperand{a, d0, d1, d2, d0};
+    return STADE_OK;
+  }
+  *out = ExpertOperand{planes, d0, d1, d2 * expert_planes(dtype), pitch8(d0)};
+  return expert_pack(dtype, a, planes, d1 * d2, d0, pitch8(d0), s);
 }
 
 stade_status check_sizes(const char* who, int dtype, int64_t n_s, int64_t n_e, int64_t n_i,
@@ -204,7 +245,8 @@ int expert_take_error() {
   const int zero = 0;
   if (cudaMemcpyFromSymbol(&host, g_expert_error, sizeof(int)) != cudaSuccess) return -1;
   if (host) cudaMemcpyToSymbol(g_expert_error, &zero, sizeof(int));
-  return host;
+  const int tc = expert_tc_take_error();
+  return tc < 0 ? -1 : host | tc;
 }
 
 }  // namespace stade
@@ -213,9 +255,7 @@ using namespace stade;
 
 extern "C" size_t stade_expert_mm_workspace(int dtype, int64_t n_s, int64_t n_e, int64_t n_i,
                                             int64_t n_o) {
-  (void)dtype;
-  if (n_s <= 0 || n_e < 0 || n_i < 0 || n_o < 0) return 0;
-  return plan_bytes(n_s, n_e);
+  return plan_bytes(dtype, n_s, n_e, n_i, n_o, false);
 }
 
 extern "C" stade_status stade_expert_mm(int dtype, const void* x, const void* w, void* y,
@@ -235,9 +275,19 @@ extern "C" stade_status stade_expert_mm(int dtype, const void* x, const void* w,
   st = get_workspace(opts, stade_expert_mm_workspace(dtype, n_s, n_e, n_i, n_o), &ws);
   if (st != STADE_OK) return st;
   PhaseScope ph("expert_mm", s);
-  Plan p;
-  st = make_plan(off, n_s, n_e, ws, &p, s);
+  Carver c(ws);
+  const Plan p = layout(c, dtype, n_s, n_e, n_i, n_o, false);
+  const bool tc = on_tensor_cores(dtype, n_i, n_o, {x, w});
+  st = make_plan(p, off, n_s, n_e, tc ? kExpertTcRows : kTile, s);
   if (st != STADE_OK) return st;
+  if (tc) {
+    ExpertOperand xo, wo;
+    st = operand(dtype, x, p.x, n_i, n_s, 1, &xo, s);
+    if (st == STADE_OK) st = operand(dtype, w, p.w, n_o, n_i, n_e, &wo, s);
+    if (st != STADE_OK) return st;
+    return expert_tc_rows(dtype, xo, wo, y, p.tiles, p.count, max_tiles(n_s, n_e, kExpertTcRows),
+                          n_i, n_o, false, false, s);
+  }
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     const dim3 grid((unsigned)max_tiles(n_s, n_e, kTile), ceil_div_u(n_o, kTile));
@@ -250,7 +300,7 @@ extern "C" stade_status stade_expert_mm(int dtype, const void* x, const void* w,
 
 extern "C" size_t stade_expert_mm_b_workspace(int dtype, int64_t n_s, int64_t n_e, int64_t n_i,
                                               int64_t n_o) {
-  return stade_expert_mm_workspace(dtype, n_s, n_e, n_i, n_o);
+  return plan_bytes(dtype, n_s, n_e, n_i, n_o, true);
 }
 
 extern "C" stade_status stade_expert_mm_b(int dtype, const void* x, void* xb, const void* w,
@@ -276,10 +326,27 @@ extern "C" stade_status stade_expert_mm_b(int dtype, const void* x, void* xb, co
   st = get_workspace(opts, stade_expert_mm_b_workspace(dtype, n_s, n_e, n_i, n_o), &ws);
   if (st != STADE_OK) return st;
   PhaseScope ph("expert_mm_b", s);
-  Plan p;
-  st = make_plan(off, n_s, n_e, ws, &p, s);
+  Carver c(ws);
+  const Plan p = layout(c, dtype, n_s, n_e, n_i, n_o, true);
+  const bool tc = on_tensor_cores(dtype, n_i, n_o, {wb ? x : yb, xb ? w : yb, yb});
+  st = make_plan(p, off, n_s, n_e, tc ? kExpertTcRows : kTile, s);
   if (st != STADE_OK) return st;
-  st = with_dtype(dtype, [&](auto t) {
+  if (tc) {
+    ExpertOperand xo, wo, yo;
+    st = operand(dtype, yb, p.yb, n_o, n_s, 1, &yo, s);
+    if (st == STADE_OK && xb) {
+      st = operand(dtype, w, p.w, n_o, n_i, n_e, &wo, s);
+      if (st == STADE_OK)
+        st = expert_tc_rows(dtype, yo, wo, xb, p.tiles, p.count,
+                            max_tiles(n_s, n_e, kExpertTcRows), n_i, n_o, true, add, s);
+    }
+    if (st == STADE_OK && wb) {
+      st = operand(dtype, x, p.x, n_i, n_s, 1, &xo, s);
+      if (st == STADE_OK)
+        st = expert_tc_wgrad(dtype, xo, yo, (float*)wb, p.bounds, n_e, n_i, n_o, add, s);
+    }
+  } else
+    st = with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     if (xb) {
       const dim3 grid((unsigned)max_tiles(n_s, n_e, kTile), ceil_div_u(n_i, kTile));

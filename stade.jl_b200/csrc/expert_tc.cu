@@ -1,0 +1,553 @@
+// Products grouped by expert on the tensor cores.
+//
+// One kernel, tcgen05.mma.cta_group::2 on 256 x 256 tiles, serves the three
+// products of expert_mm and expert_mm_b. The MMA's M dimension (256 rows over
+// the pair) is always the output's contiguous dimension and its N dimension
+// the output's rows:
+//
+//               M         N              K          A (M x K)        B (N x K)
+//   y  = x W    n_o       group's rows   n_i        W[e], M-major    x, K-major
+//   xb = yb W^T n_i       group's rows   n_o        W[e], K-major    yb, K-major
+//   wb = x^T yb n_o       n_i            its rows   yb, M-major      x, N-major
+//
+// so a group's ragged end costs what its rows cost: the last tile of a group
+// issues MMAs only as wide as its rows (a multiple of 32), columns past the
+// group are never stored, and neighbours' values there touch no other column.
+// In the third product the ragged dimension is K: the last block's rows past
+// the group are set to zero in shared memory, in both operands, before the
+// MMAs read them.
+//
+// A Float32 operand is held as three bf16 planes whose sum is the value (8
+// bits of mantissa each, rounded to nearest); the product is the six plane
+// products down to 2^-16 of it, each an ordinary K loop over its two planes.
+//
+// The tensor cores' Float32 sums truncate: their error grows with the number
+// of MMAs into one accumulator, by about 2^-25 of it each. Where the result is
+// Float32 an accumulator takes at most kChain blocks of 64 before the epilogue
+// warps add it to round-to-nearest sums in registers; where it is rounded to
+// 16 bits the whole K stays in one.
+//
+// Warp roles per CTA: 0 TMA loads, 1 (of the leader) MMAs, 2 .. 17 epilogue, 18
+// zeroes the K tail. Every wait is bounded; one that runs out sets the device
+// error word and the kernel leaves.
+
+#include <algorithm>
+
+#include "expert_tc.cuh"
+#include "tcgen05.cuh"
+#include "token_ops.cuh"
+
+namespace stade {
+namespace {
+
+__device__ int g_expert_tc_error = 0;
+
+using tc5::mbar_arrive;
+using tc5::mbar_arrive_tx;
+using tc5::mbar_init;
+using tc5::smem_u32;
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
+  return tc5::mbar_wait_cluster(bar, parity, &g_expert_tc_error);
+}
+
+constexpr int kTileN = kExpertTcRows;            // output rows of a tile
+constexpr int kHalfM = 128;                      // M rows of one CTA of the pair
+constexpr int kBlockK = 64;
+constexpr int kTileBytes = 128 * kBlockK * 2;    // one operand tile of one CTA
+constexpr int kStageBytes = 2 * kTileBytes;
+constexpr int kStages = 6;
+constexpr int kAcc = 2;                          // TMEM accumulators of kTileN columns
+constexpr int kEpiWarps = 16;
+constexpr int kThreads = (3 + kEpiWarps) * 32;
+constexpr int kBars = 3 * kStages + 2 * kAcc + 1;
+constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
+static_assert(kBars * 8 + 4 <= 256, "barrier block");
+constexpr int kChain = 4;        // K blocks of 64 per accumulator, Float32 results
+constexpr int kChainSmall = 64;  // the same for the plane products below 2^-7 of the result
+
+struct Geom {
+  int M;           // output's contiguous extent
+  int m_tiles;
+  int N;           // wgrad: n_i
+  int n_tiles;
+  int K;           // rows product: depth
+  int planes;
+  int chain;       // K blocks per accumulator of the leading product
+  bool a_mn, b_mn, bf16, add;
+  int64_t ld;      // output row pitch
+};
+
+struct Unit {
+  int expert, row, rows;   // rows product: tile; wgrad: the group
+  int m0, n0, ncols, n_mma, nkb;
+};
+
+struct RowSrc {
+  const ExpertTile* tiles;
+  const int* count;
+  __device__ __forceinline__ int total(const Geom& g) const { return *count * g.m_tiles; }
+  __device__ __forceinline__ Unit get(int t, const Geom& g) const {
+    const int4 v = *reinterpret_cast<const int4*>(tiles + t / g.m_tiles);
+    Unit u;
+    u.expert = v.x;
+    u.row = v.y;
+    u.rows = v.z;
+    u.m0 = (t % g.m_tiles) * 2 * kHalfM;
+    u.n0 = 0;
+    u.ncols = v.z;
+    u.n_mma = (v.z + 31) / 32 * 32;
+    u.nkb = v.x < 0 ? 0 : (g.K + kBlockK - 1) / kBlockK;
+    return u;
+  }
+};
+struct GroupSrc {
+  const int64_t* bounds;
+  int n_e;
+  __device__ __forceinline__ int total(const Geom& g) const { return n_e * g.m_tiles * g.n_tiles; }
+  __device__ __forceinline__ Unit get(int t, const Geom& g) const {
+    const int per = g.m_tiles * g.n_tiles;
+    Unit u;
+    u.expert = t / per;
+    const int r = t % per;
+    u.m0 = (r % g.m_tiles) * 2 * kHalfM;
+    u.n0 = (r / g.m_tiles) * kTileN;
+    const int64_t a = bounds[u.expert], b = bounds[u.expert + 1];
+    u.row = (int)a;
+    u.rows = (int)(b - a);
+    u.ncols = min(kTileN, g.N - u.n0);
+    u.n_mma = (u.ncols + 31) / 32 * 32;
+    u.nkb = (u.rows + kBlockK - 1) / kBlockK;
+    return u;
+  }
+};
+
+// The K loop of a unit: `small` blocks of the minor plane products, then nkb
+// of the leading one, cut into accumulation chains.
+struct Loop {
+  int nkb, small, n_small, n_lead;
+  __device__ __forceinline__ Loop(int nkb_, const Geom& g) : nkb(nkb_) {
+    small = g.planes == 3 ? 5 * nkb : 0;
+    n_small = (small + kChainSmall - 1) / kChainSmall;
+    n_lead = (nkb + g.chain - 1) / g.chain;
+  }
+  __device__ __forceinline__ int blocks() const { return small + nkb; }
+  __device__ __forceinline__ int chains() const { return max(1, n_small + n_lead); }
+  __device__ __forceinline__ void chain(int c, const Geom& g, int* v0, int* v1) const {
+    if (c < n_small) {
+      *v0 = c * kChainSmall;
+      *v1 = min(small, *v0 + kChainSmall);
+    } else {
+      *v0 = small + (c - n_small) * g.chain;
+      *v1 = min(small + nkb, *v0 + g.chain);
+    }
+  }
+  // block v: K block and the planes of A and B
+  __device__ __forceinline__ void block(int v, int* kb, int* pa, int* pb) const {
+    if (v >= small) {
+      *kb = v - small;
+      *pa = *pb = 0;
+      return;
+    }
+    *kb = v / 5;
+    const int p = v - *kb * 5;           // (0,2) (1,1) (2,0) (0,1) (1,0)
+    *pa = p == 1 || p == 4 ? 1 : p == 2 ? 2 : 0;
+    *pb = p == 1 || p == 3 ? 1 : p == 0 ? 2 : 0;
+  }
+};
+
+template <bool WGRAD, class Src, class Out>
+__global__ void __launch_bounds__(kThreads, 1)
+expert_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+                 const __grid_constant__ CUtensorMap bmap16, Geom g, Src src, Out* __restrict__ out,
+                 int n_e) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+  uint8_t* tiles = smem_raw + pad;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tiles + kStages * kStageBytes);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kStages;
+  const uint32_t tail0 = empty0 + 8 * kStages;      // K tail landed in this CTA
+  const uint32_t tfull0 = tail0 + 8 * kStages, tempty0 = tfull0 + 8 * kAcc;
+  const uint32_t done = tempty0 + 8 * kAcc;
+  const uint32_t rank = tc5::cluster_rank();
+  const bool leader = rank == 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full0 + 8 * s, 2);      // one arrival per CTA
+      mbar_init(empty0 + 8 * s, 1);
+      mbar_init(tail0 + 8 * s, 1);
+    }
+    for (int b = 0; b < kAcc; ++b) {
+      mbar_init(tfull0 + 8 * b, 1);
+      mbar_init(tempty0 + 8 * b, 2 * kEpiWarps);
+    }
+    mbar_init(done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tc5::tmem_alloc_pair(smem_u32(tmem_slot), 512);
+  tc5::fence_before();
+  tc5::cluster_sync();
+  tc5::fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int total = src.total(g);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---- TMA loads (both CTAs) ------------------------------------------------
+      int i = 0;
+      bool ok = true;
+      Unit u;
+      if (pair < total) u = src.get(pair, g);
+      for (int t = pair; t < total && ok; t += npairs) {
+        Unit next = u;
+        if (t + npairs < total) next = src.get(t + npairs, g);   // in flight during this unit
+        const Loop lp(u.nkb, g);
+        const int m0 = u.m0 + (int)rank * kHalfM;
+        const int half = u.n_mma / 2;
+        const int b0 = (WGRAD ? u.n0 : u.row) + (int)rank * half;
+        const int bboxes = WGRAD ? (half + 63) / 64 : half == 128 ? 1 : half / 16;
+        const uint32_t bytes =
+            kTileBytes + (WGRAD ? (uint32_t)bboxes * 8192u : (uint32_t)half * 128u);
+        for (int v = 0; v < lp.blocks(); ++v, ++i) {
+          const int s = i % kStages;
+          if (!wait(empty0 + 8 * s, ((uint32_t)(i / kStages) & 1u) ^ 1u)) { ok = false; break; }
+          int kb, pa, pb;
+          lp.block(v, &kb, &pa, &pb);
+          const int k0 = kb * kBlockK;
+          const uint32_t sa = smem_u32(tiles + s * kStageBytes), sb = sa + kTileBytes;
+          if (WGRAD && k0 + kBlockK > u.rows) {
+            // the group's K tail: landed here first, its rows past the group
+            // zeroed by warp 18, which then arrives on `full`
+            const uint32_t tb = tail0 + 8 * s;
+            mbar_arrive_tx(tb, bytes);
+            tc5::tma_load_3d(sa, &amap, m0, u.row + k0, pa, tb);
+            tc5::tma_load_3d(sa + 8192, &amap, m0 + 64, u.row + k0, pa, tb);
+            for (int q = 0; q < bboxes; ++q)
+              tc5::tma_load_3d(sb + q * 8192, &bmap, b0 + 64 * q, u.row + k0, pb, tb);
+            continue;
+          }
+          const uint32_t fb = full0 + 8 * s;
+          if (leader) mbar_arrive_tx(fb, 2 * bytes);
+          else tc5::mbar_arrive_remote(tc5::mapa(fb, 0));
+          if (WGRAD) {
+            tc5::tma_load_3d_pair(sa, &amap, m0, u.row + k0, pa, fb);
+            tc5::tma_load_3d_pair(sa + 8192, &amap, m0 + 64, u.row + k0, pa, fb);
+            for (int q = 0; q < bboxes; ++q)
+              tc5::tma_load_3d_pair(sb + q * 8192, &bmap, b0 + 64 * q, u.row + k0, pb, fb);
+          } else {
+            const int we = pa * n_e + u.expert;
+            if (g.a_mn) {
+              tc5::tma_load_3d_pair(sa, &amap, m0, k0, we, fb);
+              tc5::tma_load_3d_pair(sa + 8192, &amap, m0 + 64, k0, we, fb);
+            } else {
+              tc5::tma_load_3d_pair(sa, &amap, k0, m0, we, fb);
+            }
+            if (half == 128) {
+              tc5::tma_load_3d_pair(sb, &bmap, k0, b0, pb, fb);
+            } else {
+              for (int q = 0; q < bboxes; ++q)
+                tc5::tma_load_3d_pair(sb + q * 2048, &bmap16, k0, b0 + 16 * q, pb, fb);
+            }
+          }
+        }
+        u = next;
+      }
+      // this CTA's copies land before it leaves: the leader sees them on its
+      // own barriers, the peer when the leader's MMAs have read them
+      for (int j = 0; j < kStages && j < i; ++j) {
+        const int last = i - 1 - j;
+        wait((leader ? full0 : empty0) + 8 * (last % kStages), (uint32_t)(last / kStages) & 1u);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      // ---- MMAs --------------------------------------------------------------------
+      const uint32_t a_lbo = g.a_mn ? 8192u : 16u, b_lbo = g.b_mn ? 8192u : 16u;
+      const uint32_t a_step = g.a_mn ? 2048u : 32u, b_step = g.b_mn ? 2048u : 32u;
+      int i = 0, c_all = 0;
+      bool ok = true;
+      Unit u;
+      if (pair < total) u = src.get(pair, g);
+      for (int t = pair; t < total && ok; t += npairs) {
+        Unit next = u;
+        if (t + npairs < total) next = src.get(t + npairs, g);
+        const Loop lp(u.nkb, g);
+        const uint32_t idesc = tc5::idesc_f16(2 * kHalfM, u.n_mma, g.bf16, g.a_mn, g.b_mn);
+        for (int c = 0; c < lp.chains() && ok; ++c, ++c_all) {
+          const int b = c_all % kAcc;
+          const uint32_t acc = tmem + (uint32_t)(b * kTileN);
+          if (!wait(tempty0 + 8 * b, ((uint32_t)(c_all / kAcc) & 1u) ^ 1u)) { ok = false; break; }
+          tc5::fence_after();
+          int v0, v1;
+          lp.chain(c, g, &v0, &v1);
+          for (int v = v0; v < v1; ++v, ++i) {
+            const int s = i % kStages;
+            if (!wait(full0 + 8 * s, (uint32_t)(i / kStages) & 1u)) { ok = false; break; }
+            tc5::fence_after();
+            const uint32_t sa = smem_u32(tiles + s * kStageBytes), sb = sa + kTileBytes;
+            int steps = kBlockK / 16;
+            if (WGRAD) {
+              int kb, pa, pb;
+              lp.block(v, &kb, &pa, &pb);
+              steps = min(steps, (u.rows - kb * kBlockK + 15) / 16);
+            }
+            for (int j = 0; j < steps; ++j)
+              tc5::mma_f16_pair(acc, tc5::desc_sw128(sa + a_step * j, a_lbo, 1024u, 2u),
+                                tc5::desc_sw128(sb + b_step * j, b_lbo, 1024u, 2u), idesc,
+                                v != v0 || j != 0 ? 1u : 0u);
+            tc5::mma_commit_pair(empty0 + 8 * s);
+          }
+          tc5::mma_commit_pair(tfull0 + 8 * b);
+        }
+        u = next;
+      }
+      tc5::mma_commit_pair(done);
+    }
+    if (lane == 0) wait(done, 0);
+    __syncwarp();
+  } else if (warp == 2 + kEpiWarps) {
+    if (WGRAD) {
+      // ---- K tails (both CTAs) ---------------------------------------------------------
+      int i = 0;
+      uint32_t seen = 0;     // per stage: parity of its next tail
+      bool ok = true;
+      for (int t = pair; t < total && ok; t += npairs) {
+        const Unit u = src.get(t, g);
+        const Loop lp(u.nkb, g);
+        if (u.rows % kBlockK == 0) {
+          i += lp.blocks();
+          continue;
+        }
+        const int half = u.n_mma / 2, bboxes = (half + 63) / 64;
+        const int rem = u.rows % kBlockK, upto = (rem + 15) / 16 * 16;
+        for (int v = 0; v < lp.blocks(); ++v, ++i) {
+          int kb, pa, pb;
+          lp.block(v, &kb, &pa, &pb);
+          if (kb != u.nkb - 1) continue;
+          const int s = i % kStages;
+          ok = __all_sync(0xffffffffu, wait(tail0 + 8 * s, (seen >> s) & 1u));
+          if (!ok) break;
+          seen ^= 1u << s;
+          uint8_t* st = tiles + s * kStageBytes;
+          const int lines = (upto - rem) * (2 + bboxes);
+          for (int l = lane; l < lines * 8; l += 32) {
+            const int line = l >> 3, box = line % (2 + bboxes), row = rem + line / (2 + bboxes);
+            uint8_t* base = box < 2 ? st + box * 8192 : st + kTileBytes + (box - 2) * 8192;
+            *reinterpret_cast<int4*>(base + row * 128 + (l & 7) * 16) = make_int4(0, 0, 0, 0);
+          }
+          tc5::fence_async_smem();
+          __syncwarp();
+          if (lane == 0) tc5::mbar_arrive_remote(tc5::mapa(full0 + 8 * s, 0));
+        }
+      }
+    }
+  } else {
+    // ---- epilogue (both CTAs) ---------------------------------------------------------
+    const int e = warp - 2;
+    const int quad = warp & 3;       // TMEM lanes 32 quad ..
+    const int cg = e >> 2;           // 16-column groups cg, cg + 4, cg + 8, cg + 12
+    const uint32_t tempty_leader = tc5::mapa(tempty0, 0);
+    int c_all = 0;
+    bool ok = true;
+    Unit u;
+    if (pair < total) u = src.get(pair, g);
+    for (int t = pair; t < total && ok; t += npairs) {
+      Unit next = u;
+      if (t + npairs < total) next = src.get(t + npairs, g);
+      const Loop lp(u.nkb, g);
+      float sum[4][16];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[q][j] = 0.f;
+      for (int c = 0; c < lp.chains(); ++c, ++c_all) {
+        const int b = c_all % kAcc;
+        ok = __all_sync(0xffffffffu, wait(tfull0 + 8 * b, (uint32_t)(c_all / kAcc) & 1u));
+        if (!ok) break;
+        tc5::fence_after();
+        if (u.nkb > 0) {
+          const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * kTileN);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if ((cg + 4 * q) * 16 < u.n_mma) {     // uniform over the warp
+              float v[16];
+              tc5::tmem_ld16(base + (uint32_t)((cg + 4 * q) * 16), v);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) sum[q][j] += v[j];
+            }
+          }
+        }
+        tc5::fence_before();
+        __syncwarp();
+        if (lane == 0) tc5::mbar_arrive_remote(tempty_leader + 8 * b);
+      }
+      if (!ok) break;
+      const int m = u.m0 + (int)rank * kHalfM + quad * 32 + lane;
+      if (m < g.M) {
+        const int64_t row0 = WGRAD ? (int64_t)u.expert * g.N + u.n0 : (int64_t)u.row;
+        Out* o = out + row0 * g.ld + m;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int c0 = (cg + 4 * q) * 16;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (c0 + j < u.ncols) {
+              Out* p = o + (int64_t)(c0 + j) * g.ld;
+              *p = round_to<Out>(g.add ? load_acc<Out>(*p) + sum[q][j] : sum[q][j]);
+            }
+          }
+        }
+      }
+      u = next;
+    }
+  }
+
+  tc5::fence_before();
+  __syncthreads();
+  tc5::cluster_sync();
+  if (warp == 1) {
+    tc5::fence_after();
+    tc5::tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+stade_status operand_map(CUtensorMap* m, const ExpertOperand& o, bool bf16, uint32_t b0,
+                         uint32_t b1) {
+  const int64_t dims[3] = {o.d0, o.d1, o.d2}, pitch[2] = {o.pitch, o.pitch * o.d1};
+  const uint32_t box[3] = {b0, b1, 1};
+  return tc5::make_map_16(m, o.p, bf16, dims, pitch, box);
+}
+
+template <bool WGRAD, class Src, class Out>
+stade_status launch(const ExpertOperand& A, const ExpertOperand& B, const Geom& g, const Src& src,
+                    Out* out, int n_e, int64_t units, cudaStream_t s) {
+  CUtensorMap am, bm, bm16;
+  stade_status st = operand_map(&am, A, g.bf16, 64, g.a_mn ? 64 : 128);
+  if (st == STADE_OK) st = operand_map(&bm, B, g.bf16, 64, g.b_mn ? 64 : 128);
+  if (st == STADE_OK) st = operand_map(&bm16, B, g.bf16, 64, 16);
+  if (st != STADE_OK) return st;
+  auto kern = expert_tc_kernel<WGRAD, Src, Out>;
+  STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  const int pairs = (int)std::min<int64_t>(units, tc5::sm_count() / 2);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * pairs);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  STADE_CUDA(cudaLaunchKernelEx(&cfg, kern, am, bm, bm16, g, src, out, n_e));
+  count_launch();
+  return STADE_OK;
+}
+
+// ---- operand planes ------------------------------------------------------------------
+template <class T, int NP>
+__global__ void __launch_bounds__(256)
+pack_kernel(const T* __restrict__ src, uint16_t* __restrict__ dst, int64_t rows, int64_t cols,
+            int64_t pitch) {
+  const int64_t per = pitch / 8, n = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per, c = (i % per) * 8;
+    uint16_t o[NP][8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (NP == 1) {
+        o[0][j] = c + j < cols ? *reinterpret_cast<const uint16_t*>(src + r * cols + c + j) : 0;
+      } else {
+        float v = c + j < cols ? (float)src[r * cols + c + j] : 0.f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          __nv_bfloat16 h = __float2bfloat16_rn(v);
+          // a finite value just below 2^128 rounds to infinity: cut it instead
+          if (__hisinf(h) && isfinite(v))
+            h = __ushort_as_bfloat16((unsigned short)(__float_as_uint(v) >> 16));
+          o[p][j] = __bfloat16_as_ushort(h);
+          const float f = __bfloat162float(h);
+          v = isfinite(f) ? v - f : 0.f;   // exact
+        }
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+      *reinterpret_cast<int4*>(dst + (p * rows + r) * pitch + c) =
+          *reinterpret_cast<const int4*>(o[p]);
+  }
+}
+
+}  // namespace
+
+int64_t expert_planes(int dtype) { return dtype == STADE_F32 ? 3 : 1; }
+
+stade_status expert_pack(int dtype, const void* src, void* dst, int64_t rows, int64_t cols,
+                         int64_t pitch, cudaStream_t s) {
+  const int64_t n = rows * (pitch / 8);
+  if (n == 0) return STADE_OK;
+  const unsigned blocks = (unsigned)std::min<int64_t>((n + 255) / 256, 148 * 16);
+  if (dtype == STADE_F32)
+    pack_kernel<float, 3><<<blocks, 256, 0, s>>>((const float*)src, (uint16_t*)dst, rows, cols, pitch);
+  else
+    pack_kernel<__half, 1><<<blocks, 256, 0, s>>>((const __half*)src, (uint16_t*)dst, rows, cols,
+                                                  pitch);
+  STADE_CHECK_LAUNCH();
+  return STADE_OK;
+}
+
+stade_status expert_tc_rows(int dtype, const ExpertOperand& in, const ExpertOperand& w, void* out,
+                            const ExpertTile* tiles, const int* count, int64_t max_tiles,
+                            int64_t n_i, int64_t n_o, bool trans, bool add, cudaStream_t s) {
+  Geom g = {};
+  g.M = (int)(trans ? n_i : n_o);
+  g.K = (int)(trans ? n_o : n_i);
+  g.m_tiles = (g.M + 2 * kHalfM - 1) / (2 * kHalfM);
+  g.n_tiles = 1;
+  g.planes = (int)expert_planes(dtype);
+  g.chain = dtype == STADE_F32 ? kChain : 1 << 20;
+  g.a_mn = !trans;
+  g.b_mn = false;
+  g.bf16 = dtype != STADE_F16;
+  g.add = add;
+  g.ld = g.M;
+  const int n_e = (int)(w.d2 / g.planes);
+  const RowSrc src{tiles, count};
+  const int64_t units = max_tiles * g.m_tiles;
+  if (dtype == STADE_F32) return launch<false>(w, in, g, src, (float*)out, n_e, units, s);
+  if (dtype == STADE_BF16) return launch<false>(w, in, g, src, (__nv_bfloat16*)out, n_e, units, s);
+  return launch<false>(w, in, g, src, (__half*)out, n_e, units, s);
+}
+
+stade_status expert_tc_wgrad(int dtype, const ExpertOperand& x, const ExpertOperand& yb, float* wb,
+                             const int64_t* bounds, int64_t n_e, int64_t n_i, int64_t n_o, bool add,
+                             cudaStream_t s) {
+  Geom g = {};
+  g.M = (int)n_o;
+  g.N = (int)n_i;
+  g.m_tiles = (g.M + 2 * kHalfM - 1) / (2 * kHalfM);
+  g.n_tiles = (g.N + kTileN - 1) / kTileN;
+  g.planes = (int)expert_planes(dtype);
+  g.chain = kChain;
+  g.a_mn = g.b_mn = true;
+  g.bf16 = dtype != STADE_F16;
+  g.add = add;
+  g.ld = g.M;
+  return launch<true>(yb, x, g, GroupSrc{bounds, (int)n_e}, wb, (int)n_e,
+                      n_e * g.m_tiles * g.n_tiles, s);
+}
+
+int expert_tc_take_error() {
+  int host = 0;
+  const int zero = 0;
+  if (cudaMemcpyFromSymbol(&host, g_expert_tc_error, sizeof(int)) != cudaSuccess) return -1;
+  if (host) cudaMemcpyToSymbol(g_expert_tc_error, &zero, sizeof(int));
+  return host;
+}
+
+}  // namespace stade

@@ -211,6 +211,24 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar & 0xFEFFFFFFu)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, int c0,
+                                                 int c1, int c2, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar & 0xFEFFFFFFu)
+      : "memory");
+}
+// 16-bit operands (both bf16 or both f16, by the instruction descriptor).
+__device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                             uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 __device__ __forceinline__ void mma_tf32_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
                                               uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -264,6 +282,16 @@ __host__ __device__ constexpr uint32_t idesc_tf32(int M, int N, bool a_mn, bool 
   return (1u << 4) | (2u << 7) | (2u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
          ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
+// Instruction descriptor of kind::f16 with Float32 accumulation; both operands
+// bf16 or both f16. In shared memory a 16-bit operand tile is, K-major, rows of
+// 128 bytes (64 of K), 8-row groups 1024 B apart; MN-major, rows of 128 bytes
+// (64 of M or N) per k, 8-row K groups 1024 B apart: the 128-byte swizzle of
+// 16-byte chunks (layout type 2) in both.
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool bf16, bool a_mn, bool b_mn) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) |
+         ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
+         ((uint32_t)(M >> 4) << 24);
+}
 
 // The driver's tensor-map encoder, looked up once.
 inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -304,6 +332,32 @@ inline stade_status make_map_f32(CUtensorMap* map, const float* base, int rank,
                   d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   chunk32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(STADE_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return STADE_OK;
+}
+
+// 16-bit tensor of rank 3 (dims[0] contiguous; pitches in elements of dims 1
+// and 2), 128-byte swizzle, zero fill outside.
+inline stade_status make_map_16(CUtensorMap* map, const void* base, bool bf16, const int64_t* dims,
+                                const int64_t* pitch, const uint32_t* box) {
+  auto fn = encode_fn();
+  if (!fn) return fail(STADE_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  if (reinterpret_cast<uintptr_t>(base) & 15u)
+    return fail(STADE_EINVAL, "TMA operand must be 16-byte aligned");
+  cuuint64_t d[3], st[2];
+  cuuint32_t bx[3], es[3] = {1, 1, 1};
+  for (int i = 0; i < 3; ++i) {
+    d[i] = (cuuint64_t)dims[i];
+    bx[i] = box[i];
+  }
+  for (int i = 0; i < 2; ++i) {
+    if ((pitch[i] * 2) % 16) return fail(STADE_EINVAL, "TMA operand pitch must be 16-byte aligned");
+    st[i] = (cuuint64_t)(pitch[i] * 2);
+  }
+  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void*>(base), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(STADE_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return STADE_OK;
 }
