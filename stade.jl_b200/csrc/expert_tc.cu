@@ -32,6 +32,7 @@
 // error word and the kernel leaves.
 
 #include <algorithm>
+#include <initializer_list>
 
 #include "expert_tc.cuh"
 #include "tcgen05.cuh"
@@ -59,8 +60,10 @@ constexpr int kStages = 6;
 constexpr int kAcc = 2;                          // TMEM accumulators of kTileN columns
 constexpr int kEpiWarps = 16;
 constexpr int kThreads = (3 + kEpiWarps) * 32;
-constexpr int kBars = 3 * kStages + 2 * kAcc + 1;
-constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
+constexpr int kBars = 4 * kStages + 2 * kAcc + 1;
+constexpr int kOutBytes = 2048;                  // a warp's 16 x 32 block of the output
+constexpr int kSmem = kStages * kStageBytes + 1024 + 256 + kEpiWarps * kOutBytes;
+static_assert(kSmem <= 232448, "shared memory of a CTA");
 static_assert(kBars * 8 + 4 <= 256, "barrier block");
 constexpr int kChain = 4;        // K blocks of 64 per accumulator, Float32 results
 constexpr int kChainSmall = 64;  // the same for the plane products below 2^-7 of the result
@@ -74,6 +77,7 @@ struct Geom {
   int planes;
   int chain;       // K blocks per accumulator of the leading product
   bool a_mn, b_mn, bf16, add;
+  bool vec;        // output rows in 16-byte pieces
   int64_t ld;      // output row pitch
 };
 
@@ -155,6 +159,97 @@ struct Loop {
   }
 };
 
+// ---- output -------------------------------------------------------------------
+// A warp's 32 (M) x 16 (output rows) block goes through shared memory so that
+// it reaches memory as 16-byte pieces of output rows: straight from the
+// accumulator's layout a thread has one value per output row, 16 stores of 2
+// or 4 bytes with an address and a bound each (measured, 4096 x 512 x 4096 in
+// bf16: 37.8 us with those, 27 with these). 16-bit blocks are transposed by
+// stmatrix; rows of 64 bytes, 16-byte chunks swizzled so that the eight rows
+// of a block fall into different banks. `add` adds the old values before the
+// one rounding.
+template <class Out>
+__device__ __forceinline__ void pack2(float a, float b, uint32_t* r) {
+  const Vec<Out, 2> v{{round_to<Out>(a), round_to<Out>(b)}};
+  *r = *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Copies 16-byte chunks (or, without vec, single values) between the block in
+// shared memory and output rows c0 .. of the tile, rows < ncols, M < lim.
+template <class Out, bool LOAD>
+__device__ __forceinline__ void copy_block(uint8_t* blk, Out* o, int64_t ld, int rows, int lim,
+                                           bool vec, bool add, int lane) {
+  constexpr int kPer = 16 / (int)sizeof(Out), kChunks = 32 / kPer;   // chunks of a row: 4 or 8
+  auto at = [&](int row, int ch) {
+    return blk + row * (kChunks * 16) + 16 * (sizeof(Out) == 2 ? ch ^ ((row >> 1) & 3) : ch);
+  };
+  if (vec) {
+    const int ch = lane % kChunks;
+#pragma unroll
+    for (int it = 0; it < kChunks / 2; ++it) {
+      const int row = it * (32 / kChunks) + lane / kChunks;
+      if (row < rows && ch * kPer < lim) {
+        int4* p = reinterpret_cast<int4*>(o + row * ld + ch * kPer);
+        int4* s = reinterpret_cast<int4*>(at(row, ch));
+        if (LOAD) {
+          *s = *p;
+        } else if (sizeof(Out) == 4 && add) {
+          float4 a = *reinterpret_cast<float4*>(s);
+          const float4 b = *reinterpret_cast<float4*>(p);
+          a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+          *reinterpret_cast<float4*>(p) = a;
+        } else {
+          *p = *s;
+        }
+      }
+    }
+  } else if (lane < lim) {
+#pragma unroll 1
+    for (int row = 0; row < rows && row < 16; ++row) {
+      Out* p = o + row * ld + lane;
+      Out* s = reinterpret_cast<Out*>(at(row, lane / kPer)) + lane % kPer;
+      if (LOAD) *s = *p;
+      else *p = sizeof(Out) == 4 && add ? round_to<Out>(load_acc<Out>(*s) + load_acc<Out>(*p)) : *s;
+    }
+  }
+}
+
+template <class Out>
+__device__ __forceinline__ void store_block(float (&sum)[16], uint8_t* blk, Out* o, int64_t ld,
+                                            int rows, int lim, bool vec, bool add, int lane) {
+  if constexpr (sizeof(Out) == 2) {
+    const uint32_t base = smem_u32(blk);
+    const int row = (lane & 7) + 8 * (lane >> 4), k = (lane >> 3) & 1;
+    if (add) {
+      copy_block<Out, true>(blk, o, ld, rows, lim, vec, add, lane);
+      __syncwarp();
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t a = base + row * 64 + 16 * ((2 * h + k) ^ ((row >> 1) & 3));
+      uint32_t r[4];
+      if (add) {
+        tc5::ldmatrix4_trans(a, r);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const Vec<Out, 2> v = *reinterpret_cast<const Vec<Out, 2>*>(&r[b]);
+          sum[8 * h + 2 * b] += load_acc<Out>(v.v[0]);
+          sum[8 * h + 2 * b + 1] += load_acc<Out>(v.v[1]);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) pack2<Out>(sum[8 * h + 2 * b], sum[8 * h + 2 * b + 1], &r[b]);
+      tc5::stmatrix4_trans(a, r);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) reinterpret_cast<float*>(blk)[j * 32 + lane] = sum[j];
+  }
+  __syncwarp();
+  copy_block<Out, false>(blk, o, ld, rows, lim, vec, add, lane);
+  __syncwarp();
+}
+
 template <bool WGRAD, class Src, class Out>
 __global__ void __launch_bounds__(kThreads, 1)
 expert_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
@@ -167,7 +262,8 @@ expert_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kStages;
   const uint32_t tail0 = empty0 + 8 * kStages;      // K tail landed in this CTA
-  const uint32_t tfull0 = tail0 + 8 * kStages, tempty0 = tfull0 + 8 * kAcc;
+  const uint32_t ptail0 = tail0 + 8 * kStages;      // the leader's: the peer's tail is zeroed
+  const uint32_t tfull0 = ptail0 + 8 * kStages, tempty0 = tfull0 + 8 * kAcc;
   const uint32_t done = tempty0 + 8 * kAcc;
   const uint32_t rank = tc5::cluster_rank();
   const bool leader = rank == 0;
@@ -176,9 +272,10 @@ expert_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(full0 + 8 * s, 2);      // one arrival per CTA
+      mbar_init(full0 + 8 * s, 1);
       mbar_init(empty0 + 8 * s, 1);
       mbar_init(tail0 + 8 * s, 1);
+      mbar_init(ptail0 + 8 * s, 1);
     }
     for (int b = 0; b < kAcc; ++b) {
       mbar_init(tfull0 + 8 * b, 1);
@@ -219,8 +316,8 @@ expert_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
           const int k0 = kb * kBlockK;
           const uint32_t sa = smem_u32(tiles + s * kStageBytes), sb = sa + kTileBytes;
           if (WGRAD && k0 + kBlockK > u.rows) {
-            // the group's K tail: landed here first, its rows past the group
-            // zeroed by warp 18, which then arrives on `full`
+            // the group's K tail: lands here first; warp 18 zeroes its rows past
+            // the group, and the leader's arrives on `full` for both CTAs
             const uint32_t tb = tail0 + 8 * s;
             mbar_arrive_tx(tb, bytes);
             tc5::tma_load_3d(sa, &amap, m0, u.row + k0, pa, tb);
@@ -231,7 +328,6 @@ expert_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
           }
           const uint32_t fb = full0 + 8 * s;
           if (leader) mbar_arrive_tx(fb, 2 * bytes);
-          else tc5::mbar_arrive_remote(tc5::mapa(fb, 0));
           if (WGRAD) {
             tc5::tma_load_3d_pair(sa, &amap, m0, u.row + k0, pa, fb);
             tc5::tma_load_3d_pair(sa + 8192, &amap, m0 + 64, u.row + k0, pa, fb);
@@ -340,7 +436,13 @@ expert_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
           }
           tc5::fence_async_smem();
           __syncwarp();
-          if (lane == 0) tc5::mbar_arrive_remote(tc5::mapa(full0 + 8 * s, 0));
+          if (leader) {
+            ok = __all_sync(0xffffffffu, wait(ptail0 + 8 * s, ((seen >> s) & 1u) ^ 1u));
+            if (!ok) break;
+            if (lane == 0) mbar_arrive(full0 + 8 * s);
+          } else if (lane == 0) {
+            tc5::mbar_arrive_remote(tc5::mapa(ptail0 + 8 * s, 0));
+          }
         }
       }
     }
@@ -374,7 +476,10 @@ expert_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
           for (int q = 0; q < 4; ++q) {
             if ((cg + 4 * q) * 16 < u.n_mma) {     // uniform over the warp
               float v[16];
-              tc5::tmem_ld16(base + (uint32_t)((cg + 4 * q) * 16), v);
+              if constexpr (sizeof(Out) == 2)
+                tc5::tmem_ld16_frag(base + (uint32_t)((cg + 4 * q) * 16), v);
+              else
+                tc5::tmem_ld16(base + (uint32_t)((cg + 4 * q) * 16), v);
 #pragma unroll
               for (int j = 0; j < 16; ++j) sum[q][j] += v[j];
             }
@@ -382,23 +487,19 @@ expert_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
         }
         tc5::fence_before();
         __syncwarp();
-        if (lane == 0) tc5::mbar_arrive_remote(tempty_leader + 8 * b);
+        if (lane == 0) tc5::mbar_arrive_remote_cta(tempty_leader + 8 * b);
       }
       if (!ok) break;
-      const int m = u.m0 + (int)rank * kHalfM + quad * 32 + lane;
+      const int m = u.m0 + (int)rank * kHalfM + quad * 32;
       if (m < g.M) {
         const int64_t row0 = WGRAD ? (int64_t)u.expert * g.N + u.n0 : (int64_t)u.row;
-        Out* o = out + row0 * g.ld + m;
+        uint8_t* blk = reinterpret_cast<uint8_t*>(bars) + 256 + e * kOutBytes;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int c0 = (cg + 4 * q) * 16;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (c0 + j < u.ncols) {
-              Out* p = o + (int64_t)(c0 + j) * g.ld;
-              *p = round_to<Out>(g.add ? load_acc<Out>(*p) + sum[q][j] : sum[q][j]);
-            }
-          }
+          if (c0 < u.ncols)
+            store_block<Out>(sum[q], blk, out + (row0 + c0) * g.ld + m, g.ld, u.ncols - c0,
+                             g.M - m, g.vec, g.add, lane);
         }
       }
       u = next;
@@ -516,6 +617,7 @@ stade_status expert_tc_rows(int dtype, const ExpertOperand& in, const ExpertOper
   g.bf16 = dtype != STADE_F16;
   g.add = add;
   g.ld = g.M;
+  g.vec = row_align(g.ld * dtype_size(dtype), {out}) == 16;
   const int n_e = (int)(w.d2 / g.planes);
   const RowSrc src{tiles, count};
   const int64_t units = max_tiles * g.m_tiles;
@@ -538,6 +640,7 @@ stade_status expert_tc_wgrad(int dtype, const ExpertOperand& x, const ExpertOper
   g.bf16 = dtype != STADE_F16;
   g.add = add;
   g.ld = g.M;
+  g.vec = row_align(g.ld * 4, {wb}) == 16;
   return launch<true>(yb, x, g, GroupSrc{bounds, (int)n_e}, wb, (int)n_e,
                       n_e * g.m_tiles * g.n_tiles, s);
 }
