@@ -11,20 +11,544 @@
 // the centred values in a second pass, so a mean far from zero costs nothing
 // but its own rounding.
 
+#include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
+#include "tcgen05.cuh"
 #include "token_ops.cuh"
 
 namespace stade {
 namespace {
 
+// ---- rows held in registers -----------------------------------------------------
+// Both sweeps are bound by memory: x in and y out, or x and yb in and xb out,
+// each once. A row lives in the registers of a group of G threads, NV vectors
+// of VEC values each (slot j of a row belongs to thread j % G), so nothing is
+// read twice; rows too long for that go through the kernels further down,
+// which read a row again from the caches.
+// VEC is 16 bytes where the rows allow it, 4 bytes (16-bit types), else one
+// value; short rows take narrower vectors so that a warp's lanes all have
+// work.
+//
+// Long rows that start on 16-byte boundaries take the ring kernels: one block
+// holds a row, the rows to come are copied by cp.async.bulk into a ring in
+// shared memory, several rows ahead of the arithmetic, and w, b and the sums
+// over rows stay in registers for all of a block's rows.
+
+// Sums of two values over the group, the same in every thread. `red`: 2 x 2 x
+// 32 values, used alternately (`turn`), so that one barrier per sum is enough.
+template <class A>
+__device__ __forceinline__ void block_sum2(A& a, A& b, A (*red)[2][32], int turn, int warps) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  a = warp_sum(a);
+  b = warp_sum(b);
+  if (lane == 0) {
+    red[turn][0][warp] = a;
+    red[turn][1][warp] = b;
+  }
+  __syncthreads();
+  a = warp_sum(lane < warps ? red[turn][0][lane] : A(0));
+  b = warp_sum(lane < warps ? red[turn][1][lane] : A(0));
+}
+template <int G, class A>
+__device__ __forceinline__ void group_sum2(A& a, A& b, A (*red)[2][32], int turn) {
+  if constexpr (G > 32) {
+    block_sum2(a, b, red, turn, G / 32);
+  } else {
+    a = warp_sum(a);
+    b = warp_sum(b);
+  }
+}
+
+template <int G> constexpr int rows_per_block() { return G == 32 ? 4 : 1; }
+
+template <class T, int VEC, int G, int NV>
+__global__ void __launch_bounds__(G * rows_per_block<G>())
+ln_fwd_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
+              const acc_t<T>* __restrict__ b, T* __restrict__ y, acc_t<T>* __restrict__ m_stack,
+              acc_t<T>* __restrict__ r_stack, double eps, int64_t n_s, int n_d) {
+  using A = acc_t<T>;
+  __shared__ A red[2][2][32];
+  const int t = threadIdx.x % G;
+  const int64_t s = (int64_t)blockIdx.x * rows_per_block<G>() + threadIdx.x / G;
+  if (s >= n_s) return;                       // whole warps, and then G == 32
+  const int slots = n_d / VEC;
+  const T* xr = x + s * n_d;
+  Vec<T, VEC> raw[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i * G + t < slots) raw[i] = reinterpret_cast<const Vec<T, VEC>*>(xr)[i * G + t];
+  A sum = 0, zero = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i * G + t < slots)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) sum += load_acc<T>(raw[i].v[k]);
+  group_sum2<G>(sum, zero, red, 0);
+  const A mean = sum / (A)n_d;
+  A sq = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i * G + t < slots)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const A c = load_acc<T>(raw[i].v[k]) - mean;
+        sq += c * c;
+      }
+  group_sum2<G>(sq, zero, red, 1);
+  const A rstd = A(1) / sqrt(sq / (A)n_d + (A)eps);
+  if (t == 0) {
+    m_stack[s] = mean;
+    r_stack[s] = rstd;
+  }
+  T* yr = y + s * n_d;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i * G + t < slots) {
+      const int d = (i * G + t) * VEC;
+      A o[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        o[k] = (load_acc<T>(raw[i].v[k]) - mean) * rstd * (w ? __ldg(w + d + k) : A(1)) +
+               (b ? __ldg(b + d + k) : A(0));
+      store_vec<T, VEC>(yr + d, o);
+    }
+}
+
+// The reverse sweep. Blocks walk the rows at a stride of the grid; a thread
+// keeps its columns of w and of the two sums over rows in registers, and the
+// next row's loads are issued before the current row's sums. Per block one
+// partial of each sum, added up in block order by ln_finish_kernel.
+struct BwdArgs {
+  const void *x, *w, *m, *r;
+  void *xb, *yb, *part;
+  int64_t n_s;
+  int n_d;
+  bool add, zero, sums;
+};
+
+template <class T, int VEC, int G, int NV>
+__global__ void __launch_bounds__(G * rows_per_block<G>())
+ln_bwd_kernel(BwdArgs p) {
+  using A = acc_t<T>;
+  constexpr int R = rows_per_block<G>();
+  using V = Vec<T, VEC>;
+  __shared__ A red[2][2][32];
+  const int t = threadIdx.x % G, slots = p.n_d / VEC;
+  const V* x = (const V*)p.x;
+  V* yb = (V*)p.yb;
+  const A* m = (const A*)p.m;
+  const A* r = (const A*)p.r;
+  A w[NV][VEC], sw[NV][VEC], sb[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      w[i][k] = p.w && i * G + t < slots ? ((const A*)p.w)[(i * G + t) * VEC + k] : A(1);
+      sw[i][k] = sb[i][k] = A(0);
+    }
+  const int64_t step = (int64_t)gridDim.x * R;
+  int64_t s = (int64_t)blockIdx.x * R + threadIdx.x / G;
+  V nx[NV], ny[NV];
+  A nm = 0, nr = 0;
+  auto fetch = [&](int64_t q) {
+    if (q >= p.n_s) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i * G + t < slots) {
+        nx[i] = x[q * slots + i * G + t];
+        ny[i] = yb[q * slots + i * G + t];
+      }
+    nm = m[q];
+    nr = r[q];
+  };
+  fetch(s);
+  int turn = 0;
+  for (; s < p.n_s; s += step) {      // the same count for all threads of a group
+    V cx[NV], cy[NV];
+    const A mean = nm, rstd = nr;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) cx[i] = nx[i], cy[i] = ny[i];
+    fetch(s + step);
+    A sg = 0, sgh = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i * G + t < slots)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const A h = (load_acc<T>(cx[i].v[k]) - mean) * rstd, v = load_acc<T>(cy[i].v[k]);
+          const A g = v * w[i][k];
+          sg += g;
+          sgh += g * h;
+          sw[i][k] += v * h;
+          sb[i][k] += v;
+        }
+    if (p.xb) {
+      group_sum2<G>(sg, sgh, red, turn);
+      turn ^= 1;
+      const A mg = sg / (A)p.n_d, mgh = sgh / (A)p.n_d;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (i * G + t < slots) {
+          T* o = (T*)p.xb + (s * slots + i * G + t) * VEC;
+          A out[VEC], old[VEC];
+          if (p.add) load_vec<T, VEC>(o, old);
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            const A h = (load_acc<T>(cx[i].v[k]) - mean) * rstd;
+            const A g = load_acc<T>(cy[i].v[k]) * w[i][k];
+            out[k] = rstd * (g - mg - h * mgh);
+            if (p.add) out[k] += old[k];
+          }
+          store_vec<T, VEC>(o, out);
+        }
+    }
+    if (p.zero)
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (i * G + t < slots)
+          store_zero<T, VEC>((T*)p.yb + (s * slots + i * G + t) * VEC);
+  }
+  if (!p.sums) return;
+  A* part = (A*)p.part + (int64_t)blockIdx.x * 2 * p.n_d;
+  if constexpr (R > 1) {
+    // the block's warps, added in order
+    extern __shared__ char sm_raw[];
+    A* sm = reinterpret_cast<A*>(sm_raw);       // 2 x n_d
+    for (int q = 0; q < R; ++q) {
+      if ((int)threadIdx.x / G == q)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (i * G + t < slots)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+              const int d = (i * G + t) * VEC + k;
+              sm[d] = q ? sm[d] + sw[i][k] : sw[i][k];
+              sm[p.n_d + d] = q ? sm[p.n_d + d] + sb[i][k] : sb[i][k];
+            }
+      __syncthreads();
+    }
+    for (int d = threadIdx.x; d < 2 * p.n_d; d += G * R) part[d] = sm[d];
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i * G + t < slots)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          part[(i * G + t) * VEC + k] = sw[i][k];
+          part[p.n_d + (i * G + t) * VEC + k] = sb[i][k];
+        }
+  }
+}
+
+// ---- rings of rows -------------------------------------------------------------------
+__device__ int g_norm_error = 0;
+
+constexpr int kMaxStages = 8;
+
+// Sums of N values over the block, the same in every thread: within a warp by
+// halving (each step adds one half of the values to the lanes that keep it),
+// then one barrier and the warps' sums. `red`: 2 x 8 x 32 values, used
+// alternately (`turn`), so that no second barrier is needed.
+template <int N, class A>
+__device__ __forceinline__ void block_sums(A (&v)[N], A (*red)[8][32], int turn, int warps) {
+  constexpr int kLanes = 32 / N;       // lanes per value
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int n = N, off = 16;
+#pragma unroll
+  for (int step = 0; step < 5; ++step, off >>= 1) {
+    if (n > 1) {
+      n >>= 1;
+      const bool up = lane & off;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i)
+        if (i < n) {
+          const A send = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, off);
+        }
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
+    }
+  }
+  if (lane % kLanes == 0) red[turn][lane / kLanes][warp] = v[0];
+  __syncthreads();
+  A s = 0;
+  for (int w = lane % kLanes; w < warps; w += kLanes) s += red[turn][lane / kLanes][w];
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, s, i * kLanes);
+}
+
+// A stage holds R consecutive rows of up to two arrays, each copied as one
+// piece (row bytes are a multiple of 16). All of a block's threads call
+// wait(); behind a barrier that follows their last read of a stage, thread 0
+// calls issue() for the rows that reuse it. A wait that runs out sets the
+// error word and the block goes on without waiting, so that its barriers still
+// match.
+struct Ring {
+  uint8_t* data;
+  uint32_t bar0;
+  int stages, arrays;
+  uint32_t row_bytes, array_bytes;
+  bool dead;
+  __device__ __forceinline__ Ring(uint8_t* smem, int stages_, int rows, uint32_t row_bytes_,
+                                  int arrays_)
+      : data(smem + 128), bar0(tc5::smem_u32(smem)), stages(stages_), arrays(arrays_),
+        row_bytes(row_bytes_), array_bytes(rows * row_bytes_), dead(false) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < stages; ++i) tc5::mbar_init(bar0 + 8 * i, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ const uint8_t* row(int stage, int array, int r) const {
+    return data + (size_t)(stage * arrays + array) * array_bytes + (size_t)r * row_bytes;
+  }
+  // rows s .. s + rows - 1 of the arrays a and b
+  __device__ __forceinline__ void issue(int stage, const void* a, const void* b, int64_t s,
+                                        int rows) const {
+    const uint32_t bar = bar0 + 8 * stage, bytes = rows * row_bytes;
+    tc5::mbar_arrive_tx(bar, bytes * arrays);
+    tc5::bulk_load(tc5::smem_u32(row(stage, 0, 0)), (const uint8_t*)a + s * row_bytes, bytes, bar);
+    if (arrays == 2)
+      tc5::bulk_load(tc5::smem_u32(row(stage, 1, 0)), (const uint8_t*)b + s * row_bytes, bytes, bar);
+  }
+  __device__ __forceinline__ void wait(int stage, uint32_t parity) {
+    if (!dead) dead = !tc5::mbar_wait(bar0 + 8 * stage, parity, &g_norm_error);
+  }
+};
+
+// R rows a turn: what a turn costs beside its arithmetic (the wait, two
+// barriers, the shuffles) is shared by them. Measured, 8192 x 5000 f16: 71.7 us
+// with one row a turn.
+template <class T, int NV, int R>
+__global__ void __launch_bounds__(NV == 1 ? 1024 : 768)
+ln_fwd_ring_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
+                   const acc_t<T>* __restrict__ b, T* __restrict__ y,
+                   acc_t<T>* __restrict__ m_stack, acc_t<T>* __restrict__ r_stack, double eps,
+                   int64_t n_s, int n_d, int stages) {
+  using A = acc_t<T>;
+  constexpr int VEC = 16 / (int)sizeof(T);
+  using V = Vec<T, VEC>;
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ A red[2][8][32];
+  Ring ring(sm, stages, R, (uint32_t)(n_d * sizeof(T)), 1);
+  const int t = threadIdx.x, G = blockDim.x, slots = n_d / VEC, nw = G / 32;
+  A wr[NV][VEC], br[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const int j = i * G + t;
+      wr[i][k] = w && j < slots ? w[j * VEC + k] : A(1);
+      br[i][k] = b && j < slots ? b[j * VEC + k] : A(0);
+    }
+  const int64_t first = (int64_t)blockIdx.x * R, step = (int64_t)gridDim.x * R;
+  auto rows_at = [&](int64_t s) { return (int)min((int64_t)R, n_s - s); };
+  if (t == 0)
+    for (int i = 0; i < stages && first + i * step < n_s; ++i)
+      ring.issue(i, x, nullptr, first + i * step, rows_at(first + i * step));
+  int stage = 0;
+  uint32_t parity = 0;
+  for (int64_t s = first; s < n_s; s += step) {
+    const int rows = rows_at(s);
+    ring.wait(stage, parity);
+    V raw[R][NV];
+    A v[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      v[q] = 0;
+      if (q < rows) {
+        const V* row = reinterpret_cast<const V*>(ring.row(stage, 0, q));
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (i * G + t < slots) {
+            raw[q][i] = row[i * G + t];
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) v[q] += load_acc<T>(raw[q][i].v[k]);
+          }
+      }
+    }
+    block_sums<R>(v, red, 0, nw);
+    // every thread has read the stage: it takes the rows to come
+    if (t == 0 && s + stages * step < n_s)
+      ring.issue(stage, x, nullptr, s + stages * step, rows_at(s + stages * step));
+    A mean[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      mean[q] = v[q] / (A)n_d;
+      v[q] = 0;
+      if (q < rows)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (i * G + t < slots)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+              const A c = load_acc<T>(raw[q][i].v[k]) - mean[q];
+              v[q] += c * c;
+            }
+    }
+    block_sums<R>(v, red, 1, nw);
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      if (q < rows) {
+        const A rstd = A(1) / sqrt(v[q] / (A)n_d + (A)eps);
+        if (t == 0) {
+          m_stack[s + q] = mean[q];
+          r_stack[s + q] = rstd;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (i * G + t < slots) {
+            A o[VEC];
+#pragma unroll
+            for (int k = 0; k < VEC; ++k)
+              o[k] = (load_acc<T>(raw[q][i].v[k]) - mean[q]) * rstd * wr[i][k] + br[i][k];
+            store_vec<T, VEC>(y + (s + q) * n_d + (i * G + t) * VEC, o);
+          }
+      }
+    if (++stage == stages) stage = 0, parity ^= 1;
+  }
+}
+
+template <class T, int NV, int R>
+__global__ void __launch_bounds__(NV == 1 ? 1024 : 768)
+ln_bwd_ring_kernel(BwdArgs p, int stages) {
+  using A = acc_t<T>;
+  constexpr int VEC = 16 / (int)sizeof(T);
+  using V = Vec<T, VEC>;
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ A red[2][8][32];
+  Ring ring(sm, stages, R, (uint32_t)(p.n_d * sizeof(T)), 2);
+  const int t = threadIdx.x, G = blockDim.x, slots = p.n_d / VEC, nw = G / 32;
+  T* yb = (T*)p.yb;
+  const A* m = (const A*)p.m;
+  const A* r = (const A*)p.r;
+  A w[NV][VEC], sw[NV][VEC], sb[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      w[i][k] = p.w && i * G + t < slots ? ((const A*)p.w)[(i * G + t) * VEC + k] : A(1);
+      sw[i][k] = sb[i][k] = A(0);
+    }
+  const int64_t first = (int64_t)blockIdx.x * R, step = (int64_t)gridDim.x * R;
+  auto rows_at = [&](int64_t s) { return (int)min((int64_t)R, p.n_s - s); };
+  if (t == 0)
+    for (int i = 0; i < stages && first + i * step < p.n_s; ++i)
+      ring.issue(i, p.x, yb, first + i * step, rows_at(first + i * step));
+  int stage = 0, turn = 0, last = -1;
+  uint32_t parity = 0;
+  const A inv = A(1) / (A)p.n_d;
+  for (int64_t s = first; s < p.n_s; s += step) {
+    const int rows = rows_at(s);
+    A rstd[R], mr[R], v[2 * R];     // h = x rstd - mean rstd
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      rstd[q] = q < rows ? r[s + q] : A(0);
+      mr[q] = q < rows ? m[s + q] : A(0);
+      v[2 * q] = v[2 * q + 1] = A(0);
+    }
+    ring.wait(stage, parity);
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      if (q < rows) {
+        const V* xs = reinterpret_cast<const V*>(ring.row(stage, 0, q));
+        const V* ys = reinterpret_cast<const V*>(ring.row(stage, 1, q));
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (i * G + t < slots) {
+            const V cx = xs[i * G + t], cy = ys[i * G + t];
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+              const A h = (load_acc<T>(cx.v[k]) - mr[q]) * rstd[q], g = load_acc<T>(cy.v[k]);
+              const A gw = g * w[i][k];
+              v[2 * q] += gw;
+              v[2 * q + 1] += gw * h;
+              sw[i][k] += g * h;
+              sb[i][k] += g;
+            }
+          }
+      }
+    block_sums<2 * R>(v, red, turn, nw);
+    turn ^= 1;
+    // every thread is past the previous turn's stage: it takes the rows to come
+    const int64_t ahead = s + (stages - 1) * step;
+    if (t == 0 && last >= 0 && ahead < p.n_s) ring.issue(last, p.x, yb, ahead, rows_at(ahead));
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      if (q < rows) {
+        const V* xs = reinterpret_cast<const V*>(ring.row(stage, 0, q));
+        const V* ys = reinterpret_cast<const V*>(ring.row(stage, 1, q));
+        const A mg = v[2 * q] * inv, mgh = v[2 * q + 1] * inv;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (i * G + t < slots) {
+            const int64_t at = (s + q) * p.n_d + (int64_t)(i * G + t) * VEC;
+            if (p.xb) {
+              const V cx = xs[i * G + t], cy = ys[i * G + t];
+              T* o = (T*)p.xb + at;
+              A out[VEC], old[VEC];
+              if (p.add) load_vec<T, VEC>(o, old);
+#pragma unroll
+              for (int k = 0; k < VEC; ++k) {
+                const A h = (load_acc<T>(cx.v[k]) - mr[q]) * rstd[q];
+                out[k] = rstd[q] * (load_acc<T>(cy.v[k]) * w[i][k] - mg - h * mgh);
+                if (p.add) out[k] += old[k];
+              }
+              store_vec<T, VEC>(o, out);
+            }
+            if (p.zero) store_zero<T, VEC>(yb + at);
+          }
+      }
+    last = stage;
+    if (++stage == stages) stage = 0, parity ^= 1;
+  }
+  if (!p.sums) return;
+  A* part = (A*)p.part + (int64_t)blockIdx.x * 2 * p.n_d;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i * G + t < slots)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        part[(i * G + t) * VEC + k] = sw[i][k];
+        part[p.n_d + (i * G + t) * VEC + k] = sb[i][k];
+      }
+}
+
+// wb and bb from the partials [count][2][n_d]: 32 columns a block, 32 warps
+// that each add every 32nd partial, then the warps' sums in order.
+template <class A>
+__global__ void __launch_bounds__(1024)
+ln_finish_kernel(const A* __restrict__ part, int count, int64_t n_d, A* __restrict__ wb,
+                 A* __restrict__ bb, bool add) {
+  __shared__ A sm[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t d = (int64_t)blockIdx.x * 32 + lane;    // 0 .. 2 n_d - 1: wb, then bb
+  A acc = 0;
+  if (d < 2 * n_d)
+    acc = ordered_sum(part + d + (int64_t)warp * 2 * n_d, (count - warp + 31) / 32, 64 * n_d);
+  sm[warp][lane] = acc;
+  __syncthreads();
+  if (warp != 0 || d >= 2 * n_d) return;
+  A s = 0;
+#pragma unroll
+  for (int q = 0; q < 32; ++q) s += sm[q][lane];
+  A* o = d < n_d ? (wb ? wb + d : nullptr) : (bb ? bb + d - n_d : nullptr);
+  if (o) *o = add ? *o + s : s;
+}
+
+// ---- rows too long for registers ---------------------------------------------------
 constexpr int kThreads = 256;
 
 template <class T>
 __global__ void __launch_bounds__(kThreads)
-ln_fwd_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
-              const acc_t<T>* __restrict__ b, T* __restrict__ y, acc_t<T>* __restrict__ m_stack,
-              acc_t<T>* __restrict__ r_stack, double eps, int64_t n_d) {
+ln_fwd_long_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
+                   const acc_t<T>* __restrict__ b, T* __restrict__ y,
+                   acc_t<T>* __restrict__ m_stack, acc_t<T>* __restrict__ r_stack, double eps,
+                   int64_t n_d) {
   using A = acc_t<T>;
   __shared__ A red[kThreads / 32];
   const int64_t s = blockIdx.x;
@@ -50,9 +574,9 @@ ln_fwd_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
 
 template <class T>
 __global__ void __launch_bounds__(kThreads)
-ln_bwd_x_kernel(const T* __restrict__ x, T* __restrict__ xb, const acc_t<T>* __restrict__ w,
-                const T* __restrict__ yb, const acc_t<T>* __restrict__ m_stack,
-                const acc_t<T>* __restrict__ r_stack, int64_t n_d, bool add) {
+ln_bwd_x_long_kernel(const T* __restrict__ x, T* __restrict__ xb, const acc_t<T>* __restrict__ w,
+                     const T* __restrict__ yb, const acc_t<T>* __restrict__ m_stack,
+                     const acc_t<T>* __restrict__ r_stack, int64_t n_d, bool add) {
   using A = acc_t<T>;
   __shared__ A red[kThreads / 32];
   const int64_t s = blockIdx.x, o = s * n_d;
@@ -76,9 +600,10 @@ ln_bwd_x_kernel(const T* __restrict__ x, T* __restrict__ xb, const acc_t<T>* __r
 // Partial sums over a chunk of rows, one thread per column.
 template <class T>
 __global__ void __launch_bounds__(kThreads)
-ln_bwd_w_kernel(const T* __restrict__ x, T* __restrict__ yb, const acc_t<T>* __restrict__ m_stack,
-                const acc_t<T>* __restrict__ r_stack, int64_t n_s, int64_t n_d, int64_t rows,
-                acc_t<T>* __restrict__ part, bool zero) {
+ln_bwd_w_long_kernel(const T* __restrict__ x, T* __restrict__ yb,
+                     const acc_t<T>* __restrict__ m_stack, const acc_t<T>* __restrict__ r_stack,
+                     int64_t n_s, int64_t n_d, int64_t rows, acc_t<T>* __restrict__ part,
+                     bool zero) {
   using A = acc_t<T>;
   const int64_t d = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   if (d >= n_d) return;
@@ -90,36 +615,92 @@ ln_bwd_w_kernel(const T* __restrict__ x, T* __restrict__ yb, const acc_t<T>* __r
     b += v;
     if (zero) yb[s * n_d + d] = round_to<T>(A(0));
   }
-  part[(2 * blockIdx.y) * n_d + d] = w;
-  part[(2 * blockIdx.y + 1) * n_d + d] = b;
+  part[(2 * (int64_t)blockIdx.y) * n_d + d] = w;
+  part[(2 * (int64_t)blockIdx.y + 1) * n_d + d] = b;
 }
 
-template <class A>
-__global__ void __launch_bounds__(kThreads)
-ln_bwd_finish_kernel(const A* __restrict__ part, int count, int64_t n_d, A* __restrict__ wb,
-                     A* __restrict__ bb, bool add) {
-  const int64_t d = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (d >= n_d) return;
-  if (wb) {
-    const A s = ordered_sum(part + d, count, 2 * n_d);
-    wb[d] = add ? wb[d] + s : s;
-  }
-  if (bb) {
-    const A s = ordered_sum(part + n_d + d, count, 2 * n_d);
-    bb[d] = add ? bb[d] + s : s;
-  }
+// ---- which kernel --------------------------------------------------------------------
+// Calls f(VEC) with the widest vector the rows allow (`align` bytes) that
+// still gives each lane of a warp one.
+template <class T, class F>
+stade_status with_vec(int align, int64_t n_d, F&& f) {
+  using std::integral_constant;
+  constexpr int W = 16 / (int)sizeof(T);
+  if (align >= 16 && n_d >= 32 * W) return f(integral_constant<int, W>{});
+  if constexpr (sizeof(T) == 2)
+    if (align >= 4 && n_d >= 64) return f(integral_constant<int, 2>{});
+  return f(integral_constant<int, 1>{});
 }
 
-int row_chunks(int64_t n_s) { return (int)(n_s < 148 ? n_s : 148); }
+// Blocks of the reverse sweep, and so partials of the sums over rows: about
+// 1,024 threads an SM, but at least 32 rows a block beyond two blocks an SM (a
+// block's partials cost 16 bytes a column, its rows 6 to 12 bytes each).
+constexpr int64_t kBwdBlocks = 148 * 8;
+int64_t bwd_blocks(int64_t n_s, int threads) {
+  const int64_t fill = 148 * (1024 / threads);
+  return std::min<int64_t>(fill, std::max<int64_t>(148 * 2, n_s / 32));
+}
+
+// Ring kernels: a block of `threads` threads a row (NV vectors each), R rows a
+// turn, `stages` turns in flight, as many blocks an SM as `fit` threads
+// (registers) and 200 KB of shared memory allow.
+struct RingPlan {
+  int nv, rows, threads, stages, blocks;
+  size_t smem;
+};
+bool ring_plan(int64_t n_s, int64_t row_bytes, int arrays, int fit, RingPlan* p) {
+  const int64_t slots = row_bytes / 16;
+  if (slots < 96 || slots > 2 * 768) return false;
+  p->nv = slots <= 1024 ? 1 : 2;
+  p->threads = (int)(((slots + p->nv - 1) / p->nv + 31) / 32 * 32);
+  const int per_sm = std::max(1, std::min(8, fit / p->threads));
+  const int64_t room = 200 * 1024 / (per_sm * row_bytes * arrays);   // rows in flight a block
+  // several rows a turn where every block still gets two turns
+  p->rows = p->nv > 1 ? 1 : room >= 8 && n_s >= 8 * 148 * per_sm ? 4
+                          : room >= 4 && n_s >= 4 * 148 * per_sm ? 2 : 1;
+  p->stages = (int)std::min<int64_t>(kMaxStages, std::max<int64_t>(2, room / p->rows));
+  p->smem = 128 + p->stages * p->rows * row_bytes * arrays;
+  p->blocks = (int)std::min<int64_t>((n_s + p->rows - 1) / p->rows, 148 * per_sm);
+  return p->smem <= 200 * 1024 + 128;
+}
 
 template <class T>
 stade_status fwd(const void* x, const void* w, const void* b, void* y, void* m, void* r, double eps,
                  int64_t n_s, int64_t n_d, cudaStream_t st) {
   using A = acc_t<T>;
-  ln_fwd_kernel<T><<<(unsigned)n_s, kThreads, 0, st>>>(
-      (const T*)x, (const A*)w, (const A*)b, (T*)y, (A*)m, (A*)r, eps, n_d);
-  STADE_CHECK_LAUNCH();
-  return STADE_OK;
+  using std::integral_constant;
+  const int align = row_align(n_d * sizeof(T), {x, y});
+  RingPlan rp;
+  if (align == 16 && ring_plan(n_s, n_d * sizeof(T), 1, 1536, &rp)) {
+    auto kern = rp.nv == 2 ? ln_fwd_ring_kernel<T, 2, 1>
+                : rp.rows == 4 ? ln_fwd_ring_kernel<T, 1, 4>
+                : rp.rows == 2 ? ln_fwd_ring_kernel<T, 1, 2> : ln_fwd_ring_kernel<T, 1, 1>;
+    STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rp.smem));
+    kern<<<rp.blocks, rp.threads, rp.smem, st>>>((const T*)x, (const A*)w, (const A*)b, (T*)y, (A*)m,
+                                                 (A*)r, eps, n_s, (int)n_d, rp.stages);
+    STADE_CHECK_LAUNCH();
+    return STADE_OK;
+  }
+  return with_vec<T>(align, n_d, [&](auto vec) {
+    constexpr int VEC = decltype(vec)::value;
+    const int64_t slots = n_d / VEC;
+    auto go = [&](auto g, auto nv) {
+      constexpr int G = decltype(g)::value, NV = decltype(nv)::value, R = rows_per_block<G>();
+      ln_fwd_kernel<T, VEC, G, NV><<<ceil_div_u(n_s, R), G * R, 0, st>>>(
+          (const T*)x, (const A*)w, (const A*)b, (T*)y, (A*)m, (A*)r, eps, n_s, (int)n_d);
+      STADE_CHECK_LAUNCH();
+      return (stade_status)STADE_OK;
+    };
+    if (slots <= 64) return go(integral_constant<int, 32>{}, integral_constant<int, 2>{});
+    if (slots <= 256) return go(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    if (slots <= 1024) return go(integral_constant<int, 128>{}, integral_constant<int, 8>{});
+    if (slots <= 4096) return go(integral_constant<int, 512>{}, integral_constant<int, 8>{});
+    if (slots <= 8192) return go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
+    ln_fwd_long_kernel<T><<<(unsigned)n_s, kThreads, 0, st>>>(
+        (const T*)x, (const A*)w, (const A*)b, (T*)y, (A*)m, (A*)r, eps, n_d);
+    STADE_CHECK_LAUNCH();
+    return (stade_status)STADE_OK;
+  });
 }
 
 template <class T>
@@ -127,19 +708,59 @@ stade_status bwd(const void* x, void* xb, const void* w, void* wb, void* bb, voi
                  const void* m, const void* r, int64_t n_s, int64_t n_d, void* ws, bool add,
                  bool zero, cudaStream_t st) {
   using A = acc_t<T>;
-  if (xb) {
-    ln_bwd_x_kernel<T><<<(unsigned)n_s, kThreads, 0, st>>>(
-        (const T*)x, (T*)xb, (const A*)w, (const T*)yb, (const A*)m, (const A*)r, n_d, add);
+  using std::integral_constant;
+  const bool sums = wb || bb;
+  if (!xb && !sums && !zero) return STADE_OK;
+  int count = 0;
+  const int align = row_align(n_d * sizeof(T), {x, xb, yb});
+  RingPlan rp;
+  stade_status e = STADE_OK;
+  if (align == 16 && ring_plan(n_s, n_d * sizeof(T), 2, 1024, &rp)) {
+    count = rp.blocks;
+    const BwdArgs p{x, w, m, r, xb, yb, ws, n_s, (int)n_d, add, zero, sums};
+    auto kern = rp.nv == 2 ? ln_bwd_ring_kernel<T, 2, 1>
+                : rp.rows == 4 ? ln_bwd_ring_kernel<T, 1, 4>
+                : rp.rows == 2 ? ln_bwd_ring_kernel<T, 1, 2> : ln_bwd_ring_kernel<T, 1, 1>;
+    STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rp.smem));
+    kern<<<rp.blocks, rp.threads, rp.smem, st>>>(p, rp.stages);
     STADE_CHECK_LAUNCH();
+  } else {
+    e = with_vec<T>(align, n_d, [&](auto vec) {
+    constexpr int VEC = decltype(vec)::value;
+    const int64_t slots = n_d / VEC;
+    auto go = [&](auto g, auto nv) {
+      constexpr int G = decltype(g)::value, NV = decltype(nv)::value, R = rows_per_block<G>();
+      count = (int)std::min<int64_t>((n_s + R - 1) / R, bwd_blocks(n_s, G * R));
+      const BwdArgs p{x, w, m, r, xb, yb, ws, n_s, (int)n_d, add, zero, sums};
+      ln_bwd_kernel<T, VEC, G, NV><<<count, G * R, R > 1 ? 2 * n_d * sizeof(A) : 0, st>>>(p);
+      STADE_CHECK_LAUNCH();
+      return (stade_status)STADE_OK;
+    };
+    constexpr int NV = VEC >= 4 ? 2 : 4;
+    if (slots <= 32 * NV) return go(integral_constant<int, 32>{}, integral_constant<int, NV>{});
+    if (slots <= 128 * NV) return go(integral_constant<int, 128>{}, integral_constant<int, NV>{});
+    if (slots <= 256 * NV) return go(integral_constant<int, 256>{}, integral_constant<int, NV>{});
+    if (slots <= 512 * NV) return go(integral_constant<int, 512>{}, integral_constant<int, NV>{});
+    // 1,024 threads leave 64 registers each: enough for narrow vectors only
+    if constexpr (VEC == 1)
+      if (slots <= 1024 * NV) return go(integral_constant<int, 1024>{}, integral_constant<int, NV>{});
+    if (xb) {
+      ln_bwd_x_long_kernel<T><<<(unsigned)n_s, kThreads, 0, st>>>(
+          (const T*)x, (T*)xb, (const A*)w, (const T*)yb, (const A*)m, (const A*)r, n_d, add);
+      STADE_CHECK_LAUNCH();
+    }
+    count = (int)std::min<int64_t>(n_s, 148);
+    const int64_t rows = (n_s + count - 1) / count;
+    const dim3 grid(ceil_div_u(n_d, kThreads), count);
+    ln_bwd_w_long_kernel<T><<<grid, kThreads, 0, st>>>((const T*)x, (T*)yb, (const A*)m,
+                                                       (const A*)r, n_s, n_d, rows, (A*)ws, zero);
+    STADE_CHECK_LAUNCH();
+    return (stade_status)STADE_OK;
+    });
   }
-  const int chunks = row_chunks(n_s);
-  const int64_t rows = (n_s + chunks - 1) / chunks;
-  const dim3 grid(ceil_div_u(n_d, kThreads), chunks);
-  ln_bwd_w_kernel<T><<<grid, kThreads, 0, st>>>((const T*)x, (T*)yb, (const A*)m, (const A*)r, n_s,
-                                                n_d, rows, (A*)ws, zero);
-  STADE_CHECK_LAUNCH();
-  ln_bwd_finish_kernel<A><<<ceil_div_u(n_d, kThreads), kThreads, 0, st>>>((const A*)ws, chunks, n_d,
-                                                                         (A*)wb, (A*)bb, add);
+  if (e != STADE_OK || !sums) return e;
+  ln_finish_kernel<A><<<ceil_div_u(2 * n_d, 32), 1024, 0, st>>>((const A*)ws, count, n_d, (A*)wb,
+                                                                (A*)bb, add);
   STADE_CHECK_LAUNCH();
   return STADE_OK;
 }
@@ -152,6 +773,15 @@ stade_status check_sizes(const char* who, int dtype, int64_t n_s, int64_t n_d) {
 }
 
 }  // namespace
+
+int norm_take_error() {
+  int host = 0;
+  const int zero = 0;
+  if (cudaMemcpyFromSymbol(&host, g_norm_error, sizeof(int)) != cudaSuccess) return -1;
+  if (host) cudaMemcpyToSymbol(g_norm_error, &zero, sizeof(int));
+  return host;
+}
+
 }  // namespace stade
 
 using namespace stade;
@@ -174,7 +804,7 @@ extern "C" stade_status stade_layer_norm(int dtype, const void* x, const void* w
 extern "C" size_t stade_layer_norm_b_workspace(int dtype, int64_t n_s, int64_t n_d) {
   if (n_s <= 0 || n_d <= 0) return 0;
   Sizer z;
-  z.take<char>((size_t)row_chunks(n_s) * 2 * n_d * (dtype == STADE_F64 ? 8 : 4));
+  z.take<char>((size_t)std::min(n_s, kBwdBlocks) * 2 * n_d * (dtype == STADE_F64 ? 8 : 4));
   return z.bytes();
 }
 

@@ -1171,6 +1171,7 @@ int conv_tc_take_error();
 int heat_take_error();
 int embed_take_error();
 int expert_take_error();
+int norm_take_error();
 
 namespace {
 __device__ int g_wait_check_out = 0;
@@ -1214,6 +1215,7 @@ extern "C" int stade_device_error(void) {
   const int h = stade::heat_take_error();
   const int e = stade::embed_take_error();
   const int x = stade::expert_take_error();
-  if (t < 0 || c < 0 || h < 0 || e < 0 || x < 0) return -1;
-  return t | c | h | e | x;
+  const int n = stade::norm_take_error();
+  if (t < 0 || c < 0 || h < 0 || e < 0 || x < 0 || n < 0) return -1;
+  return t | c | h | e | x | n;
 }
