@@ -31,7 +31,7 @@ namespace {
 // value; short rows take narrower vectors so that a warp's lanes all have
 // work.
 //
-// Long rows that start on 16-byte boundaries take the ring kernels: one block
+// Long rows of arrays that start on 16-byte boundaries take the ring kernels: one block
 // holds a row, the rows to come are copied by cp.async.bulk into a ring in
 // shared memory, several rows ahead of the arithmetic, and w, b and the sums
 // over rows stay in registers for all of a block's rows.
@@ -247,12 +247,15 @@ __device__ int g_norm_error = 0;
 
 constexpr int kMaxStages = 8;
 
-// Sums of N values over the block, the same in every thread: within a warp by
-// halving (each step adds one half of the values to the lanes that keep it),
-// then one barrier and the warps' sums. `red`: 2 x 8 x 32 values, used
-// alternately (`turn`), so that no second barrier is needed.
-template <int N, class A>
-__device__ __forceinline__ void block_sums(A (&v)[N], A (*red)[8][32], int turn, int warps) {
+// v[i] = f(sum of v[i] over the block), the same in every thread: within a warp
+// by halving (each step adds one half of the values to the lanes that keep
+// it), then one barrier and the warps' sums; f runs once, on the lanes that
+// hold the sums, before they are spread (a division and a root per row in
+// every thread were a third of the forward's instructions). `red`: 2 x 8 x 32
+// values, zero where the block has no warp, used alternately (`turn`), so that
+// no second barrier is needed.
+template <int N, class A, class F>
+__device__ __forceinline__ void block_sums(A (&v)[N], A (*red)[8][32], int turn, F f) {
   constexpr int kLanes = 32 / N;       // lanes per value
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int n = N, off = 16;
@@ -274,248 +277,374 @@ __device__ __forceinline__ void block_sums(A (&v)[N], A (*red)[8][32], int turn,
   if (lane % kLanes == 0) red[turn][lane / kLanes][warp] = v[0];
   __syncthreads();
   A s = 0;
-  for (int w = lane % kLanes; w < warps; w += kLanes) s += red[turn][lane / kLanes][w];
+#pragma unroll
+  for (int i = 0; i < N; ++i) s += red[turn][lane / kLanes][lane % kLanes + i * kLanes];
 #pragma unroll
   for (int o = kLanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  s = f(s);
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, s, i * kLanes);
 }
 
 // A stage holds R consecutive rows of up to two arrays, each copied as one
-// piece (row bytes are a multiple of 16). All of a block's threads call
-// wait(); behind a barrier that follows their last read of a stage, thread 0
-// calls issue() for the rows that reuse it. A wait that runs out sets the
-// error word and the block goes on without waiting, so that its barriers still
-// match.
+// piece. Copies start and end on 16-byte boundaries: where row bytes are no
+// multiple of 16 a piece is widened to them (its rows then begin `mis` bytes
+// into the stage), and what would pass the array's end, under 16 bytes, is
+// copied by patch(). All of a block's threads call wait(); behind a barrier
+// that follows their last read of a stage, thread 0 calls issue() for the rows
+// that reuse it. A wait that runs out sets the error word and the block goes
+// on without waiting, so that its barriers still match.
+template <class T, int ARRAYS, bool WIDE>
 struct Ring {
+  const uint8_t* src[2];
   uint8_t* data;
   uint32_t bar0;
-  int stages, arrays;
+  int stages, R;
   uint32_t row_bytes, array_bytes;
+  int64_t total;
   bool dead;
-  __device__ __forceinline__ Ring(uint8_t* smem, int stages_, int rows, uint32_t row_bytes_,
-                                  int arrays_)
-      : data(smem + 128), bar0(tc5::smem_u32(smem)), stages(stages_), arrays(arrays_),
-        row_bytes(row_bytes_), array_bytes(rows * row_bytes_), dead(false) {
+  __device__ __forceinline__ Ring(uint8_t* smem, int stages_, int rows, int n_d, int64_t n_s,
+                                  const void* a, const void* b)
+      : data(smem + 128), bar0(tc5::smem_u32(smem)), stages(stages_), R(rows),
+        row_bytes(n_d * (uint32_t)sizeof(T)),
+        array_bytes(WIDE ? rows * row_bytes : (rows * row_bytes + 31) & ~15u),
+        total(n_s * row_bytes), dead(false) {
+    src[0] = (const uint8_t*)a;
+    src[1] = (const uint8_t*)b;
     if (threadIdx.x == 0) {
       for (int i = 0; i < stages; ++i) tc5::mbar_init(bar0 + 8 * i, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    __syncthreads();
   }
-  __device__ __forceinline__ const uint8_t* row(int stage, int array, int r) const {
-    return data + (size_t)(stage * arrays + array) * array_bytes + (size_t)r * row_bytes;
+  // the stage's rows, s on, of the first array; the second's follow array_bytes on
+  __device__ __forceinline__ const uint8_t* rows_of(int stage, int64_t s) const {
+    return data + (uint32_t)(stage * ARRAYS) * array_bytes +
+           (WIDE ? 0u : (uint32_t)(s * row_bytes) & 15u);
   }
-  // rows s .. s + rows - 1 of the arrays a and b
-  __device__ __forceinline__ void issue(int stage, const void* a, const void* b, int64_t s,
-                                        int rows) const {
-    const uint32_t bar = bar0 + 8 * stage, bytes = rows * row_bytes;
-    tc5::mbar_arrive_tx(bar, bytes * arrays);
-    tc5::bulk_load(tc5::smem_u32(row(stage, 0, 0)), (const uint8_t*)a + s * row_bytes, bytes, bar);
-    if (arrays == 2)
-      tc5::bulk_load(tc5::smem_u32(row(stage, 1, 0)), (const uint8_t*)b + s * row_bytes, bytes, bar);
+  __device__ __forceinline__ void issue(int stage, int64_t s) const {
+    const int64_t from = (s * row_bytes) & ~int64_t(15);
+    int64_t to = ((s + R) * row_bytes + 15) & ~int64_t(15);
+    if (to > total) to = total & ~int64_t(15);
+    const uint32_t bar = bar0 + 8 * stage, bytes = to > from ? (uint32_t)(to - from) : 0u;
+    tc5::mbar_arrive_tx(bar, bytes * ARRAYS);
+    if (bytes)
+#pragma unroll
+      for (int i = 0; i < ARRAYS; ++i)
+        tc5::bulk_load(tc5::smem_u32(data) + (stage * ARRAYS + i) * array_bytes, src[i] + from,
+                       bytes, bar);
   }
   __device__ __forceinline__ void wait(int stage, uint32_t parity) {
     if (!dead) dead = !tc5::mbar_wait(bar0 + 8 * stage, parity, &g_norm_error);
   }
+  // The array's last bytes into the stage of its last rows, s on.
+  __device__ __forceinline__ void patch(int stage, int64_t s) const {
+    if (WIDE || (s + R) * row_bytes < total || (total & 15) == 0) return;
+    const int64_t from = (s * row_bytes) & ~int64_t(15), cut = max(total & ~int64_t(15), from);
+    if ((int)threadIdx.x < (int)(total - cut))
+      for (int i = 0; i < ARRAYS; ++i)
+        data[(stage * ARRAYS + i) * array_bytes + (cut - from) + threadIdx.x] =
+            src[i][cut + threadIdx.x];
+    __syncthreads();
+  }
 };
 
+// The E columns of a row that a thread owns, in pairs: WIDE, M vectors of 16
+// bytes, vector i at slot i G + t; else single columns e G + t, for rows that
+// are no multiple of 16 bytes (one 2- or 4-byte access each, still 64 or 128
+// bytes a warp).
+template <class T, int M, bool WIDE>
+struct Own {
+  using A = acc_t<T>;
+  static constexpr int VEC = 16 / (int)sizeof(T), E = VEC * M;
+  int t, G, n_d;
+  uint32_t off, step;      // bytes: the first column, and from one vector (value) to the next
+  __device__ __forceinline__ Own(int t_, int G_, int n_d_)
+      : t(t_), G(G_), n_d(n_d_), off(t_ * (WIDE ? 16 : (int)sizeof(T))),
+        step(G_ * (WIDE ? 16 : (int)sizeof(T))) {}
+  __device__ __forceinline__ bool has(int e) const {
+    return WIDE ? (e / VEC * G + t) * VEC < n_d : e * G + t < n_d;
+  }
+  __device__ __forceinline__ int col(int e) const {
+    return WIDE ? (e / VEC * G + t) * VEC + e % VEC : e * G + t;
+  }
+  // zeros where the thread has no column (one vector a thread: only called
+  // where it has it)
+  __device__ __forceinline__ void load(const uint8_t* row, Pair<A> (&o)[E / 2]) const {
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        Vec<T, VEC> v;
+        if (M > 1) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) v.v[k] = round_to<T>(A(0));
+        }
+        if (M == 1 || has(i * VEC))
+          v = *reinterpret_cast<const Vec<T, VEC>*>(row + off + i * step);
+#pragma unroll
+        for (int k = 0; k < VEC / 2; ++k)
+          o[i * (VEC / 2) + k] = widen2(*reinterpret_cast<const Vec<T, 2>*>(&v.v[2 * k]));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const T* p = reinterpret_cast<const T*>(row + off + e * step);
+        const T* q = reinterpret_cast<const T*>(row + off + (e + 1) * step);
+        o[e / 2] = Pair<A>(has(e) ? load_acc<T>(*p) : A(0), has(e + 1) ? load_acc<T>(*q) : A(0));
+      }
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t* row, const Pair<A> (&o)[E / 2]) const {
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        Vec<T, VEC> v;
+#pragma unroll
+        for (int k = 0; k < VEC / 2; ++k)
+          *reinterpret_cast<Vec<T, 2>*>(&v.v[2 * k]) = narrow2<T>(o[i * (VEC / 2) + k]);
+        if (has(i * VEC)) *reinterpret_cast<Vec<T, VEC>*>(row + off + i * step) = v;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        if (has(e)) *reinterpret_cast<T*>(row + off + e * step) = round_to<T>(o[e / 2].lo());
+        if (has(e + 1))
+          *reinterpret_cast<T*>(row + off + (e + 1) * step) = round_to<T>(o[e / 2].hi());
+      }
+    }
+  }
+  __device__ __forceinline__ void params(const A* p, A other, Pair<A> (&o)[E / 2]) const {
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+      o[e / 2] = Pair<A>(p && has(e) ? p[col(e)] : other, p && has(e + 1) ? p[col(e + 1)] : other);
+  }
+  __device__ __forceinline__ void store_params(A* p, const Pair<A> (&o)[E / 2]) const {
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      if (has(e)) p[col(e)] = o[e / 2].lo();
+      if (has(e + 1)) p[col(e + 1)] = o[e / 2].hi();
+    }
+  }
+};
+
+template <class A>
+__device__ __forceinline__ void clear_red(A (*red)[8][32]) {
+  for (int i = threadIdx.x; i < 2 * 8 * 32; i += blockDim.x) (&red[0][0][0])[i] = A(0);
+  __syncthreads();
+}
+
 // R rows a turn: what a turn costs beside its arithmetic (the wait, two
-// barriers, the shuffles) is shared by them. Measured, 8192 x 5000 f16: 71.7 us
-// with one row a turn.
-template <class T, int NV, int R>
-__global__ void __launch_bounds__(NV == 1 ? 1024 : 768)
+// barriers, the shuffles) is shared by them.
+template <class T, int M, bool WIDE, int R, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB)
 ln_fwd_ring_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
                    const acc_t<T>* __restrict__ b, T* __restrict__ y,
                    acc_t<T>* __restrict__ m_stack, acc_t<T>* __restrict__ r_stack, double eps,
                    int64_t n_s, int n_d, int stages) {
   using A = acc_t<T>;
-  constexpr int VEC = 16 / (int)sizeof(T);
-  using V = Vec<T, VEC>;
+  using O = Own<T, M, WIDE>;
+  constexpr int E = O::E;
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ A red[2][8][32];
-  Ring ring(sm, stages, R, (uint32_t)(n_d * sizeof(T)), 1);
-  const int t = threadIdx.x, G = blockDim.x, slots = n_d / VEC, nw = G / 32;
-  A wr[NV][VEC], br[NV][VEC];
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      const int j = i * G + t;
-      wr[i][k] = w && j < slots ? w[j * VEC + k] : A(1);
-      br[i][k] = b && j < slots ? b[j * VEC + k] : A(0);
-    }
+  Ring<T, 1, WIDE> ring(sm, stages, R, n_d, n_s, x, nullptr);
+  clear_red(red);
+  const int t = threadIdx.x;
+  const O own(t, (int)blockDim.x, n_d);
+  Pair<A> wr[E / 2], br[E / 2];
+  own.params(w, A(1), wr);
+  own.params(b, A(0), br);
   const int64_t first = (int64_t)blockIdx.x * R, step = (int64_t)gridDim.x * R;
-  auto rows_at = [&](int64_t s) { return (int)min((int64_t)R, n_s - s); };
   if (t == 0)
-    for (int i = 0; i < stages && first + i * step < n_s; ++i)
-      ring.issue(i, x, nullptr, first + i * step, rows_at(first + i * step));
+    for (int i = 0; i < stages && first + i * step < n_s; ++i) ring.issue(i, first + i * step);
   int stage = 0;
   uint32_t parity = 0;
-  for (int64_t s = first; s < n_s; s += step) {
-    const int rows = rows_at(s);
+  const A inv = A(1) / (A)n_d;
+  uint8_t* out = reinterpret_cast<uint8_t*>(y) + first * ring.row_bytes;
+  const bool mine = own.has(0);
+  for (int64_t s = first; s < n_s; s += step, out += step * ring.row_bytes) {
+    const int rows = (int)min((int64_t)R, n_s - s);
     ring.wait(stage, parity);
-    V raw[R][NV];
+    ring.patch(stage, s);
+    const uint8_t* in = ring.rows_of(stage, s);
+    Pair<A> c[R][E / 2];
     A v[R];
+    // rows past the last one: whatever the stage holds, never stored
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       v[q] = 0;
-      if (q < rows) {
-        const V* row = reinterpret_cast<const V*>(ring.row(stage, 0, q));
+      if (mine) {
+        own.load(in + q * ring.row_bytes, c[q]);
+        Pair<A> sum = c[q][0];
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (i * G + t < slots) {
-            raw[q][i] = row[i * G + t];
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) v[q] += load_acc<T>(raw[q][i].v[k]);
-          }
+        for (int k = 1; k < E / 2; ++k) sum = add2(sum, c[q][k]);
+        v[q] = sum.lo() + sum.hi();
       }
     }
-    block_sums<R>(v, red, 0, nw);
+    block_sums<R>(v, red, 0, [&](A z) { return z * inv; });
     // every thread has read the stage: it takes the rows to come
-    if (t == 0 && s + stages * step < n_s)
-      ring.issue(stage, x, nullptr, s + stages * step, rows_at(s + stages * step));
+    if (t == 0 && s + stages * step < n_s) ring.issue(stage, s + stages * step);
     A mean[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      mean[q] = v[q] / (A)n_d;
-      v[q] = 0;
-      if (q < rows)
+      mean[q] = v[q];
+      const Pair<A> minus = both(-v[q]);
+      Pair<A> sq = both(A(0));
+      if constexpr (WIDE) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (i * G + t < slots)
+        for (int k = 0; k < E / 2; ++k) {
+          c[q][k] = add2(c[q][k], minus);
+          if (M == 1 || own.has(2 * k)) sq = fma2(c[q][k], c[q][k], sq);
+        }
+        v[q] = mine ? sq.lo() + sq.hi() : A(0);
+      } else {
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-              const A c = load_acc<T>(raw[q][i].v[k]) - mean[q];
-              v[q] += c * c;
-            }
+        for (int k = 0; k < E / 2; ++k) {
+          c[q][k] = add2(c[q][k], minus);
+          const Pair<A> z(own.has(2 * k) ? c[q][k].lo() : A(0),
+                          own.has(2 * k + 1) ? c[q][k].hi() : A(0));
+          sq = fma2(z, z, sq);
+        }
+        v[q] = sq.lo() + sq.hi();
+      }
     }
-    block_sums<R>(v, red, 1, nw);
+    block_sums<R>(v, red, 1, [&](A z) { return A(1) / sqrt(z * inv + (A)eps); });
 #pragma unroll
     for (int q = 0; q < R; ++q)
-      if (q < rows) {
-        const A rstd = A(1) / sqrt(v[q] / (A)n_d + (A)eps);
-        if (t == 0) {
-          m_stack[s + q] = mean[q];
-          r_stack[s + q] = rstd;
-        }
+      if (q < rows && mine) {
+        const Pair<A> rstd = both(v[q]);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (i * G + t < slots) {
-            A o[VEC];
-#pragma unroll
-            for (int k = 0; k < VEC; ++k)
-              o[k] = (load_acc<T>(raw[q][i].v[k]) - mean[q]) * rstd * wr[i][k] + br[i][k];
-            store_vec<T, VEC>(y + (s + q) * n_d + (i * G + t) * VEC, o);
-          }
+        for (int k = 0; k < E / 2; ++k) c[q][k] = fma2(mul2(c[q][k], rstd), wr[k], br[k]);
+        own.store(out + q * ring.row_bytes, c[q]);
       }
+    if (t < rows) {
+      A a = mean[0], z = v[0];
+#pragma unroll
+      for (int q = 1; q < R; ++q)
+        if (t == q) a = mean[q], z = v[q];
+      m_stack[s + t] = a;
+      r_stack[s + t] = z;
+    }
     if (++stage == stages) stage = 0, parity ^= 1;
   }
 }
 
-template <class T, int NV, int R>
-__global__ void __launch_bounds__(NV == 1 ? 1024 : 768)
+// KEEP: h and g w stay in registers over the sums; otherwise the row is read
+// and widened from the stage once more (the longest rows, whose threads have 80
+// registers). 16-bit rows are bound by instructions and by the latency of a
+// turn's sums, not by memory: 16384 x 4096 takes 103 us in bf16 when the row is
+// read twice (32 instructions an element), 83 us kept, 61 us by memory alone;
+// in Float32 129 us, 0.95 of the measured copy rate.
+template <class T, int M, bool WIDE, int R, int MAXT, bool KEEP>
+__global__ void __launch_bounds__(MAXT, 1)
 ln_bwd_ring_kernel(BwdArgs p, int stages) {
   using A = acc_t<T>;
-  constexpr int VEC = 16 / (int)sizeof(T);
-  using V = Vec<T, VEC>;
+  using O = Own<T, M, WIDE>;
+  constexpr int E = O::E;
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ A red[2][8][32];
-  Ring ring(sm, stages, R, (uint32_t)(p.n_d * sizeof(T)), 2);
-  const int t = threadIdx.x, G = blockDim.x, slots = p.n_d / VEC, nw = G / 32;
-  T* yb = (T*)p.yb;
+  Ring<T, 2, WIDE> ring(sm, stages, R, p.n_d, p.n_s, p.x, p.yb);
+  clear_red(red);
+  const int t = threadIdx.x;
+  const O own(t, (int)blockDim.x, p.n_d);
   const A* m = (const A*)p.m;
   const A* r = (const A*)p.r;
-  A w[NV][VEC], sw[NV][VEC], sb[NV][VEC];
+  Pair<A> w[E / 2], sw[E / 2], sb[E / 2];
+  own.params((const A*)p.w, A(1), w);
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      w[i][k] = p.w && i * G + t < slots ? ((const A*)p.w)[(i * G + t) * VEC + k] : A(1);
-      sw[i][k] = sb[i][k] = A(0);
-    }
+  for (int k = 0; k < E / 2; ++k) sw[k] = sb[k] = both(A(0));
   const int64_t first = (int64_t)blockIdx.x * R, step = (int64_t)gridDim.x * R;
-  auto rows_at = [&](int64_t s) { return (int)min((int64_t)R, p.n_s - s); };
   if (t == 0)
-    for (int i = 0; i < stages && first + i * step < p.n_s; ++i)
-      ring.issue(i, p.x, yb, first + i * step, rows_at(first + i * step));
+    for (int i = 0; i < stages && first + i * step < p.n_s; ++i) ring.issue(i, first + i * step);
   int stage = 0, turn = 0, last = -1;
   uint32_t parity = 0;
   const A inv = A(1) / (A)p.n_d;
-  for (int64_t s = first; s < p.n_s; s += step) {
-    const int rows = rows_at(s);
-    A rstd[R], mr[R], v[2 * R];     // h = x rstd - mean rstd
+  A nr[R], nm[R];                 // the next turn's statistics, loaded a turn ahead
+  auto stats = [&](int64_t s) {
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      if (s + q < p.n_s) nr[q] = r[s + q], nm[q] = m[s + q];
+  };
+  stats(first);
+  int64_t out = first * ring.row_bytes;
+  // a thread past the row's end has nothing to do (single columns: some of them)
+  const bool mine = own.has(0);
+  for (int64_t s = first; s < p.n_s; s += step, out += step * ring.row_bytes) {
+    const int rows = (int)min((int64_t)R, p.n_s - s);
+    A rstd[R], shift[R], v[2 * R];     // h = x rstd + shift
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      rstd[q] = q < rows ? r[s + q] : A(0);
-      mr[q] = q < rows ? m[s + q] : A(0);
+      rstd[q] = nr[q];
+      shift[q] = -nm[q] * nr[q];
       v[2 * q] = v[2 * q + 1] = A(0);
     }
+    stats(s + step);
     ring.wait(stage, parity);
+    ring.patch(stage, s);
+    const uint8_t* in = ring.rows_of(stage, s);
+    Pair<A> kh[KEEP ? R : 1][E / 2], kg[KEEP ? R : 1][E / 2];
 #pragma unroll
     for (int q = 0; q < R; ++q)
-      if (q < rows) {
-        const V* xs = reinterpret_cast<const V*>(ring.row(stage, 0, q));
-        const V* ys = reinterpret_cast<const V*>(ring.row(stage, 1, q));
+      if (q < rows && mine) {
+        Pair<A> cx[E / 2], cy[E / 2], sg = both(A(0)), sgh = both(A(0));
+        own.load(in + q * ring.row_bytes, cx);
+        own.load(in + ring.array_bytes + q * ring.row_bytes, cy);
+        const Pair<A> rs = both(rstd[q]), sh = both(shift[q]);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (i * G + t < slots) {
-            const V cx = xs[i * G + t], cy = ys[i * G + t];
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-              const A h = (load_acc<T>(cx.v[k]) - mr[q]) * rstd[q], g = load_acc<T>(cy.v[k]);
-              const A gw = g * w[i][k];
-              v[2 * q] += gw;
-              v[2 * q + 1] += gw * h;
-              sw[i][k] += g * h;
-              sb[i][k] += g;
-            }
-          }
+        for (int k = 0; k < E / 2; ++k) {
+          // columns the thread does not have: yb = 0 there, so nothing is added
+          const Pair<A> h = fma2(cx[k], rs, sh), gw = mul2(cy[k], w[k]);
+          sg = add2(sg, gw);
+          sgh = fma2(gw, h, sgh);
+          sw[k] = fma2(cy[k], h, sw[k]);
+          sb[k] = add2(sb[k], cy[k]);
+          if (KEEP) kh[KEEP ? q : 0][k] = h, kg[KEEP ? q : 0][k] = gw;
+        }
+        v[2 * q] = sg.lo() + sg.hi();
+        v[2 * q + 1] = sgh.lo() + sgh.hi();
       }
-    block_sums<2 * R>(v, red, turn, nw);
+    block_sums<2 * R>(v, red, turn, [&](A z) { return z * inv; });
     turn ^= 1;
     // every thread is past the previous turn's stage: it takes the rows to come
-    const int64_t ahead = s + (stages - 1) * step;
-    if (t == 0 && last >= 0 && ahead < p.n_s) ring.issue(last, p.x, yb, ahead, rows_at(ahead));
+    if (t == 0 && last >= 0 && s + (stages - 1) * step < p.n_s)
+      ring.issue(last, s + (stages - 1) * step);
 #pragma unroll
     for (int q = 0; q < R; ++q)
-      if (q < rows) {
-        const V* xs = reinterpret_cast<const V*>(ring.row(stage, 0, q));
-        const V* ys = reinterpret_cast<const V*>(ring.row(stage, 1, q));
-        const A mg = v[2 * q] * inv, mgh = v[2 * q + 1] * inv;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (i * G + t < slots) {
-            const int64_t at = (s + q) * p.n_d + (int64_t)(i * G + t) * VEC;
-            if (p.xb) {
-              const V cx = xs[i * G + t], cy = ys[i * G + t];
-              T* o = (T*)p.xb + at;
-              A out[VEC], old[VEC];
-              if (p.add) load_vec<T, VEC>(o, old);
-#pragma unroll
-              for (int k = 0; k < VEC; ++k) {
-                const A h = (load_acc<T>(cx.v[k]) - mr[q]) * rstd[q];
-                out[k] = rstd[q] * (load_acc<T>(cy.v[k]) * w[i][k] - mg - h * mgh);
-                if (p.add) out[k] += old[k];
-              }
-              store_vec<T, VEC>(o, out);
-            }
-            if (p.zero) store_zero<T, VEC>(yb + at);
+      if (q < rows && mine) {
+        Pair<A> cx[E / 2], cy[E / 2];
+        if (p.xb) {
+          uint8_t* o = (uint8_t*)p.xb + out + q * ring.row_bytes;
+          // rstd (g - mean(g) - h mean(g h))
+          const Pair<A> rs = both(rstd[q]), sh = both(shift[q]);
+          const Pair<A> mg = both(-v[2 * q] * rstd[q]), mgh = both(-v[2 * q + 1] * rstd[q]);
+          if (!KEEP) {
+            own.load(in + q * ring.row_bytes, cx);
+            own.load(in + ring.array_bytes + q * ring.row_bytes, cy);
           }
+#pragma unroll
+          for (int k = 0; k < E / 2; ++k) {
+            const Pair<A> h = KEEP ? kh[KEEP ? q : 0][k] : fma2(cx[k], rs, sh);
+            const Pair<A> gw = KEEP ? kg[KEEP ? q : 0][k] : mul2(cy[k], w[k]);
+            cx[k] = fma2(gw, rs, fma2(h, mgh, mg));
+          }
+          if (p.add) {
+            own.load(o, cy);
+#pragma unroll
+            for (int k = 0; k < E / 2; ++k) cx[k] = add2(cx[k], cy[k]);
+          }
+          own.store(o, cx);
+        }
+        if (p.zero) {
+#pragma unroll
+          for (int k = 0; k < E / 2; ++k) cy[k] = both(A(0));
+          own.store((uint8_t*)p.yb + out + q * ring.row_bytes, cy);
+        }
       }
     last = stage;
     if (++stage == stages) stage = 0, parity ^= 1;
   }
   if (!p.sums) return;
   A* part = (A*)p.part + (int64_t)blockIdx.x * 2 * p.n_d;
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (i * G + t < slots)
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        part[(i * G + t) * VEC + k] = sw[i][k];
-        part[p.n_d + (i * G + t) * VEC + k] = sb[i][k];
-      }
+  own.store_params(part, sw);
+  own.store_params(part + p.n_d, sb);
 }
 
 // wb and bb from the partials [count][2][n_d]: 32 columns a block, 32 warps
@@ -641,27 +770,37 @@ int64_t bwd_blocks(int64_t n_s, int threads) {
   return std::min<int64_t>(fill, std::max<int64_t>(148 * 2, n_s / 32));
 }
 
-// Ring kernels: a block of `threads` threads a row (NV vectors each), R rows a
-// turn, `stages` turns in flight, as many blocks an SM as `fit` threads
-// (registers) and 200 KB of shared memory allow.
+// Ring kernels: a block of `threads` threads a row (m vectors each), `rows` rows
+// a turn, `stages` turns in flight, as many blocks an SM as registers and 200
+// KB of shared memory allow.
+//  - Forward: one vector a thread and several rows a turn, 1,024 threads an SM
+//    at 64 registers; two vectors where a row would take 513 to 672 threads and
+//    leave the SM a third empty (8192 x 5000 f16: 49.6 -> 41.9 us).
+//  - Reverse: the row's h and g w stay in registers, 512 threads at 128, so two
+//    vectors a thread and two or more blocks an SM rather than several rows a
+//    turn, which left one block and its barriers alone on the SM (16384 x 4096
+//    bf16: 83 us against 106 with four rows a turn; 32768 x 1024: 48 against
+//    56). Single columns spill at two vectors' worth: two rows a turn there
+//    (32768 x 1023 bf16: 63 us against 93).
 struct RingPlan {
-  int nv, rows, threads, stages, blocks;
+  int m, rows, threads, stages, blocks;
   size_t smem;
 };
-bool ring_plan(int64_t n_s, int64_t row_bytes, int arrays, int fit, RingPlan* p) {
-  const int64_t slots = row_bytes / 16;
+bool ring_plan(int64_t n_s, int64_t row_bytes, bool rev, bool wide, RingPlan* p) {
+  const int64_t slots = (row_bytes + 15) / 16;   // a thread owns 16 bytes of a row, or 32
   if (slots < 96 || slots > 2 * 768) return false;
-  p->nv = slots <= 1024 ? 1 : 2;
-  p->threads = (int)(((slots + p->nv - 1) / p->nv + 31) / 32 * 32);
-  const int per_sm = std::max(1, std::min(8, fit / p->threads));
+  p->m = rev ? (wide || slots > 512 ? 2 : 1) : slots <= 512 || (slots > 672 && slots <= 1024) ? 1 : 2;
+  p->threads = (int)(((slots + p->m - 1) / p->m + 31) / 32 * 32);
+  const int per_sm = std::max(1, (rev ? 512 : p->m == 2 ? 768 : 1024) / p->threads);
+  const int arrays = rev ? 2 : 1;
   const int64_t room = 200 * 1024 / (per_sm * row_bytes * arrays);   // rows in flight a block
   // several rows a turn where every block still gets two turns
-  p->rows = p->nv > 1 ? 1 : room >= 8 && n_s >= 8 * 148 * per_sm ? 4
-                          : room >= 4 && n_s >= 4 * 148 * per_sm ? 2 : 1;
+  p->rows = p->m > 1 || n_s < 4 * 148 * per_sm || room < 4 ? 1
+            : !rev && p->threads <= 512 && room >= 8 && n_s >= 8 * 148 * per_sm ? 4 : 2;
   p->stages = (int)std::min<int64_t>(kMaxStages, std::max<int64_t>(2, room / p->rows));
-  p->smem = 128 + p->stages * p->rows * row_bytes * arrays;
+  p->smem = 128 + p->stages * arrays * ((p->rows * row_bytes + 31) & ~int64_t(15));
   p->blocks = (int)std::min<int64_t>((n_s + p->rows - 1) / p->rows, 148 * per_sm);
-  return p->smem <= 200 * 1024 + 128;
+  return p->smem <= 205 * 1024;
 }
 
 template <class T>
@@ -671,15 +810,22 @@ stade_status fwd(const void* x, const void* w, const void* b, void* y, void* m, 
   using std::integral_constant;
   const int align = row_align(n_d * sizeof(T), {x, y});
   RingPlan rp;
-  if (align == 16 && ring_plan(n_s, n_d * sizeof(T), 1, 1536, &rp)) {
-    auto kern = rp.nv == 2 ? ln_fwd_ring_kernel<T, 2, 1>
-                : rp.rows == 4 ? ln_fwd_ring_kernel<T, 1, 4>
-                : rp.rows == 2 ? ln_fwd_ring_kernel<T, 1, 2> : ln_fwd_ring_kernel<T, 1, 1>;
-    STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rp.smem));
-    kern<<<rp.blocks, rp.threads, rp.smem, st>>>((const T*)x, (const A*)w, (const A*)b, (T*)y, (A*)m,
-                                                 (A*)r, eps, n_s, (int)n_d, rp.stages);
-    STADE_CHECK_LAUNCH();
-    return STADE_OK;
+  if (row_align(16, {x}) == 16 && ring_plan(n_s, n_d * sizeof(T), false, align == 16, &rp)) {
+    auto go = [&](auto wide) {
+      constexpr bool WIDE = decltype(wide)::value;
+      auto kern = rp.m == 2 ? ln_fwd_ring_kernel<T, 2, WIDE, 1, 768, 1>
+                  : rp.threads > 512 ? (rp.rows == 2 ? ln_fwd_ring_kernel<T, 1, WIDE, 2, 1024, 1>
+                                                     : ln_fwd_ring_kernel<T, 1, WIDE, 1, 1024, 1>)
+                  : rp.rows == 4 ? ln_fwd_ring_kernel<T, 1, WIDE, 4, 512, 2>
+                  : rp.rows == 2 ? ln_fwd_ring_kernel<T, 1, WIDE, 2, 512, 2>
+                                 : ln_fwd_ring_kernel<T, 1, WIDE, 1, 512, 2>;
+      STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rp.smem));
+      kern<<<rp.blocks, rp.threads, rp.smem, st>>>((const T*)x, (const A*)w, (const A*)b, (T*)y, (A*)m,
+                                                   (A*)r, eps, n_s, (int)n_d, rp.stages);
+      STADE_CHECK_LAUNCH();
+      return (stade_status)STADE_OK;
+    };
+    return align == 16 ? go(std::true_type{}) : go(std::false_type{});
   }
   return with_vec<T>(align, n_d, [&](auto vec) {
     constexpr int VEC = decltype(vec)::value;
@@ -715,15 +861,23 @@ stade_status bwd(const void* x, void* xb, const void* w, void* wb, void* bb, voi
   const int align = row_align(n_d * sizeof(T), {x, xb, yb});
   RingPlan rp;
   stade_status e = STADE_OK;
-  if (align == 16 && ring_plan(n_s, n_d * sizeof(T), 2, 1024, &rp)) {
+  if (row_align(16, {x, yb}) == 16 && ring_plan(n_s, n_d * sizeof(T), true, align == 16, &rp)) {
     count = rp.blocks;
     const BwdArgs p{x, w, m, r, xb, yb, ws, n_s, (int)n_d, add, zero, sums};
-    auto kern = rp.nv == 2 ? ln_bwd_ring_kernel<T, 2, 1>
-                : rp.rows == 4 ? ln_bwd_ring_kernel<T, 1, 4>
-                : rp.rows == 2 ? ln_bwd_ring_kernel<T, 1, 2> : ln_bwd_ring_kernel<T, 1, 1>;
-    STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rp.smem));
-    kern<<<rp.blocks, rp.threads, rp.smem, st>>>(p, rp.stages);
-    STADE_CHECK_LAUNCH();
+    auto go = [&](auto wide) {
+      constexpr bool WIDE = decltype(wide)::value;
+      void (*kern)(BwdArgs, int) = rp.threads > 512 ? ln_bwd_ring_kernel<T, 2, WIDE, 1, 768, false>
+                                                   : ln_bwd_ring_kernel<T, 2, WIDE, 1, 512, true>;
+      if constexpr (!WIDE)
+        if (rp.m == 1)
+          kern = rp.rows == 2 ? ln_bwd_ring_kernel<T, 1, false, 2, 512, true>
+                              : ln_bwd_ring_kernel<T, 1, false, 1, 512, true>;
+      STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rp.smem));
+      kern<<<rp.blocks, rp.threads, rp.smem, st>>>(p, rp.stages);
+      STADE_CHECK_LAUNCH();
+      return (stade_status)STADE_OK;
+    };
+    e = align == 16 ? go(std::true_type{}) : go(std::false_type{});
   } else {
     e = with_vec<T>(align, n_d, [&](auto vec) {
     constexpr int VEC = decltype(vec)::value;

@@ -54,6 +54,79 @@ __device__ __forceinline__ void store_zero(T* __restrict__ p) {
   *reinterpret_cast<Vec<T, V>*>(p) = r;
 }
 
+// Two values of the sums' type computed on together: one instruction for two
+// Float32 multiply-adds (fma.rn.f32x2), where the issue rate and not memory
+// would bound a kernel on 16-bit data.
+template <class A> struct Pair {
+  A a, b;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(A x, A y) : a(x), b(y) {}
+  __device__ __forceinline__ A lo() const { return a; }
+  __device__ __forceinline__ A hi() const { return b; }
+};
+template <> struct Pair<float> {
+  unsigned long long r;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float x, float y) {
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  }
+  __device__ __forceinline__ float lo() const {
+    return __uint_as_float((uint32_t)r);
+  }
+  __device__ __forceinline__ float hi() const {
+    return __uint_as_float((uint32_t)(r >> 32));
+  }
+};
+template <class A> __device__ __forceinline__ Pair<A> both(A x) { return Pair<A>(x, x); }
+template <class A> __device__ __forceinline__ Pair<A> add2(Pair<A> x, Pair<A> y) {
+  return Pair<A>(x.a + y.a, x.b + y.b);
+}
+template <class A> __device__ __forceinline__ Pair<A> mul2(Pair<A> x, Pair<A> y) {
+  return Pair<A>(x.a * y.a, x.b * y.b);
+}
+template <class A> __device__ __forceinline__ Pair<A> fma2(Pair<A> x, Pair<A> y, Pair<A> z) {
+  return Pair<A>(fma(x.a, y.a, z.a), fma(x.b, y.b, z.b));
+}
+template <> __device__ __forceinline__ Pair<float> add2(Pair<float> x, Pair<float> y) {
+  Pair<float> o;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(o.r) : "l"(x.r), "l"(y.r));
+  return o;
+}
+template <> __device__ __forceinline__ Pair<float> mul2(Pair<float> x, Pair<float> y) {
+  Pair<float> o;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(o.r) : "l"(x.r), "l"(y.r));
+  return o;
+}
+template <> __device__ __forceinline__ Pair<float> fma2(Pair<float> x, Pair<float> y,
+                                                        Pair<float> z) {
+  Pair<float> o;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(o.r) : "l"(x.r), "l"(y.r), "l"(z.r));
+  return o;
+}
+// Two neighbouring elements widened, and rounded back.
+template <class T> __device__ __forceinline__ Pair<acc_t<T>> widen2(const Vec<T, 2>& v) {
+  return Pair<acc_t<T>>(load_acc<T>(v.v[0]), load_acc<T>(v.v[1]));
+}
+template <> __device__ __forceinline__ Pair<float> widen2(const Vec<__nv_bfloat16, 2>& v) {
+  const uint32_t u = *reinterpret_cast<const uint32_t*>(&v);
+  return Pair<float>(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+template <> __device__ __forceinline__ Pair<float> widen2(const Vec<__half, 2>& v) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+  return Pair<float>(f.x, f.y);
+}
+template <class T> __device__ __forceinline__ Vec<T, 2> narrow2(Pair<acc_t<T>> p) {
+  return Vec<T, 2>{{round_to<T>(p.lo()), round_to<T>(p.hi())}};
+}
+template <> __device__ __forceinline__ Vec<__nv_bfloat16, 2> narrow2<__nv_bfloat16>(Pair<float> p) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(p.lo(), p.hi());
+  return *reinterpret_cast<const Vec<__nv_bfloat16, 2>*>(&h);
+}
+template <> __device__ __forceinline__ Vec<__half, 2> narrow2<__half>(Pair<float> p) {
+  const __half2 h = __floats2half2_rn(p.lo(), p.hi());
+  return *reinterpret_cast<const Vec<__half, 2>*>(&h);
+}
+
 inline bool known_dtype(int d) {
   return d == STADE_F32 || d == STADE_F64 || d == STADE_BF16 || d == STADE_F16;
 }

@@ -35,7 +35,12 @@ def _dev(t, dt, offset=0):
 # ---- layer_norm --------------------------------------------------------------------
 NORM_SIZES = [(1, 1, 0), (1, 512, 0), (3, 7, 0), (5, 33, 1), (37, 96, 0), (2, 1000, 0), (9, 1024, 1),
               (4, 784, 0), (3, 2500, 0), (2, 4096, 0), (3, 5000, 3), (2, 8191, 0), (1, 16384, 0),
-              (2, 20000, 0), (300, 64, 0), (2, 40001, 0)]
+              (2, 20000, 0), (300, 64, 0), (2, 40001, 0),
+              # enough rows for several a turn and turns beyond a block's first, row
+              # counts that end inside one; widths with every remainder class
+              (1300, 1024, 0), (2501, 800, 0), (1500, 1023, 0), (2400, 771, 0), (700, 4096, 0),
+              (650, 5000, 0), (630, 5001, 0), (320, 8192, 0), (310, 8187, 0), (160, 9000, 0),
+              (40, 12282, 0)]
 
 
 @pytest.mark.parametrize("dt", ALL)
