@@ -73,23 +73,10 @@ embed_fwd_kernel(const T* __restrict__ w, const int64_t* __restrict__ ids, T* __
 // numbers, so their order does not matter).
 constexpr int kMaxBins = 512;
 constexpr int kWarps = 8;
-constexpr int kWarpItems = 256;
+constexpr int kWarpItems = 128;
 constexpr int kChunk = kWarps * kWarpItems;   // elements of one block
 constexpr int kFusedScan = 64;                // blocks up to which a scatter adds the counts itself
 constexpr int kSmallSort = 4096;
-
-// ---- sums of rows ----------------------------------------------------------------
-// After the sort a table row's positions lie side by side. Rows of up to kShort
-// positions are summed by one warp; longer ones are cut into pieces of up to
-// kPiece positions, a block each (its warps take an eighth of the piece one
-// after the other's end), whose sums the last block of the row adds up in
-// order. The id that takes a tenth of a batch then costs what its rows cost.
-constexpr int kShort = 32;
-constexpr int kPiece = 512;
-
-struct Piece {
-  uint32_t v, from, len, first, count;   // first piece of the row and how many it has
-};
 
 struct SortIn {
   const int64_t* ids;      // first pass: keys from the ids, positions 0 .. n - 1
@@ -106,25 +93,51 @@ __device__ __forceinline__ uint32_t sort_key(const SortIn& in, int64_t i) {
   return in.ids ? id_key(in, i) : in.keys[i];
 }
 
-// First pass: digit counts per block; zeroes the later passes' counts and the
-// number of pieces.
+// Digit counts per block: [block][digit], which every block of the scatter reads
+// through, or [digit][block] for the scan of many blocks.
+__device__ __forceinline__ int64_t count_at(int digit, int block, int bins, int blocks,
+                                            bool by_digit) {
+  return by_digit ? (int64_t)digit * blocks + block : (int64_t)block * bins + digit;
+}
+
+// The sort keeps a few dozen blocks busy for some 30 us; the rest of the GPU
+// meanwhile clears the gradient (when it is stored, not added to), so that the
+// sums write only the rows that have positions. A kernel's blocks past `first`
+// clear one part of it.
+struct Fill {
+  int4* p;              // 16-byte pieces, then single bytes up to `bytes`
+  int64_t bytes;
+  int part, parts;
+};
+__device__ __forceinline__ bool fill_block(const Fill& f, int first) {
+  if ((int)blockIdx.x < first) return false;
+  const int64_t n = f.bytes / 16, a = n * f.part / f.parts, z = n * (f.part + 1) / f.parts;
+  const int64_t step = (int64_t)(gridDim.x - first) * blockDim.x;
+  const int64_t t = (int64_t)(blockIdx.x - first) * blockDim.x + threadIdx.x;
+  for (int64_t i = a + t; i < z; i += step) f.p[i] = make_int4(0, 0, 0, 0);
+  if (f.part == 0 && t < f.bytes % 16) reinterpret_cast<char*>(f.p + n)[t] = 0;
+  return true;
+}
+
+// First pass: digit counts per block; zeroes the later passes' counts.
 __global__ void __launch_bounds__(kThreads)
-sort_count_kernel(SortIn in, int64_t n, int bins, uint32_t* __restrict__ counts, int64_t rest,
-                  uint32_t* __restrict__ n_pieces) {
+sort_count_kernel(SortIn in, int64_t n, int bins, int blocks, uint32_t* __restrict__ counts,
+                  int64_t rest, bool by_digit, Fill fill) {
   __shared__ uint32_t h[kMaxBins];
+  before_next();
+  if (fill_block(fill, blocks)) return;
   for (int b = threadIdx.x; b < bins; b += kThreads) h[b] = 0;
-  const int64_t mine = (int64_t)bins * gridDim.x;
+  const int64_t mine = (int64_t)bins * blocks;
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rest;
-       i += (int64_t)gridDim.x * kThreads)
+       i += (int64_t)blocks * kThreads)
     counts[mine + i] = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *n_pieces = 0;
   __syncthreads();
   const int64_t i0 = (int64_t)blockIdx.x * kChunk, i1 = min(n, i0 + kChunk);
   for (int64_t i = i0 + threadIdx.x; i < i1; i += kThreads)
     atomicAdd(&h[sort_key(in, i) & (bins - 1)], 1u);
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += kThreads)
-    counts[(int64_t)b * gridDim.x + blockIdx.x] = h[b];
+    counts[count_at(b, blockIdx.x, bins, blocks, by_digit)] = h[b];
 }
 
 // Exclusive scan of one value per thread over the block; `sums`: 32 words.
@@ -158,6 +171,8 @@ __device__ __forceinline__ uint32_t block_exclusive(uint32_t x, uint32_t* sums, 
 __global__ void __launch_bounds__(1024) scan_kernel(uint32_t* __restrict__ v, int64_t n) {
   __shared__ uint32_t sums[32];
   uint32_t carry = 0;
+  before_next();
+  after_previous();
   for (int64_t i0 = 0; i0 < n; i0 += 1024) {
     const int64_t i = i0 + threadIdx.x;
     uint32_t total;
@@ -170,14 +185,17 @@ __global__ void __launch_bounds__(1024) scan_kernel(uint32_t* __restrict__ v, in
 // counts: digit counts per block (`scanned`: their exclusive scan); next: the
 // next pass's counts, which this one adds up, or null.
 __global__ void __launch_bounds__(kThreads)
-sort_scatter_kernel(SortIn in, int64_t n, int shift, int bins, const uint32_t* __restrict__ counts,
-                    bool scanned, uint32_t* __restrict__ next, uint32_t* __restrict__ keys_out,
-                    uint32_t* __restrict__ pos_out) {
+sort_scatter_kernel(SortIn in, int64_t n, int shift, int bins, int blocks,
+                    const uint32_t* __restrict__ counts, bool scanned, uint32_t* __restrict__ next,
+                    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out, Fill fill) {
   __shared__ uint32_t h[kWarps][kMaxBins];
   __shared__ uint32_t start[kMaxBins];
   __shared__ uint32_t sums[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = gridDim.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  before_next();
+  if (fill_block(fill, blocks)) return;      // touches nothing of the kernel before
   for (int b = threadIdx.x; b < kWarps * kMaxBins; b += kThreads) (&h[0][0])[b] = 0;
+  after_previous();
   const int64_t w0 = (int64_t)blockIdx.x * kChunk + warp * kWarpItems;
   uint32_t key[kWarpItems / 32];
 #pragma unroll
@@ -188,7 +206,7 @@ sort_scatter_kernel(SortIn in, int64_t n, int shift, int bins, const uint32_t* _
   // where this block's elements of each digit begin
   if (scanned) {
     for (int b = threadIdx.x; b < bins; b += kThreads)
-      start[b] = counts[(int64_t)b * blocks + blockIdx.x];
+      start[b] = counts[count_at(b, blockIdx.x, bins, blocks, true)];
     __syncthreads();
   } else {
     uint32_t carry = 0;
@@ -196,8 +214,9 @@ sort_scatter_kernel(SortIn in, int64_t n, int shift, int bins, const uint32_t* _
       const int b = b0 + threadIdx.x;
       uint32_t all = 0, before = 0;
       if (b < bins)
+#pragma unroll 8
         for (int j = 0; j < blocks; ++j) {
-          const uint32_t c = counts[(int64_t)b * blocks + j];
+          const uint32_t c = counts[count_at(b, j, bins, blocks, false)];
           all += c;
           if (j < (int)blockIdx.x) before += c;
         }
@@ -239,84 +258,31 @@ sort_scatter_kernel(SortIn in, int64_t n, int shift, int bins, const uint32_t* _
       keys_out[at] = key[u];
       pos_out[at] = in.ids ? (uint32_t)i : in.pos[i];
       if (next)
-        atomicAdd(&next[(int64_t)((key[u] >> (shift + __popc(bins - 1))) & (bins - 1)) * blocks +
-                        at / kChunk], 1u);
+        atomicAdd(&next[count_at((key[u] >> (shift + __popc(bins - 1))) & (bins - 1), at / kChunk,
+                                 bins, blocks, scanned)], 1u);
     }
   }
 }
 
-// The piece list of a row of more than kShort positions.
-__device__ __forceinline__ void list_pieces(uint32_t v, uint32_t from, uint32_t to,
-                                            uint32_t* n_pieces, Piece* pieces, uint32_t* joins,
-                                            int chunks) {
-  const uint32_t len = to - from, count = (len + kPiece - 1) / kPiece;
-  const uint32_t first = atomicAdd(n_pieces, count);
-  for (uint32_t p = 0; p < count; ++p)
-    pieces[first + p] = Piece{v, from + p * kPiece, min((uint32_t)kPiece, len - p * kPiece), first,
-                              count};
-  for (int c = 0; c < chunks; ++c) joins[(int64_t)first * chunks + c] = 0;
-}
-
-// start[v] = number of sorted keys below v, v = 0 .. n_v, and the pieces of the
-// long rows. One thread per position: it fills the gap of keys that end at its
-// own, together with its warp where the gap is long.
-template <class Keys>
-__device__ __forceinline__ void row_starts(Keys keys, uint32_t n, uint32_t n_v, uint32_t i,
-                                           uint32_t* start, uint32_t* n_pieces, Piece* pieces,
-                                           uint32_t* joins, int chunks) {
-  const int lane = threadIdx.x & 31;
-  // keys key[i - 1] + 1 .. key[i] begin at i (i = n: up to n_v)
-  const uint32_t lo = i == 0 ? 0u : i <= n ? keys(i - 1) + 1 : 1u;
-  const uint32_t hi = i < n ? keys(i) : i == n ? n_v : 0u;
-  const bool has = i <= n && lo <= hi;
-  const bool wide = has && hi - lo >= 8;
-  if (has && !wide)
-    for (uint32_t v = lo; v <= hi; ++v) start[v] = i;
-  uint32_t todo = __ballot_sync(0xffffffffu, wide);
-  while (todo) {
-    const int src = __ffs(todo) - 1;
-    todo &= todo - 1;
-    const uint32_t a = __shfl_sync(0xffffffffu, lo, src), z = __shfl_sync(0xffffffffu, hi, src);
-    const uint32_t at = __shfl_sync(0xffffffffu, i, src);
-    for (uint64_t v = (uint64_t)a + lane; v <= z; v += 32) start[v] = at;
-  }
-  if (has && i < n && hi < n_v && i + kShort < n && keys(i + kShort) == hi) {
-    uint32_t a = i + kShort, z = n;          // keys(a) == hi, the run ends in (a, z]
-    while (z - a > 1) {
-      const uint32_t mid = a + (z - a) / 2;
-      if (keys(mid) == hi) a = mid;
-      else z = mid;
-    }
-    list_pieces(hi, i, z, n_pieces, pieces, joins, chunks);
-  }
-}
-
-__global__ void __launch_bounds__(kThreads)
-row_start_kernel(const uint32_t* __restrict__ keys, uint32_t n, uint32_t n_v,
-                 uint32_t* __restrict__ start, uint32_t* __restrict__ n_pieces,
-                 Piece* __restrict__ pieces, uint32_t* __restrict__ joins, int chunks) {
-  row_starts([&](uint32_t i) { return keys[i]; }, n, n_v, blockIdx.x * kThreads + threadIdx.x,
-             start, n_pieces, pieces, joins, chunks);
-}
-
-// Everything up to the row starts for n <= kSmallSort, one block.
-constexpr int kSmallWarps = kSmallSort / kWarpItems;
+// The whole sort for n <= kSmallSort in one block (the others clear).
+constexpr int kSmallItems = 256;              // elements of a warp
+constexpr int kSmallWarps = kSmallSort / kSmallItems;
 constexpr int kSmallThreads = kSmallWarps * 32;
 __global__ void __launch_bounds__(kSmallThreads)
-small_sort_kernel(SortIn in, int n, int passes, int bits, uint32_t* __restrict__ pos_out,
-                  uint32_t* __restrict__ start, uint32_t* __restrict__ n_pieces,
-                  Piece* __restrict__ pieces, uint32_t* __restrict__ joins, int chunks) {
+small_sort_kernel(SortIn in, int n, int passes, int bits, uint32_t* __restrict__ keys_out,
+                  uint32_t* __restrict__ pos_out, Fill fill) {
   extern __shared__ uint32_t sm[];
   uint32_t* keys = sm;
   uint32_t* pos = sm + kSmallSort;
   uint32_t* h = sm + 2 * kSmallSort;             // [kSmallWarps][bins]
   __shared__ uint32_t sums[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bins = 1 << bits;
-  if (threadIdx.x == 0) *n_pieces = 0;
-  const int w0 = warp * kWarpItems;
-  uint32_t key[kWarpItems / 32], p[kWarpItems / 32];
+  before_next();
+  if (fill_block(fill, 1)) return;
+  const int w0 = warp * kSmallItems;
+  uint32_t key[kSmallItems / 32], p[kSmallItems / 32];
 #pragma unroll
-  for (int u = 0; u < kWarpItems / 32; ++u) {
+  for (int u = 0; u < kSmallItems / 32; ++u) {
     const int i = w0 + u * 32 + lane;
     key[u] = i < n ? id_key(in, i) : 0xffffffffu;
     p[u] = i;
@@ -326,7 +292,7 @@ small_sort_kernel(SortIn in, int n, int passes, int bits, uint32_t* __restrict__
     for (int b = threadIdx.x; b < kSmallWarps * bins; b += kSmallThreads) h[b] = 0;
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kWarpItems / 32; ++u)
+    for (int u = 0; u < kSmallItems / 32; ++u)
       if (w0 + u * 32 + lane < n) atomicAdd(&h[warp * bins + ((key[u] >> shift) & (bins - 1))], 1u);
     __syncthreads();
     // one digit a thread (bins <= 512 threads), its warps one after the other
@@ -342,7 +308,7 @@ small_sort_kernel(SortIn in, int n, int passes, int bits, uint32_t* __restrict__
       }
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kWarpItems / 32; ++u) {
+    for (int u = 0; u < kSmallItems / 32; ++u) {
       const bool in_range = w0 + u * 32 + lane < n;
       const uint32_t bin = in_range ? (key[u] >> shift) & (bins - 1) : 0xffffffffu;
       const uint32_t peers = __match_any_sync(0xffffffffu, bin);
@@ -360,159 +326,171 @@ small_sort_kernel(SortIn in, int n, int passes, int bits, uint32_t* __restrict__
     __syncthreads();
     if (pass + 1 < passes)
 #pragma unroll
-      for (int u = 0; u < kWarpItems / 32; ++u) {
+      for (int u = 0; u < kSmallItems / 32; ++u) {
         const int i = w0 + u * 32 + lane;
         if (i < n) key[u] = keys[i], p[u] = pos[i];
       }
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < n; i += kSmallThreads) pos_out[i] = pos[i];
-  for (int i0 = 0; i0 <= n; i0 += kSmallThreads)
-    row_starts([&](uint32_t i) { return keys[i]; }, n, (uint32_t)in.n_v, i0 + threadIdx.x, start,
-               n_pieces, pieces, joins, chunks);
+  for (int i = threadIdx.x; i < n; i += kSmallThreads) {
+    keys_out[i] = keys[i];
+    pos_out[i] = pos[i];
+  }
 }
 
+// ---- sums of rows ----------------------------------------------------------------
+// After the sort a table row's positions lie side by side: a run. A warp takes
+// a window of `width` sorted positions and kCols vectors a lane of their
+// columns, whatever runs lie in it, so all warps read the same amount; a run
+// inside the window is written where it ends, one that crosses the window's
+// edges leaves its part (head: begun before the window; tail: begun in it) and
+// join_kernel adds a run's parts in order. The id that takes a tenth of a batch
+// costs what its rows cost.
 struct SumArgs {
-  const uint32_t *start, *pos, *n_pieces;
-  const Piece* pieces;
-  uint32_t* joins;
+  const uint32_t *keys, *pos;
   const void* yb;
-  void *wb, *part;
+  void *wb, *part;       // part: [window][head, tail][n_d]
   double scale;
-  int64_t n_v;
-  int n_d, chunks, piece_blocks;
+  int64_t n, n_v;
+  int n_d, width, chunks;
   bool add;
 };
 
-// The sum of one vector of columns over positions from .. from + len - 1, in order.
-template <class T, int VEC>
-__device__ __forceinline__ void sum_rows(const uint32_t* __restrict__ pos, uint32_t from,
-                                         uint32_t len, const T* __restrict__ yb, int n_d, int col,
-                                         acc_t<T> (&acc)[VEC]) {
-  using V = Vec<T, VEC>;
-  constexpr int U = 8;
+// A vector of VEC columns is 16 bytes of the gradient: 4 Float32 (read as 8 or
+// 16 bytes of yb), 2 Float64, or single columns where rows do not allow it.
+template <class A, int VEC>
+__device__ __forceinline__ void put(A* p, const A (&v)[VEC], A scale, bool add) {
+  Vec<A, VEC> o;
+  if (add) o = *reinterpret_cast<const Vec<A, VEC>*>(p);
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) acc[k] = 0;
-  for (uint32_t i = 0; i < len; i += U) {
+  for (int k = 0; k < VEC; ++k) o.v[k] = add ? o.v[k] + v[k] * scale : v[k] * scale;
+  *reinterpret_cast<Vec<A, VEC>*>(p) = o;
+}
+
+constexpr int kCols = 4;         // vectors of a lane that a warp sums at once
+constexpr int kMaxWidth = 64;
+
+template <class T, int VEC>
+__global__ void __launch_bounds__(kThreads)
+window_sum_kernel(SumArgs p) {
+  using A = acc_t<T>;
+  using V = Vec<T, VEC>;
+  constexpr int kSpan = 32 * VEC * kCols, U = 4;
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int64_t win = item / p.chunks, p0 = win * p.width;
+  if (p0 >= p.n) return;
+  const int col = (int)(item % p.chunks) * kSpan + lane * VEC;
+  before_next();
+  after_previous();
+  const int len = (int)min((int64_t)p.width, p.n - p0);
+  const uint32_t none = (uint32_t)p.n_v;
+  // this window's keys and positions, two a lane, and the keys beside it
+  uint32_t key[2], at[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const bool in = 32 * h + lane < len;
+    key[h] = in ? p.keys[p0 + 32 * h + lane] : none;
+    at[h] = in ? p.pos[p0 + 32 * h + lane] : 0u;
+  }
+  const uint32_t before = p0 > 0 ? p.keys[p0 - 1] : 0xffffffffu;
+  const uint32_t after = p0 + len < p.n ? p.keys[p0 + len] : 0xffffffffu;
+  auto key_of = [&](int i) {
+    return __shfl_sync(0xffffffffu, i < 32 ? key[0] : key[1], i & 31);
+  };
+  const T* yb = (const T*)p.yb;
+  const A scale = (A)p.scale;
+  A acc[kCols][VEC] = {};
+  int first = 0;                       // where the current run begins in the window
+  for (int i0 = 0; i0 < len; i0 += U) {
+    if (key_of(i0) == none) break;     // padding sorts last
+    V r[U][kCols];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u;
+      const uint32_t row = __shfl_sync(0xffffffffu, i < 32 ? at[0] : at[1], i & 31);
+      if (i < len) {
+        const T* q = yb + (int64_t)row * p.n_d + col;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+          if (col + c * 32 * VEC < p.n_d) r[u][c] = *reinterpret_cast<const V*>(q + c * 32 * VEC);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u;
+      const uint32_t k = key_of(i < len ? i : 0), k1 = key_of(i + 1 < len ? i + 1 : 0);
+      if (i >= len || k == none) break;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+        if (col + c * 32 * VEC < p.n_d)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) acc[c][j] += load_acc<T>(r[u][c].v[j]);
+      const bool edge = i + 1 == len;
+      if (!edge && k1 == k) continue;
+      // the run, or the window's share of it, ends here
+      const bool begun = first > 0 || before != k, ended = !edge || after != k;
+      const bool whole = begun && ended;
+      A* o = whole ? (A*)p.wb + (int64_t)k * p.n_d
+                   : (A*)p.part + (2 * win + (begun ? 1 : 0)) * p.n_d;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+        if (col + c * 32 * VEC < p.n_d) {
+          put<A, VEC>(o + col + c * 32 * VEC, acc[c], whole ? scale : A(1), whole && p.add);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) acc[c][j] = 0;
+        }
+      first = i + 1;
+    }
+  }
+}
+
+// A run that begins in a window and goes on past it: its tail there, then the
+// heads of the windows that follow, in order.
+template <class A, int VEC>
+__global__ void __launch_bounds__(kThreads)
+join_kernel(SumArgs p) {
+  constexpr int kSpan = 32 * VEC, U = 16;
+  const int lane = threadIdx.x & 31;
+  const int chunks = (p.n_d + kSpan - 1) / kSpan;
+  const int64_t item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int64_t win = item / chunks, p1 = (win + 1) * p.width;
+  if (p1 >= p.n) return;
+  after_previous();
+  const uint32_t k = p.keys[p1 - 1];
+  if (k == (uint32_t)p.n_v || p.keys[p1] != k) return;
+  const int64_t p0 = win * p.width;
+  if (p0 > 0 && p.keys[p0 - 1] == k) return;     // begun before this window
+  // heads: of window win + 1 + j while its first key is k
+  int64_t heads = 0;
+  for (;;) {
+    const int64_t q = p1 + (heads + lane) * p.width;
+    const uint32_t same = __ballot_sync(0xffffffffu, q < p.n && p.keys[min(q, p.n - 1)] == k);
+    const int run = same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+    heads += run;
+    if (run < 32) break;
+  }
+  const int col = (int)(item % chunks) * kSpan + lane * VEC;
+  if (col >= p.n_d) return;
+  const A* part = (const A*)p.part + col;
+  using V = Vec<A, VEC>;
+  const V t = *reinterpret_cast<const V*>(part + (2 * win + 1) * p.n_d);
+  A acc[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) acc[j] = t.v[j];
+  for (int64_t h = 0; h < heads; h += U) {
     V r[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (i + u < len)
-        r[u] = *reinterpret_cast<const V*>(yb + (int64_t)pos[from + i + u] * n_d + col);
+      if (h + u < heads)
+        r[u] = *reinterpret_cast<const V*>(part + 2 * (win + 1 + h + u) * p.n_d);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (i + u < len)
+      if (h + u < heads)
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] += load_acc<T>(r[u].v[k]);
+        for (int j = 0; j < VEC; ++j) acc[j] += r[u].v[j];
   }
-}
-
-// VEC columns of a gradient row, in pieces of 16 bytes.
-template <class A, int VEC>
-__device__ __forceinline__ void put(A* p, const A (&v)[VEC], A scale, bool add) {
-  constexpr int W = VEC * sizeof(A) >= 16 ? 16 / (int)sizeof(A) : VEC;
-#pragma unroll
-  for (int i = 0; i < VEC; i += W) {
-    Vec<A, W> o;
-    if (add) o = *reinterpret_cast<const Vec<A, W>*>(p + i);
-#pragma unroll
-    for (int k = 0; k < W; ++k) o.v[k] = add ? o.v[k] + v[i + k] * scale : v[i + k] * scale;
-    *reinterpret_cast<Vec<A, W>*>(p + i) = o;
-  }
-}
-
-constexpr int kRowsPerWarp = 8;
-
-// Blocks 0 .. piece_blocks - 1 take the pieces of long rows, the others eight
-// table rows a warp, zeros included.
-template <class T, int VEC>
-__global__ void __launch_bounds__(kThreads)
-row_sum_kernel(SumArgs p) {
-  using A = acc_t<T>;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const T* yb = (const T*)p.yb;
-  A* wb = (A*)p.wb;
-  const A scale = (A)p.scale;
-  if ((int)blockIdx.x < p.piece_blocks) {
-    __shared__ A sm[kWarps][32 * VEC];
-    __shared__ bool last;
-    const uint32_t items = *p.n_pieces * (uint32_t)p.chunks;
-    for (uint32_t it = blockIdx.x; it < items; it += p.piece_blocks) {
-      const Piece q = p.pieces[it / p.chunks];
-      const int chunk = it % p.chunks, col = (chunk * 32 + lane) * VEC;
-      const uint32_t sub = (q.len + kWarps - 1) / kWarps, i0 = min(q.len, warp * sub);
-      A acc[VEC];
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) acc[k] = 0;
-      if (col < p.n_d)
-        sum_rows<T, VEC>(p.pos, q.from + i0, min(sub, q.len - i0), yb, p.n_d, col, acc);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) sm[warp][k * 32 + lane] = acc[k];
-      __syncthreads();
-      A* part = (A*)p.part;
-      if (warp == 0 && col < p.n_d) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          acc[k] = sm[0][k * 32 + lane];
-#pragma unroll
-          for (int w = 1; w < kWarps; ++w) acc[k] += sm[w][k * 32 + lane];
-        }
-        if (q.count == 1)
-          put<A, VEC>(wb + (int64_t)q.v * p.n_d + col, acc, scale, p.add);
-        else
-          put<A, VEC>(part + (int64_t)(it / p.chunks) * p.n_d + col, acc, A(1), false);
-      }
-      if (q.count > 1) {
-        // the last block of this row and these columns adds the pieces in order
-        if (warp == 0) {
-          __threadfence();
-          __syncwarp();
-          if (lane == 0)
-            last = atomicAdd(&p.joins[(int64_t)q.first * p.chunks + chunk], 1u) == q.count - 1;
-        }
-        __syncthreads();
-        if (last && warp == 0 && col < p.n_d) {
-          __threadfence();
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) acc[k] = 0;
-          constexpr int U = 4;
-          for (uint32_t j = 0; j < q.count; j += U) {
-            Vec<A, VEC> r[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-              if (j + u < q.count)
-#pragma unroll
-                for (int k = 0; k < VEC; ++k)
-                  r[u].v[k] = __ldcg(part + (int64_t)(q.first + j + u) * p.n_d + col + k);
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-              if (j + u < q.count)
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) acc[k] += r[u].v[k];
-          }
-          put<A, VEC>(wb + (int64_t)q.v * p.n_d + col, acc, scale, p.add);
-        }
-      }
-      __syncthreads();
-    }
-    return;
-  }
-  const int64_t v0 =
-      ((int64_t)(blockIdx.x - p.piece_blocks) * (kThreads / 32) + warp) * kRowsPerWarp;
-  if (v0 >= p.n_v) return;
-  const uint32_t bound = lane <= kRowsPerWarp && v0 + lane <= p.n_v ? p.start[v0 + lane] : 0u;
-  const int rows = (int)min((int64_t)kRowsPerWarp, p.n_v - v0);
-  for (int q = 0; q < rows; ++q) {
-    const uint32_t i0 = __shfl_sync(0xffffffffu, bound, q);
-    const uint32_t len = __shfl_sync(0xffffffffu, bound, q + 1) - i0;
-    if (len > kShort || (p.add && len == 0)) continue;
-    A* row = wb + (v0 + q) * p.n_d;
-    for (int col = lane * VEC; col < p.n_d; col += 32 * VEC) {
-      A acc[VEC];
-      sum_rows<T, VEC>(p.pos, i0, len, yb, p.n_d, col, acc);
-      put<A, VEC>(row + col, acc, scale, p.add);
-    }
-  }
+  put<A, VEC>((A*)p.wb + (int64_t)k * p.n_d + col, acc, (A)p.scale, p.add);
 }
 
 struct SortPlan {
@@ -530,22 +508,35 @@ SortPlan sort_plan(int64_t n_s, int64_t n_v) {
   return p;
 }
 
-// Columns a warp covers at once: a vector of VEC a lane.
+// Calls f(VEC): 16 bytes of the 16-bit type (forward) or of the gradient
+// (reverse) where alignment allows it, else 4 bytes forward, else one value.
 template <class T, class F>
-stade_status with_vec(int align_t, int align_p, F&& f) {
+stade_status with_fwd_vec(int align, F&& f) {
   using std::integral_constant;
-  constexpr int W = 16 / (int)sizeof(T);
-  if (align_t >= 16 && align_p >= 16) return f(integral_constant<int, W>{});
+  if (align >= 16) return f(integral_constant<int, 16 / (int)sizeof(T)>{});
   if constexpr (sizeof(T) == 2)
-    if (align_t >= 4 && align_p >= 8) return f(integral_constant<int, 2>{});
+    if (align >= 4) return f(integral_constant<int, 2>{});
   return f(integral_constant<int, 1>{});
 }
-int64_t most_pieces(int64_t n_s) { return n_s / (kShort + 1) + n_s / kPiece + 1; }
+template <class T, class F>
+stade_status with_sum_vec(int align_t, int align_p, F&& f) {
+  using std::integral_constant;
+  constexpr int W = 16 / (int)sizeof(acc_t<T>);
+  if (align_t >= W * (int)sizeof(T) && align_p >= 16) return f(integral_constant<int, W>{});
+  return f(integral_constant<int, 1>{});
+}
+// Positions of a window: as many as leave eight warps an SM something to do (a
+// warp's four rows in flight are 4 KB of 16-bit values; narrower windows leave
+// more parts to join: 104 us against 96 with 24 warps an SM, 32768 x 1024 bf16).
+int window_width(int64_t n_s, int64_t chunks) {
+  int w = kMaxWidth;
+  while (w > 8 && n_s * chunks / w < 148 * 8) w /= 2;
+  return w;
+}
 
 struct Scratch {
-  uint32_t *keys[2], *pos[2], *counts, *start, *n_pieces, *joins;
-  Piece* pieces;
-  char* part;
+  uint32_t *keys[2], *pos[2], *counts;
+  double* part;
 };
 // S: Sizer or Carver
 template <class S>
@@ -561,12 +552,9 @@ Scratch layout(S& z, int64_t n_s, int64_t n_v, int64_t n_d) {
     take(&s.pos[i], n_s);
   }
   take(&s.counts, sort_plan(n_s, n_v).counts());
-  take(&s.start, n_v + 1);
-  take(&s.n_pieces, 1);
-  take(&s.pieces, most_pieces(n_s));
-  take(&s.joins, most_pieces(n_s) * ((n_d + 31) / 32));
-  // partial sums: only of rows of more than kPiece positions
-  if (n_s > kPiece) take(&s.part, (size_t)most_pieces(n_s) * n_d * 8);
+  // the widest windows' parts, or the narrowest's of a short batch
+  const int64_t wins = std::min<int64_t>((n_s + 7) / 8, (n_s + kMaxWidth - 1) / kMaxWidth + 148 * 16);
+  take(&s.part, 2 * wins * n_d);
   return s;
 }
 
@@ -605,7 +593,7 @@ extern "C" stade_status stade_embed(int dtype, const void* w, const int64_t* ids
   PhaseScope ph("embed", s);
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    return with_vec<T>(row_align(n_d * sizeof(T), {w, y}), 16, [&](auto vec) {
+    return with_fwd_vec<T>(row_align(n_d * sizeof(T), {w, y}), [&](auto vec) {
       embed_fwd_kernel<T, decltype(vec)::value>
           <<<ceil_div_u(n_s, kFwdRows * (kThreads / 32)), kThreads, 0, s>>>(
               (const T*)w, ids, (T*)y, (acc_t<T>)scale, base, n_s, n_v, (int)n_d);
@@ -648,58 +636,61 @@ extern "C" stade_status stade_embed_b(int dtype, void* wb, const int64_t* ids, v
     st = with_dtype(dtype, [&](auto t) {
       using T = decltype(t);
       using A = acc_t<T>;
-      return with_vec<T>(row_align(n_d * sizeof(T), {yb}), row_align(n_d * sizeof(A), {wb}),
-                         [&](auto vec) {
+      return with_sum_vec<T>(row_align(n_d * sizeof(T), {yb}), row_align(n_d * sizeof(A), {wb}),
+                             [&](auto vec) -> stade_status {
         constexpr int VEC = decltype(vec)::value;
-        const int chunks = (int)((n_d + 32 * VEC - 1) / (32 * VEC));
-        const uint32_t* pos;
+        const int chunks = (int)((n_d + 32 * VEC * kCols - 1) / (32 * VEC * kCols));
+        const int64_t bytes = n_v * n_d * (int64_t)sizeof(A);
+        const bool whole = row_align(16, {wb}) == 16;     // 16-byte pieces can clear it
+        if (!add && !whole) STADE_CUDA(cudaMemsetAsync(wb, 0, bytes, s));
+        const int clearers =
+            add || !whole ? 0 : (int)std::min<int64_t>(148 * 4, bytes / 16384 + 1);
+        Fill fill{static_cast<int4*>(wb), bytes, 0, 1};
+        int last = 0;
         if (n_s <= kSmallSort) {
           const size_t smem = (2 * kSmallSort + (size_t)kSmallWarps * bins) * 4;
           STADE_CUDA(cudaFuncSetAttribute(small_sort_kernel,
                                           cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-          small_sort_kernel<<<1, kSmallThreads, smem, s>>>(
-              SortIn{ids, nullptr, nullptr, base, n_v}, (int)n_s, p.passes, p.bits, sc.pos[0],
-              sc.start, sc.n_pieces, sc.pieces, sc.joins, chunks);
+          small_sort_kernel<<<1 + clearers, kSmallThreads, smem, s>>>(
+              SortIn{ids, nullptr, nullptr, base, n_v}, (int)n_s, p.passes, p.bits, sc.keys[0],
+              sc.pos[0], fill);
           STADE_CHECK_LAUNCH();
-          pos = sc.pos[0];
         } else {
           const int64_t per_pass = p.blocks << p.bits;
+          const bool scan = p.blocks > kFusedScan;
+          fill.parts = p.passes + 1;
           for (int i = 0; i < p.passes; ++i) {
             const SortIn in{i == 0 ? ids : nullptr, sc.keys[(i + 1) & 1], sc.pos[(i + 1) & 1], base,
                             n_v};
             uint32_t* counts = sc.counts + i * per_pass;
             if (i == 0) {
-              sort_count_kernel<<<(unsigned)p.blocks, kThreads, 0, s>>>(
-                  in, n_s, bins, counts, (p.passes - 1) * per_pass, sc.n_pieces);
+              sort_count_kernel<<<(unsigned)p.blocks + clearers, kThreads, 0, s>>>(
+                  in, n_s, bins, (int)p.blocks, counts, (p.passes - 1) * per_pass, scan, fill);
               STADE_CHECK_LAUNCH();
             }
-            const bool scan = p.blocks > kFusedScan;
             if (scan) {
-              scan_kernel<<<1, 1024, 0, s>>>(counts, per_pass);
-              STADE_CHECK_LAUNCH();
+              st = launch_next(scan_kernel, 1, 1024, 0, s, counts, per_pass);
+              if (st != STADE_OK) return st;
             }
-            sort_scatter_kernel<<<(unsigned)p.blocks, kThreads, 0, s>>>(
-                in, n_s, i * p.bits, bins, counts, scan,
-                i + 1 < p.passes ? counts + per_pass : nullptr, sc.keys[i & 1], sc.pos[i & 1]);
-            STADE_CHECK_LAUNCH();
+            fill.part = i + 1;
+            st = launch_next(sort_scatter_kernel, (unsigned)p.blocks + clearers, kThreads, 0, s, in,
+                             n_s, i * p.bits, bins, (int)p.blocks, counts, scan,
+                             i + 1 < p.passes ? counts + per_pass : nullptr, sc.keys[i & 1],
+                             sc.pos[i & 1], fill);
+            if (st != STADE_OK) return st;
           }
-          const int last = (p.passes - 1) & 1;
-          row_start_kernel<<<ceil_div_u(n_s + 1, kThreads), kThreads, 0, s>>>(
-              sc.keys[last], (uint32_t)n_s, (uint32_t)n_v, sc.start, sc.n_pieces, sc.pieces,
-              sc.joins, chunks);
-          STADE_CHECK_LAUNCH();
-          pos = sc.pos[last];
+          last = (p.passes - 1) & 1;
         }
-        SumArgs a{sc.start, pos, sc.n_pieces, sc.pieces, sc.joins, yb, wb, sc.part, scale, n_v,
-                  (int)n_d, chunks, 0, add};
-        // blocks for the pieces, where there can be any
-        a.piece_blocks =
-            n_s > kShort ? (int)std::min<int64_t>(148 * 4, most_pieces(n_s) * chunks) : 0;
-        const int64_t row_blocks =
-            (n_v + kRowsPerWarp * (kThreads / 32) - 1) / (kRowsPerWarp * (kThreads / 32));
-        row_sum_kernel<T, VEC><<<(unsigned)(a.piece_blocks + row_blocks), kThreads, 0, s>>>(a);
-        STADE_CHECK_LAUNCH();
-        return (stade_status)STADE_OK;
+        const int width = window_width(n_s, chunks);
+        const SumArgs a{sc.keys[last], sc.pos[last], yb, wb, sc.part, scale, n_s, n_v, (int)n_d,
+                        width, chunks, add};
+        const int64_t wins = (n_s + width - 1) / width;
+        st = launch_next(window_sum_kernel<T, VEC>, ceil_div_u(wins * chunks, kWarps), kThreads, 0, s,
+                         a);
+        if (st != STADE_OK || wins == 1) return st;
+        const int64_t join_chunks = (n_d + 32 * VEC - 1) / (32 * VEC);
+        return launch_next(join_kernel<A, VEC>, ceil_div_u((wins - 1) * join_chunks, kWarps),
+                           kThreads, 0, s, a);
       });
     });
     if (st != STADE_OK) return st;

@@ -127,6 +127,37 @@ template <> __device__ __forceinline__ Vec<__half, 2> narrow2<__half>(Pair<float
   return *reinterpret_cast<const Vec<__half, 2>*>(&h);
 }
 
+// ---- launches that overlap the kernel before them ---------------------------------
+// Kernels of one call that follow each other: launched with
+// programmatic stream serialisation, a kernel's blocks are set up while the one
+// before is still running; after_previous(), before any access to memory, waits
+// until that one has completed. Only for kernels whose predecessor in the
+// stream is a kernel of the same call.
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// Lets the next kernel's blocks be set up from here on.
+__device__ __forceinline__ void before_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+template <class... P, class... A>
+stade_status launch_next(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
+                         A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  STADE_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+  count_launch();
+  return STADE_OK;
+}
+
 inline bool known_dtype(int d) {
   return d == STADE_F32 || d == STADE_F64 || d == STADE_BF16 || d == STADE_F16;
 }

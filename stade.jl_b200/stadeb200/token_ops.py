@@ -19,26 +19,52 @@ import ctypes as C
 
 import torch
 
-from ._lib import (STADE_ADJ_STORE, STADE_BF16, STADE_F16, STADE_F32, STADE_F64, STADE_SEED_KEEP,
-                   check, lib)
-from .kernels import _arr, _opts
+from ._lib import (STADE_ADJ_STORE, STADE_BF16, STADE_F16, STADE_F32, STADE_F64, STADE_OK,
+                   STADE_SEED_KEEP, check, lib, stade_opts)
+from .kernels import _arr
 
 _DTYPES = {torch.float32: STADE_F32, torch.float64: STADE_F64, torch.bfloat16: STADE_BF16,
            torch.float16: STADE_F16}
 ACTIVATIONS = {"relu": 1, "tanh": 2, "silu": 3, "gelu": 4}
 
 
+_TYPES = {t: (code, t, torch.float64 if t == torch.float64 else torch.float32)
+          for t, code in _DTYPES.items()}
+
+
 def _dtype(t, name: str):
     """(dtype code, element type, parameter type) by an activation array."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a CUDA tensor, got {type(t).__name__}")
-    code = _DTYPES.get(t.dtype)
-    if code is None:
+    types = _TYPES.get(t.dtype)
+    if types is None:
         raise TypeError(f"{name}: unsupported dtype {t.dtype}")
-    if t.is_cuda and t.device.index != torch.cuda.current_device():
+    if t.is_cuda and t.get_device() != torch.cuda.current_device():
         raise ValueError(f"{name}: tensor lives on {t.device}, the current device is "
                          f"cuda:{torch.cuda.current_device()}")
-    return code, t.dtype, torch.float64 if t.dtype == torch.float64 else torch.float32
+    return types
+
+
+# The current stream's handle without building a Stream object, which costs as
+# much as the launch of a kernel.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _run(fn, *args, stream=None, workspace=None, flags=0) -> None:
+    if stream is not None:
+        handle = stream.cuda_stream
+    elif _raw_stream is not None:
+        handle = _raw_stream(torch.cuda.current_device())
+    else:
+        handle = torch.cuda.current_stream().cuda_stream
+    if workspace is None:
+        o = stade_opts(handle, None, 0, flags)
+    else:
+        o = stade_opts(handle, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                       flags)
+    code = fn(*args, C.byref(o))
+    if code != STADE_OK:
+        check(code)
 
 
 def _opt(t, dtype, n, name):
@@ -49,10 +75,9 @@ def _flags(accumulate: bool, consume: bool) -> int:
     return (0 if accumulate else STADE_ADJ_STORE) | (0 if consume else STADE_SEED_KEEP)
 
 
-def _sizes(**kw) -> None:
-    for name, n in kw.items():
-        if n < 0:
-            raise ValueError(f"{name}: negative size {n}")
+def _sizes(*sizes) -> None:
+    if min(sizes) < 0:
+        raise ValueError(f"negative size in {sizes}")
 
 
 def _act(act: str) -> int:
@@ -65,23 +90,21 @@ def _act(act: str) -> int:
 def embed_cuda(w, ids, y, scale, n_s, n_v, n_d, *, base=0, stream=None):
     """y[s] = scale w[ids[s] - base]; ids below base are padding (zero rows).
     ids: int64. Gathers rows of any n_v x n_d array by an index list."""
-    _sizes(n_s=n_s, n_v=n_v, n_d=n_d)
+    _sizes(n_s, n_v, n_d)
     code, T, _ = _dtype(y, "y")
-    check(lib().stade_embed(code, _arr(w, T, n_v * n_d, "w"), _arr(ids, torch.int64, n_s, "ids"),
-                            _arr(y, T, n_s * n_d, "y"), float(scale), base, n_s, n_v, n_d,
-                            C.byref(_opts(stream, None))))
+    _run(lib().stade_embed, code, _arr(w, T, n_v * n_d, "w"), _arr(ids, torch.int64, n_s, "ids"),
+         _arr(y, T, n_s * n_d, "y"), float(scale), base, n_s, n_v, n_d, stream=stream)
 
 
 def embed_b_cuda(wb, ids, yb, scale, n_s, n_v, n_d, *, base=0, accumulate=True, consume=True,
                  stream=None, workspace=None):
     """wb[v] += scale * sum of yb[s] over the positions s that hold id v, in
     increasing s (bit-identical from call to call)."""
-    _sizes(n_s=n_s, n_v=n_v, n_d=n_d)
+    _sizes(n_s, n_v, n_d)
     code, T, P = _dtype(yb, "yb")
-    check(lib().stade_embed_b(code, _arr(wb, P, n_v * n_d, "wb"),
-                              _arr(ids, torch.int64, n_s, "ids"), _arr(yb, T, n_s * n_d, "yb"),
-                              float(scale), base, n_s, n_v, n_d,
-                              C.byref(_opts(stream, workspace, _flags(accumulate, consume)))))
+    _run(lib().stade_embed_b, code, _arr(wb, P, n_v * n_d, "wb"),
+         _arr(ids, torch.int64, n_s, "ids"), _arr(yb, T, n_s * n_d, "yb"), float(scale), base, n_s,
+         n_v, n_d, stream=stream, workspace=workspace, flags=_flags(accumulate, consume))
 
 
 def embed_b_workspace(n_s, n_v, n_d) -> int:
@@ -92,26 +115,24 @@ def embed_b_workspace(n_s, n_v, n_d) -> int:
 def layer_norm_cuda(x, w, b, y, m_stack, r_stack, eps, n_s, n_d, *, stream=None):
     """y = (x - mean) rstd w + b over rows of n_d; w and b may be None. The
     tape m_stack, r_stack (n_s each) receives mean and rstd."""
-    _sizes(n_s=n_s, n_d=n_d)
+    _sizes(n_s, n_d)
     code, T, P = _dtype(x, "x")
-    check(lib().stade_layer_norm(code, _arr(x, T, n_s * n_d, "x"), _opt(w, P, n_d, "w"),
-                                 _opt(b, P, n_d, "b"), _arr(y, T, n_s * n_d, "y"),
-                                 _arr(m_stack, P, n_s, "m_stack"), _arr(r_stack, P, n_s, "r_stack"),
-                                 float(eps), n_s, n_d, C.byref(_opts(stream, None))))
+    _run(lib().stade_layer_norm, code, _arr(x, T, n_s * n_d, "x"), _opt(w, P, n_d, "w"),
+         _opt(b, P, n_d, "b"), _arr(y, T, n_s * n_d, "y"), _arr(m_stack, P, n_s, "m_stack"),
+         _arr(r_stack, P, n_s, "r_stack"), float(eps), n_s, n_d, stream=stream)
 
 
 def layer_norm_b_cuda(x, xb, w, wb, bb, yb, m_stack, r_stack, n_s, n_d, *, accumulate=True,
                       consume=True, stream=None, workspace=None):
     """Reverse sweep of layer_norm from x and the tape; xb, wb and bb may be
     None (not wanted)."""
-    _sizes(n_s=n_s, n_d=n_d)
+    _sizes(n_s, n_d)
     code, T, P = _dtype(x, "x")
-    check(lib().stade_layer_norm_b(code, _arr(x, T, n_s * n_d, "x"), _opt(xb, T, n_s * n_d, "xb"),
-                                   _opt(w, P, n_d, "w"), _opt(wb, P, n_d, "wb"),
-                                   _opt(bb, P, n_d, "bb"), _arr(yb, T, n_s * n_d, "yb"),
-                                   _arr(m_stack, P, n_s, "m_stack"),
-                                   _arr(r_stack, P, n_s, "r_stack"), n_s, n_d,
-                                   C.byref(_opts(stream, workspace, _flags(accumulate, consume)))))
+    _run(lib().stade_layer_norm_b, code, _arr(x, T, n_s * n_d, "x"), _opt(xb, T, n_s * n_d, "xb"),
+         _opt(w, P, n_d, "w"), _opt(wb, P, n_d, "wb"), _opt(bb, P, n_d, "bb"),
+         _arr(yb, T, n_s * n_d, "yb"), _arr(m_stack, P, n_s, "m_stack"),
+         _arr(r_stack, P, n_s, "r_stack"), n_s, n_d, stream=stream, workspace=workspace,
+         flags=_flags(accumulate, consume))
 
 
 def layer_norm_b_workspace(dtype, n_s, n_d) -> int:
@@ -135,41 +156,37 @@ def _tape(q, e, n_s, n_d):
 
 def tape8_push_cuda(x, q_stack, e_stack, n_s, n_d, *, stream=None):
     """Writes x to the 8-bit tape."""
-    _sizes(n_s=n_s, n_d=n_d)
+    _sizes(n_s, n_d)
     code, T, _ = _dtype(x, "x")
-    check(lib().stade_tape8_push(code, _arr(x, T, n_s * n_d, "x"),
-                                 *_tape(q_stack, e_stack, n_s, n_d), n_s, n_d,
-                                 C.byref(_opts(stream, None))))
+    _run(lib().stade_tape8_push, code, _arr(x, T, n_s * n_d, "x"),
+         *_tape(q_stack, e_stack, n_s, n_d), n_s, n_d, stream=stream)
 
 
 def tape8_pop_cuda(x, q_stack, e_stack, n_s, n_d, *, stream=None):
     """Restores x from the 8-bit tape (overwrites x)."""
-    _sizes(n_s=n_s, n_d=n_d)
+    _sizes(n_s, n_d)
     code, T, _ = _dtype(x, "x")
-    check(lib().stade_tape8_pop(code, _arr(x, T, n_s * n_d, "x"),
-                                *_tape(q_stack, e_stack, n_s, n_d), n_s, n_d,
-                                C.byref(_opts(stream, None))))
+    _run(lib().stade_tape8_pop, code, _arr(x, T, n_s * n_d, "x"),
+         *_tape(q_stack, e_stack, n_s, n_d), n_s, n_d, stream=stream)
 
 
 def act_tape8_cuda(act, x, y, q_stack, e_stack, n_s, n_d, *, stream=None):
     """y = f(x), f one of relu, tanh, silu, gelu (erf form); x goes to the
     8-bit tape for act_tape8_b."""
-    _sizes(n_s=n_s, n_d=n_d)
+    _sizes(n_s, n_d)
     code, T, _ = _dtype(x, "x")
-    check(lib().stade_act_tape8(code, _act(act), _arr(x, T, n_s * n_d, "x"),
-                                _arr(y, T, n_s * n_d, "y"), *_tape(q_stack, e_stack, n_s, n_d),
-                                n_s, n_d, C.byref(_opts(stream, None))))
+    _run(lib().stade_act_tape8, code, _act(act), _arr(x, T, n_s * n_d, "x"),
+         _arr(y, T, n_s * n_d, "y"), *_tape(q_stack, e_stack, n_s, n_d), n_s, n_d, stream=stream)
 
 
 def act_tape8_b_cuda(act, xb, yb, q_stack, e_stack, n_s, n_d, *, accumulate=True, consume=True,
                      stream=None):
     """xb += yb f'(x^), x^ the input as the 8-bit tape holds it."""
-    _sizes(n_s=n_s, n_d=n_d)
+    _sizes(n_s, n_d)
     code, T, _ = _dtype(yb, "yb")
-    check(lib().stade_act_tape8_b(code, _act(act), _arr(xb, T, n_s * n_d, "xb"),
-                                  _arr(yb, T, n_s * n_d, "yb"), *_tape(q_stack, e_stack, n_s, n_d),
-                                  n_s, n_d,
-                                  C.byref(_opts(stream, None, _flags(accumulate, consume)))))
+    _run(lib().stade_act_tape8_b, code, _act(act), _arr(xb, T, n_s * n_d, "xb"),
+         _arr(yb, T, n_s * n_d, "yb"), *_tape(q_stack, e_stack, n_s, n_d), n_s, n_d, stream=stream,
+         flags=_flags(accumulate, consume))
 
 
 # ---------------------------------------------------------------------------
@@ -177,11 +194,11 @@ def expert_mm_cuda(x, w, y, off, n_s, n_e, n_i, n_o, *, stream=None, workspace=N
     """y[s] = x[s] w[e] for the rows off[e] .. off[e + 1] - 1 of expert e; w:
     n_e x n_i x n_o, off: n_e + 1 rising bounds (int64, on the device). Rows in
     no group get y = 0."""
-    _sizes(n_s=n_s, n_e=n_e, n_i=n_i, n_o=n_o)
+    _sizes(n_s, n_e, n_i, n_o)
     code, T, _ = _dtype(x, "x")
-    check(lib().stade_expert_mm(code, _arr(x, T, n_s * n_i, "x"), _arr(w, T, n_e * n_i * n_o, "w"),
-                                _arr(y, T, n_s * n_o, "y"), _arr(off, torch.int64, n_e + 1, "off"),
-                                n_s, n_e, n_i, n_o, C.byref(_opts(stream, workspace))))
+    _run(lib().stade_expert_mm, code, _arr(x, T, n_s * n_i, "x"), _arr(w, T, n_e * n_i * n_o, "w"),
+         _arr(y, T, n_s * n_o, "y"), _arr(off, torch.int64, n_e + 1, "off"), n_s, n_e, n_i, n_o,
+         stream=stream, workspace=workspace)
 
 
 def expert_mm_workspace(dtype, n_s, n_e, n_i, n_o) -> int:
@@ -192,13 +209,12 @@ def expert_mm_b_cuda(x, xb, w, wb, yb, off, n_s, n_e, n_i, n_o, *, accumulate=Tr
                      stream=None, workspace=None):
     """xb[s] += yb[s] w[e]^T and wb[e] += x^T yb over the rows of expert e; xb
     or wb may be None (not wanted)."""
-    _sizes(n_s=n_s, n_e=n_e, n_i=n_i, n_o=n_o)
+    _sizes(n_s, n_e, n_i, n_o)
     code, T, P = _dtype(yb, "yb")
-    check(lib().stade_expert_mm_b(code, _opt(x, T, n_s * n_i, "x"), _opt(xb, T, n_s * n_i, "xb"),
-                                  _opt(w, T, n_e * n_i * n_o, "w"),
-                                  _opt(wb, P, n_e * n_i * n_o, "wb"), _arr(yb, T, n_s * n_o, "yb"),
-                                  _arr(off, torch.int64, n_e + 1, "off"), n_s, n_e, n_i, n_o,
-                                  C.byref(_opts(stream, workspace, _flags(accumulate, consume)))))
+    _run(lib().stade_expert_mm_b, code, _opt(x, T, n_s * n_i, "x"), _opt(xb, T, n_s * n_i, "xb"),
+         _opt(w, T, n_e * n_i * n_o, "w"), _opt(wb, P, n_e * n_i * n_o, "wb"),
+         _arr(yb, T, n_s * n_o, "yb"), _arr(off, torch.int64, n_e + 1, "off"), n_s, n_e, n_i, n_o,
+         stream=stream, workspace=workspace, flags=_flags(accumulate, consume))
 
 
 def expert_mm_b_workspace(dtype, n_s, n_e, n_i, n_o) -> int:

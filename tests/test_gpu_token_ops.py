@@ -201,7 +201,7 @@ def test_embed_b(n_s, n_v, n_d, off, dt):
     ids = _ids(4, n_s, n_v, 0)
     dev = torch.from_numpy(ids).cuda()
     ref, mag, cnt = R.embed_b(R.f64(yb), ids, 1.7, n_v)
-    wb = torch.full((n_v, n_d), math.nan, dtype=P, device="cuda")
+    wb = _dev(torch.full((n_v, n_d), math.nan), P, off)
     sb.embed_b_cuda(wb, dev, yb, 1.7, n_s, n_v, n_d, accumulate=False, consume=False)
     R.assert_close(wb, ref, mag, cnt.max() + 4, "wb")
     again = torch.full_like(wb, math.nan)
