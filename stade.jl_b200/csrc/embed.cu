@@ -450,7 +450,7 @@ window_sum_kernel(SumArgs p) {
 template <class A, int VEC>
 __global__ void __launch_bounds__(kThreads)
 join_kernel(SumArgs p) {
-  constexpr int kSpan = 32 * VEC, U = 16;
+  constexpr int kSpan = 32 * VEC, U = 8;
   const int lane = threadIdx.x & 31;
   const int chunks = (p.n_d + kSpan - 1) / kSpan;
   const int64_t item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);

@@ -41,85 +41,144 @@ __device__ __forceinline__ float restore(int q, int code) {
 }
 
 // ---- activations -------------------------------------------------------------------
-// FAST (16-bit arrays): errors of a few 1e-7 of 1 + |x|, below a hundredth of
-// what rounding the result costs, at two special-function instructions an
-// element. With CUDA's erff, expf and tanhf a gelu step of 8192 x 8192 in bf16
-// was bound by their instructions (213 us, 103 us by memory). Float32 arrays
-// use those.
-
-// 1 - Phi(z), z >= 0, and exp(-z^2 / 2): the rational approximation 7.1.26 of
-// Abramowitz and Stegun for erfc(z / sqrt 2), error at most 1.5e-7.
-__device__ __forceinline__ float tail_fast(float z, float* g) {
-  const float t = __fdividef(1.f, fmaf(z, 0.3275911f * 0.70710678f, 1.f));
-  const float p = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t,
-                            -0.284496736f), t, 0.254829592f) * t;
-  *g = __expf(-0.5f * z * z);
-  return 0.5f * p * *g;
-}
-__device__ __forceinline__ float cdf_fast(float x, float* g) {
-  const float q = tail_fast(fabsf(x), g);
-  return x < 0.f ? q : 1.f - q;
-}
-// 1 - 2 / (1 + exp 2x), and the Taylor polynomial near 0, where that cancels
-__device__ __forceinline__ float tanh_fast(float x) {
-  const float s = x * x;
-  const float small =
-      x * fmaf(s, fmaf(s, fmaf(s, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
-  const float big = 1.f - __fdividef(2.f, 1.f + __expf(2.f * fminf(x, 40.f)));
-  return s < 0.0625f ? small : big;
-}
-__device__ __forceinline__ float sigmoid_fast(float x) {
-  return __fdividef(1.f, 1.f + __expf(fminf(-x, 80.f)));
-}
-
-template <int ACT, bool FAST>
+// f(x) and f'(x) with CUDA's erff, expf and tanhf, for Float32 arrays.
+template <int ACT>
 __device__ __forceinline__ float act_f(float x) {
   if constexpr (ACT == STADE_ACT_RELU) return x > 0.f ? x : (x != x ? x : 0.f);
-  if constexpr (ACT == STADE_ACT_TANH) return FAST ? tanh_fast(x) : tanhf(x);
-  if constexpr (ACT == STADE_ACT_SILU) return FAST ? x * sigmoid_fast(x) : x / (1.f + expf(-x));
-  if constexpr (ACT == STADE_ACT_GELU) {
-    float g;
-    return FAST ? x * cdf_fast(x, &g) : 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
-  }
+  if constexpr (ACT == STADE_ACT_TANH) return tanhf(x);
+  if constexpr (ACT == STADE_ACT_SILU) return x / (1.f + expf(-x));
+  if constexpr (ACT == STADE_ACT_GELU) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
   return x;
 }
 // relu: max(x, 0)' = (1 + sign x) / 2, the partial of the generated sweeps
-template <int ACT, bool FAST>
+template <int ACT>
 __device__ __forceinline__ float act_df(float x) {
   if constexpr (ACT == STADE_ACT_RELU) return x > 0.f ? 1.f : x < 0.f ? 0.f : x == 0.f ? 0.5f : x;
   if constexpr (ACT == STADE_ACT_TANH) {
-    const float h = FAST ? tanh_fast(x) : tanhf(x);
+    const float h = tanhf(x);
     return 1.f - h * h;
   }
   if constexpr (ACT == STADE_ACT_SILU) {
-    const float p = FAST ? sigmoid_fast(x) : 1.f / (1.f + expf(-x));
+    const float p = 1.f / (1.f + expf(-x));
     return p * (1.f + x * (1.f - p));
   }
-  if constexpr (ACT == STADE_ACT_GELU) {
-    if (FAST) {
-      float g;
-      const float c = cdf_fast(x, &g);
-      return fmaf(x * 0.39894228040143268f, g, c);
-    }
+  if constexpr (ACT == STADE_ACT_GELU)
     return 0.5f * (1.f + erff(x * 0.70710678118654752f)) +
            x * expf(-0.5f * x * x) * 0.39894228040143268f;
-  }
   return 1.f;
+}
+
+// The same for 16-bit arrays: errors of a few 1e-7 of 1 + |x|, below a hundredth
+// of what rounding the result costs, at two special-function instructions an
+// element and two elements an instruction elsewhere. With erff and expf a gelu
+// step of 8192 x 8192 in bf16 was bound by its instructions (213 us; memory
+// alone 103 us).
+using P2 = Pair<float>;
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// q = 1 - Phi(|x|) and g = exp(-x^2 / 2): the rational approximation 7.1.26 of
+// Abramowitz and Stegun for erfc(|x| / sqrt 2) / 2, error at most 7.5e-8.
+__device__ __forceinline__ P2 tail2(P2 x, P2* g) {
+  constexpr float c = 0.3275911f * 0.70710678118654752f;
+  const P2 t(rcp(fmaf(fabsf(x.lo()), c, 1.f)), rcp(fmaf(fabsf(x.hi()), c, 1.f)));
+  const P2 s = mul2(mul2(x, x), both(-0.5f * kLog2e));
+  *g = P2(ex2(s.lo()), ex2(s.hi()));
+  P2 p = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
+  p = fma2(p, t, both(0.5f * 1.421413741f));
+  p = fma2(p, t, both(0.5f * -0.284496736f));
+  p = fma2(p, t, both(0.5f * 0.254829592f));
+  return mul2(mul2(p, t), *g);
+}
+// 1 / (1 + exp(-x))
+__device__ __forceinline__ P2 sigmoid2(P2 x) {
+  return P2(rcp(1.f + ex2(fminf(x.lo() * -kLog2e, 120.f))),
+            rcp(1.f + ex2(fminf(x.hi() * -kLog2e, 120.f))));
+}
+// 1 - 2 / (1 + exp 2x), and the Taylor polynomial near 0, where that cancels
+__device__ __forceinline__ P2 tanh2(P2 x) {
+  const P2 s = mul2(x, x);
+  P2 p = fma2(s, both(-17.f / 315.f), both(2.f / 15.f));
+  p = fma2(s, p, both(-1.f / 3.f));
+  const P2 small = mul2(x, fma2(s, p, both(1.f)));
+  const float a = fmaf(rcp(1.f + ex2(fminf(x.lo() * (2.f * kLog2e), 120.f))), -2.f, 1.f);
+  const float b = fmaf(rcp(1.f + ex2(fminf(x.hi() * (2.f * kLog2e), 120.f))), -2.f, 1.f);
+  // a NaN takes the polynomial, which passes it on
+  return P2(s.lo() >= 0.0625f ? a : small.lo(), s.hi() >= 0.0625f ? b : small.hi());
+}
+
+template <int ACT>
+__device__ __forceinline__ P2 act_f2(P2 x) {
+  if constexpr (ACT == STADE_ACT_TANH) return tanh2(x);
+  if constexpr (ACT == STADE_ACT_SILU) {
+    return mul2(x, sigmoid2(x));
+  }
+  if constexpr (ACT == STADE_ACT_GELU) {
+    // x Phi(x) = max(x, 0) - |x| (1 - Phi(|x|)); the product is 0 from 14 on, also
+    // for an infinity, and NaN for a NaN
+    P2 g;
+    const P2 q = tail2(x, &g);
+    return P2(fmaf(-fminf(fabsf(x.lo()), 14.f), q.lo(), fmaxf(x.lo(), 0.f)),
+              fmaf(-fminf(fabsf(x.hi()), 14.f), q.hi(), fmaxf(x.hi(), 0.f)));
+  }
+  return P2(act_f<ACT>(x.lo()), act_f<ACT>(x.hi()));
+}
+template <int ACT>
+__device__ __forceinline__ P2 act_df2(P2 x) {
+  if constexpr (ACT == STADE_ACT_TANH) {
+    const P2 h = tanh2(x);
+    return fma2(mul2(h, both(-1.f)), h, both(1.f));
+  }
+  if constexpr (ACT == STADE_ACT_SILU) {
+    const P2 p = sigmoid2(x);
+    return mul2(p, fma2(x, fma2(p, both(-1.f), both(1.f)), both(1.f)));
+  }
+  if constexpr (ACT == STADE_ACT_GELU) {
+    P2 g;
+    const P2 h = fma2(tail2(x, &g), both(-1.f), both(0.5f));    // |Phi(x) - 1/2|
+    const P2 c = add2(P2(copysignf(h.lo(), x.lo()), copysignf(h.hi(), x.hi())), both(0.5f));
+    return fma2(mul2(x, both(0.39894228040143268f)), g, c);
+  }
+  return P2(act_df<ACT>(x.lo()), act_df<ACT>(x.hi()));
+}
+template <int ACT, bool FAST> __device__ __forceinline__ P2 act_pair(P2 x) {
+  if constexpr (FAST) return act_f2<ACT>(x);
+  return P2(act_f<ACT>(x.lo()), act_f<ACT>(x.hi()));
+}
+template <int ACT, bool FAST> __device__ __forceinline__ P2 act_d_pair(P2 x) {
+  if constexpr (FAST) return act_df2<ACT>(x);
+  return P2(act_df<ACT>(x.lo()), act_df<ACT>(x.hi()));
 }
 
 // Adding 1.5 2^23 rounds a value of less than 2^22 to the nearest whole number,
 // ties to even, and leaves it in the low bits: the code's byte is the low one.
 constexpr float kMagic = 12582912.f;
-__device__ __forceinline__ uint32_t code_bits(float v, float inv) {
-  return __float_as_uint(fminf(fmaxf(v * inv, -127.f), 127.f) + kMagic);
+__device__ __forceinline__ P2 code_bits2(P2 v, float inv) {
+  const P2 r = mul2(v, both(inv));
+  return add2(P2(fminf(fmaxf(r.lo(), -127.f), 127.f), fminf(fmaxf(r.hi(), -127.f), 127.f)),
+              both(kMagic));
 }
-__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+__device__ __forceinline__ uint32_t pack4(P2 a, P2 b) {
+  return __byte_perm(__byte_perm(__float_as_uint(a.lo()), __float_as_uint(a.hi()), 0x0040),
+                     __byte_perm(__float_as_uint(b.lo()), __float_as_uint(b.hi()), 0x0040), 0x5410);
 }
-// Byte k of w, biased by 128 (w = codes ^ 0x80808080), times step.
-__device__ __forceinline__ float code_value(uint32_t w, int k, float step) {
-  const float f = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + k));   // 2^23 + byte
-  return (f - 8388736.f) * step;
+// Bytes k and k + 1 of w, biased by 128 (w = codes ^ 0x80808080), times step:
+// 2^23 + byte has the byte in its low bits; all of it exact (the difference
+// first: 2^23 step passes Float32's range where step is its largest).
+__device__ __forceinline__ P2 code_value2(uint32_t w, int k, P2 step) {
+  const P2 f(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + k)),
+             __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + k + 1)));
+  return mul2(add2(f, both(-8388736.f)), step);
 }
 
 // A thread takes V = 8 values of a row, four threads a group: 16 to 32 bytes
@@ -130,24 +189,36 @@ __device__ __forceinline__ float code_value(uint32_t w, int k, float step) {
 constexpr int kV = 8;
 
 template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[kV]) {
+struct alignas(16) Eight {
+  T v[kV];
+};
+// 8 values as the array holds them: one access of 16 bytes, or two of them.
+template <class T> __device__ __forceinline__ Eight<T> load8(const T* p) {
+  Eight<T> r;
   if constexpr (sizeof(T) == 2) {
-    const Vec<T, 8> r = *reinterpret_cast<const Vec<T, 8>*>(p);
-#pragma unroll
-    for (int k = 0; k < kV; ++k) v[k] = load_acc<T>(r.v[k]);
+    *reinterpret_cast<int4*>(&r) = *reinterpret_cast<const int4*>(p);
   } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float4 r = reinterpret_cast<const float4*>(p)[h];
-      v[4 * h] = r.x; v[4 * h + 1] = r.y; v[4 * h + 2] = r.z; v[4 * h + 3] = r.w;
-    }
+    reinterpret_cast<int4*>(&r)[0] = reinterpret_cast<const int4*>(p)[0];
+    reinterpret_cast<int4*>(&r)[1] = reinterpret_cast<const int4*>(p)[1];
   }
+  return r;
+}
+template <class T> __device__ __forceinline__ P2 pair_of(const Eight<T>& r, int k) {
+  return widen2(reinterpret_cast<const Vec<T, 2>*>(&r)[k]);
+}
+template <class T> __device__ __forceinline__ void store8(T* p, const P2 (&v)[4]) {
+  Eight<T> r;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) reinterpret_cast<Vec<T, 2>*>(&r)[k] = narrow2<T>(v[k]);
+  reinterpret_cast<int4*>(p)[0] = reinterpret_cast<const int4*>(&r)[0];
+  if constexpr (sizeof(T) == 4) reinterpret_cast<int4*>(p)[1] = reinterpret_cast<const int4*>(&r)[1];
 }
 // Largest magnitude of 8 values, NaN if one is.
-__device__ __forceinline__ float top8(const float* p, const float (&v)[kV]) {
+__device__ __forceinline__ float top8(const Eight<float>& r) {
   uint32_t m = 0;        // magnitudes are ordered as whole numbers, NaN above infinity
 #pragma unroll
-  for (int k = 0; k < kV; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
+  for (int k = 0; k < kV; ++k)
+    m = max(m, reinterpret_cast<const uint32_t*>(&r)[k] & 0x7fffffffu);
   return __uint_as_float(m);
 }
 template <class T2>
@@ -155,13 +226,11 @@ __device__ __forceinline__ T2 top2(const T2* r) {
   return __hmax2_nan(__hmax2_nan(__habs2(r[0]), __habs2(r[1])),
                      __hmax2_nan(__habs2(r[2]), __habs2(r[3])));
 }
-__device__ __forceinline__ float top8(const __nv_bfloat16* p, const float (&)[kV]) {
-  const int4 r = *reinterpret_cast<const int4*>(p);
+__device__ __forceinline__ float top8(const Eight<__nv_bfloat16>& r) {
   const __nv_bfloat162 m = top2(reinterpret_cast<const __nv_bfloat162*>(&r));
   return __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
 }
-__device__ __forceinline__ float top8(const __half* p, const float (&)[kV]) {
-  const int4 r = *reinterpret_cast<const int4*>(p);
+__device__ __forceinline__ float top8(const Eight<__half>& r) {
   const __half2 m = top2(reinterpret_cast<const __half2*>(&r));
   return __half2float(__hmax_nan(__low2half(m), __high2half(m)));
 }
@@ -169,64 +238,51 @@ __device__ __forceinline__ float top8(const __half* p, const float (&)[kV]) {
 __device__ __forceinline__ float larger(float a, float b) {
   return __uint_as_float(max(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu));
 }
-template <class T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[kV]) {
-  if constexpr (sizeof(T) == 2) {
-    Vec<T, 8> r;
-#pragma unroll
-    for (int k = 0; k < kV; ++k) r.v[k] = round_to<T>(v[k]);
-    *reinterpret_cast<Vec<T, 8>*>(p) = r;
-  } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      reinterpret_cast<float4*>(p)[h] =
-          make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
-  }
-}
 
-// Rows of n8 eights; thread i of `count` (a multiple of 4 a row: a row's last
-// group may have threads past its end).
+// Rows of n8 eights, thread i of `count`, 4 n_g a row: a row's last group may
+// have threads past its end.
 template <class T, int ACT>
 __global__ void __launch_bounds__(kThreads)
 push8_kernel(const T* __restrict__ x, T* __restrict__ y, int8_t* __restrict__ q,
              uint8_t* __restrict__ e, uint32_t n8, uint32_t n_g, int64_t count) {
-  for (int64_t i0 = (int64_t)blockIdx.x * kThreads; i0 < count; i0 += (int64_t)gridDim.x * kThreads) {
-    const int64_t i = i0 + threadIdx.x;
-    const bool live = i < count;
-    // the usual case, rows of whole groups, needs no division
-    int64_t at = i, group = i >> 2;
-    bool in = live;
-    if (n8 != 4 * n_g) {
-      const int64_t s = i / (4 * n_g);
-      const uint32_t c = (uint32_t)(i - s * (4 * n_g));
-      in = live && c < n8;
-      at = s * n8 + c;
-    }
-    float v[kV];
-    float top = 0.f;
-    if (in) {
-      load8<T>(x + at * kV, v);
-      top = top8(x + at * kV, v);
-    }
-    top = larger(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = larger(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int code = scale_code(top);
-    if (in) {
-      const float inv = pow2f(127 - min(code, 253));
-      uint32_t c[kV];
-#pragma unroll
-      for (int k = 0; k < kV; ++k) c[k] = code_bits(v[k], inv);
-      uint2 w = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
-      if (code == 255) w = make_uint2(0, 0);
-      *reinterpret_cast<uint2*>(q + at * kV) = w;
-      if constexpr (ACT != STADE_ACT_NONE) {
-#pragma unroll
-        for (int k = 0; k < kV; ++k) v[k] = act_f<ACT, sizeof(T) == 2>(v[k]);
-        store8<T>(y + at * kV, v);
-      }
-    }
-    if (live && (threadIdx.x & 3) == 0) e[group] = (uint8_t)code;
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const bool live = i < count;
+  // the usual case, rows of whole groups, needs no division
+  int64_t at = i;
+  bool in = live;
+  if (n8 != 4 * n_g) {
+    const int64_t s = i / (4 * n_g);
+    const uint32_t c = (uint32_t)(i - s * (4 * n_g));
+    in = live && c < n8;
+    at = s * n8 + c;
   }
+  Eight<T> v;
+  float top = 0.f;
+  if (in) {
+    v = load8<T>(x + at * kV);
+    top = top8(v);
+  }
+  top = larger(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = larger(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const int code = scale_code(top);
+  if (in) {
+    const float inv = pow2f(127 - min(code, 253));
+    P2 p[4], c[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      p[k] = pair_of<T>(v, k);
+      c[k] = code_bits2(p[k], inv);
+    }
+    uint2 w = make_uint2(pack4(c[0], c[1]), pack4(c[2], c[3]));
+    if (code == 255) w = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(q + at * kV) = w;
+    if constexpr (ACT != STADE_ACT_NONE) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) p[k] = act_pair<ACT, sizeof(T) == 2>(p[k]);
+      store8<T>(y + at * kV, p);
+    }
+  }
+  if (live && (threadIdx.x & 3) == 0) e[i >> 2] = (uint8_t)code;
 }
 
 template <class T, int ACT>
@@ -234,38 +290,40 @@ __global__ void __launch_bounds__(kThreads)
 pop8_kernel(T* __restrict__ xb, T* __restrict__ yb, const int8_t* __restrict__ q,
             const uint8_t* __restrict__ e, uint32_t n8, uint32_t n_g, int64_t count, bool add,
             bool zero) {
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count;
-       i += (int64_t)gridDim.x * kThreads) {
-    int64_t group = i >> 2;
-    if (n8 != 4 * n_g) {
-      const int64_t s = i / n8;
-      group = s * n_g + (uint32_t)(i - s * n8) / 4;
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i >= count) return;
+  int64_t group = i >> 2;
+  if (n8 != 4 * n_g) {
+    const int64_t s = i / n8;
+    group = s * n_g + (uint32_t)(i - s * n8) / 4;
+  }
+  uint2 w = *reinterpret_cast<const uint2*>(q + i * kV);
+  Eight<T> g;
+  if constexpr (ACT != STADE_ACT_NONE) g = load8<T>(yb + i * kV);
+  const int code = e[group];
+  w.x ^= 0x80808080u;
+  w.y ^= 0x80808080u;
+  const float step = code == 255 ? __int_as_float(0x7fffffff) : pow2f(code - 127);
+  const P2 step2 = both(step);
+  P2 v[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    v[k] = code_value2(k < 2 ? w.x : w.y, 2 * (k % 2), step2);
+  if constexpr (ACT == STADE_ACT_NONE) {
+    store8<T>(xb + i * kV, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      v[k] = mul2(pair_of<T>(g, k), act_d_pair<ACT, sizeof(T) == 2>(v[k]));
+    if (add) {
+      const Eight<T> old = load8<T>(xb + i * kV);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = add2(v[k], pair_of<T>(old, k));
     }
-    const int code = e[group];
-    uint2 w = *reinterpret_cast<const uint2*>(q + i * kV);
-    w.x ^= 0x80808080u;
-    w.y ^= 0x80808080u;
-    const float step = code == 255 ? __int_as_float(0x7fffffff) : pow2f(code - 127);
-    float v[kV], g[kV];
-#pragma unroll
-    for (int k = 0; k < kV; ++k) v[k] = code_value(k < 4 ? w.x : w.y, k % 4, step);
-    if constexpr (ACT == STADE_ACT_NONE) {
-      store8<T>(xb + i * kV, v);
-    } else {
-      load8<T>(yb + i * kV, g);
-#pragma unroll
-      for (int k = 0; k < kV; ++k) g[k] *= act_df<ACT, sizeof(T) == 2>(v[k]);
-      if (add) {
-        load8<T>(xb + i * kV, v);
-#pragma unroll
-        for (int k = 0; k < kV; ++k) g[k] += v[k];
-      }
-      store8<T>(xb + i * kV, g);
-      if (zero) {
-#pragma unroll
-        for (int k = 0; k < kV; ++k) g[k] = 0.f;
-        store8<T>(yb + i * kV, g);
-      }
+    store8<T>(xb + i * kV, v);
+    if (zero) {
+      P2 z[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
+      store8<T>(yb + i * kV, z);
     }
   }
 }
@@ -294,11 +352,13 @@ push_kernel(const T* __restrict__ x, T* __restrict__ y, int8_t* __restrict__ q,
       const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(v[j]) & 0x7fffffffu);
       const int code = scale_code(__uint_as_float(top));
       if (lane == j) mine = code;
-      const uint32_t c = code == 255 ? 0u : code_bits(v[j], pow2f(127 - min(code, 253)));
+      const uint32_t c =
+          code == 255 ? 0u
+                      : __float_as_uint(code_bits2(both(v[j]), pow2f(127 - min(code, 253))).lo());
       if (j * kGroup < left) {
         q[at + j * kGroup] = (int8_t)(c & 255u);
         if constexpr (ACT != STADE_ACT_NONE)
-          y[at + j * kGroup] = round_to<T>(act_f<ACT, sizeof(T) == 2>(v[j]));
+          y[at + j * kGroup] = round_to<T>(act_pair<ACT, sizeof(T) == 2>(both(v[j])).lo());
       }
     }
     if (lane < kGroups && g0 + lane < n_g) e[s * n_g + g0 + lane] = (uint8_t)mine;
@@ -337,7 +397,7 @@ pop_kernel(T* __restrict__ xb, T* __restrict__ yb, const int8_t* __restrict__ q,
         if constexpr (ACT == STADE_ACT_NONE) {
           xb[at + j * kGroup] = round_to<T>(v);
         } else {
-          float r = g[j] * act_df<ACT, sizeof(T) == 2>(v);
+          float r = g[j] * act_d_pair<ACT, sizeof(T) == 2>(both(v)).lo();
           if (add) r += old[j];
           xb[at + j * kGroup] = round_to<T>(r);
           if (zero) yb[at + j * kGroup] = round_to<T>(0.f);
@@ -371,8 +431,7 @@ unsigned blocks_for(int64_t warps) {
 }
 
 unsigned blocks8(int64_t count) {
-  const int64_t b = (count + kThreads - 1) / kThreads;
-  return (unsigned)std::min<int64_t>(b, 148 * 8 * 16);
+  return (unsigned)((count + kThreads - 1) / kThreads);
 }
 
 stade_status check_args(const char* who, int dtype, int act, int64_t n_s, int64_t n_d) {
@@ -397,7 +456,7 @@ stade_status push(const char* who, int dtype, int act, const void* x, void* y, i
   const int64_t n_g = (n_d + kGroup - 1) / kGroup;
   // 8 values of every array in whole accesses
   const bool eights = n_d % kV == 0 && row_align(16, {x, y}) == 16 && row_align(8, {q}) >= 8 &&
-                      n_d < (int64_t(1) << 31);
+                      n_d < (int64_t(1) << 31) && n_s * n_g < (int64_t(1) << 36);
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     return with_act(act, [&](auto a) {
@@ -427,7 +486,7 @@ stade_status pop(const char* who, int dtype, int act, void* xb, void* yb, const 
   PhaseScope ph(who, s);
   const int64_t n_g = (n_d + kGroup - 1) / kGroup;
   const bool eights = n_d % kV == 0 && row_align(16, {xb, yb}) == 16 && row_align(8, {q}) >= 8 &&
-                      n_d < (int64_t(1) << 31);
+                      n_d < (int64_t(1) << 31) && n_s * n_g < (int64_t(1) << 36);
   return with_type(dtype, [&](auto t) {
     using T = decltype(t);
     return with_act(act, [&](auto a) {
