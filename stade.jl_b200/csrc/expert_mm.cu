@@ -26,22 +26,45 @@ using Tile = ExpertTile;
 constexpr int kTile = 64;       // rows and columns of a CUDA-core tile
 constexpr int kStep = 16;
 
+// Inclusive scan of one value per thread over a block of 1024; `sm`: 32 values.
+template <class F>
+__device__ __forceinline__ long long block_scan(long long v, long long* sm, F op) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v = op(u, v);
+  }
+  if (lane == 31) sm[warp] = v;
+  __syncthreads();
+  long long t = sm[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, t, o);
+    if (lane >= o) t = op(u, t);
+  }
+  const long long before = __shfl_sync(0xffffffffu, t, warp > 0 ? warp - 1 : 0);
+  if (warp > 0) v = op(before, v);
+  __syncthreads();
+  return v;
+}
+
 // One block. bounds[0 .. n_e]: the clamped, rising bounds; tiles of at most
 // `tile` rows of every group, then of the rows in no group; count[0]: how many.
 __global__ void __launch_bounds__(1024)
 plan_kernel(const int64_t* __restrict__ off, int64_t n_s, int64_t n_e, int tile,
             int64_t* __restrict__ bounds, Tile* __restrict__ tiles, int* __restrict__ count) {
-  __shared__ long long scan[1024];
-  __shared__ long long carry_bound;
-  __shared__ int carry_tiles;
+  __shared__ long long sm[32];
+  __shared__ long long edge[1024];
+  __shared__ long long last;
   const int t = threadIdx.x;
-  if (t == 0) {
-    carry_bound = 0;
-    carry_tiles = 0;
-  }
-  __syncthreads();
-  // rising bounds: a running maximum of the clamped entries
-  for (int64_t e0 = 0; e0 <= n_e; e0 += 1024) {
+  before_next();
+  auto larger = [](long long a, long long b) { return a > b ? a : b; };
+  auto sum = [](long long a, long long b) { return a + b; };
+  long long low = 0, low_end = 0;     // the bound before this round's first, the first of all
+  int done = 0;                       // tiles so far
+  // round r: entries 1023 r .. 1023 r + 1023, the last of them the next round's first
+  for (int64_t e0 = 0; e0 <= n_e; e0 += 1023) {
     const int64_t e = e0 + t;
     long long v = 0;
     if (e <= n_e) {
@@ -49,44 +72,35 @@ plan_kernel(const int64_t* __restrict__ off, int64_t n_s, int64_t n_e, int tile,
       if (raw < 0 || raw > n_s || (e > 0 && raw < off[e - 1])) g_expert_error = 1;
       v = min(max(raw, 0ll), (long long)n_s);
     }
-    scan[t] = v;
+    // rising bounds: a running maximum of the clamped entries
+    v = larger(block_scan(v, sm, larger), low);
+    edge[t] = v;
+    if (e <= n_e) bounds[e] = v;
+    if (t == 1023) last = v;
     __syncthreads();
-    for (int o = 1; o < 1024; o <<= 1) {
-      const long long u = t >= o ? scan[t - o] : 0;
-      __syncthreads();
-      scan[t] = max(scan[t], u);
-      __syncthreads();
-    }
-    if (e <= n_e) bounds[e] = max(scan[t], carry_bound);
+    low = last;
+    if (e0 == 0) low_end = edge[0];
+    const bool group = t < 1023 && e < n_e;
+    const long long a = v, b = group ? edge[t + 1] : v;
+    const long long mine = group ? (b - a + tile - 1) / tile : 0;
+    const long long upto = block_scan(mine, sm, sum);
+    int at = done + (int)(upto - mine);
+    for (long long i = 0; i < mine; ++i, ++at)
+      tiles[at] = Tile{(int)e, (int)(a + i * tile), (int)min((long long)tile, b - a - i * tile), 0};
+    if (t == 1023) last = upto;
     __syncthreads();
-    if (t == 1023) carry_bound = max(scan[t], carry_bound);
-    __syncthreads();
-  }
-  // group n_e: the rows before the first bound, group n_e + 1: those after the last
-  for (int64_t e0 = 0; e0 < n_e + 2; e0 += 1024) {
-    const int64_t e = e0 + t;
-    int64_t a = 0, b = 0;
-    if (e < n_e) a = bounds[e], b = bounds[e + 1];
-    else if (e == n_e) b = bounds[0];
-    else if (e == n_e + 1) a = bounds[n_e], b = n_s;
-    const int mine = (int)((b - a + tile - 1) / tile);
-    scan[t] = mine;
-    __syncthreads();
-    for (int o = 1; o < 1024; o <<= 1) {
-      const long long u = t >= o ? scan[t - o] : 0;
-      __syncthreads();
-      scan[t] += u;
-      __syncthreads();
-    }
-    int at = carry_tiles + (int)scan[t] - mine;
-    for (int i = 0; i < mine; ++i, ++at)
-      tiles[at] = Tile{e < n_e ? (int)e : -1, (int)(a + (int64_t)i * tile),
-                       (int)min((int64_t)tile, b - a - (int64_t)i * tile), 0};
-    __syncthreads();
-    if (t == 1023) carry_tiles += (int)scan[t];
+    done += (int)last;
     __syncthreads();
   }
-  if (t == 0) count[0] = carry_tiles;
+  // rows before the first bound and after the last
+  const long long top = low;
+  const long long head = (low_end + tile - 1) / tile, foot = (n_s - top + tile - 1) / tile;
+  for (long long i = t; i < head + foot; i += 1024) {
+    const long long a = i < head ? i * tile : top + (i - head) * tile;
+    const long long z = i < head ? low_end : n_s;
+    tiles[done + i] = Tile{-1, (int)a, (int)min((long long)tile, z - a), 0};
+  }
+  if (t == 0) count[0] = done + (int)(head + foot);
 }
 
 // C[m][n] (+)= sum_k A(m, k) B(k, n) of one 64 x 64 tile, A(m, k) =

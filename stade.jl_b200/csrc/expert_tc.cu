@@ -113,12 +113,20 @@ struct GroupSrc {
   int n_e;
   __device__ __forceinline__ int total(const Geom& g) const { return n_e * g.m_tiles * g.n_tiles; }
   __device__ __forceinline__ Unit get(int t, const Geom& g) const {
-    const int per = g.m_tiles * g.n_tiles;
+    // whole tiles of all groups first, the narrow last ones after them: the
+    // pairs that a last round leaves with one more unit then have a small one
+    const int whole = g.N / kTileN, per = g.m_tiles * whole, first = n_e * per;
     Unit u;
-    u.expert = t / per;
-    const int r = t % per;
-    u.m0 = (r % g.m_tiles) * 2 * kHalfM;
-    u.n0 = (r / g.m_tiles) * kTileN;
+    if (t < first) {
+      u.expert = t / per;
+      const int r = t - u.expert * per, n = r / g.m_tiles;
+      u.m0 = (r - n * g.m_tiles) * 2 * kHalfM;
+      u.n0 = n * kTileN;
+    } else {
+      u.expert = (t - first) / g.m_tiles;
+      u.m0 = (t - first - u.expert * g.m_tiles) * 2 * kHalfM;
+      u.n0 = whole * kTileN;
+    }
     const int64_t a = bounds[u.expert], b = bounds[u.expert + 1];
     u.row = (int)a;
     u.rows = (int)(b - a);
@@ -281,6 +289,10 @@ expert_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
 
+  if (threadIdx.x == 32) {
+    tc5::prefetch_map(&amap);
+    for (int i = 0; i < 4; ++i) tc5::prefetch_map(&bmaps.m[i]);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(full0 + 8 * s, 1);
@@ -300,6 +312,7 @@ expert_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
   tc5::cluster_sync();
   tc5::fence_after();
   const uint32_t tmem = *tmem_slot;
+  after_previous();        // what is above overlaps the kernels that prepare the operands
   const int total = src.total(g);
 
   if (warp == 0) {
@@ -544,10 +557,14 @@ template <bool WGRAD, class Src, class Out>
 stade_status launch(const ExpertOperand& A, const ExpertOperand& B, const Geom& g, const Src& src,
                     Out* out, int n_e, int64_t units, cudaStream_t s) {
   CUtensorMap am;
-  BMaps bm = {};
+  BMaps bm;
   stade_status st = operand_map(&am, A, g.bf16, 64, g.a_mn ? 64 : 128);
-  for (int i = 0; i < (g.b_mn ? 1 : 4) && st == STADE_OK; ++i)
-    st = operand_map(&bm.m[i], B, g.bf16, 64, g.b_mn ? 64 : 16 << i);
+  if (st == STADE_OK) st = operand_map(&bm.m[0], B, g.bf16, 64, g.b_mn ? 64 : 16);
+  // taller boxes only where a tile can have the rows for them
+  for (int i = 1; i < 4 && st == STADE_OK; ++i) {
+    if (g.b_mn || B.d1 <= 16 << i) bm.m[i] = bm.m[i - 1];
+    else st = operand_map(&bm.m[i], B, g.bf16, 64, 16 << i);
+  }
   if (st != STADE_OK) return st;
   auto kern = expert_tc_kernel<WGRAD, Src, Out>;
   STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
@@ -557,49 +574,64 @@ stade_status launch(const ExpertOperand& A, const ExpertOperand& B, const Geom& 
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   STADE_CUDA(cudaLaunchKernelEx(&cfg, kern, am, bm, g, src, out, n_e));
   count_launch();
   return STADE_OK;
 }
 
 // ---- operand planes ------------------------------------------------------------------
-template <class T, int NP>
+// Eight columns a thread; VEC: source rows are multiples of 16 bytes.
+template <class T, int NP, bool VEC>
 __global__ void __launch_bounds__(256)
 pack_kernel(const T* __restrict__ src, uint16_t* __restrict__ dst, int64_t rows, int64_t cols,
             int64_t pitch) {
+  before_next();
+  after_previous();
   const int64_t per = pitch / 8, n = rows * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per, c = (i % per) * 8;
-    uint16_t o[NP][8];
+    const int64_t r = VEC ? 0 : i / per, c = VEC ? 0 : (i - r * per) * 8;
+    alignas(16) T in[8];
+    if constexpr (VEC) {       // rows follow each other without a gap
+      constexpr int kPieces = 8 * (int)sizeof(T) / 16;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (NP == 1) {
-        o[0][j] = c + j < cols ? *reinterpret_cast<const uint16_t*>(src + r * cols + c + j) : 0;
-      } else {
-        float v = c + j < cols ? (float)src[r * cols + c + j] : 0.f;
+      for (int h = 0; h < kPieces; ++h)
+        reinterpret_cast<int4*>(in)[h] = reinterpret_cast<const int4*>(src + i * 8)[h];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) in[j] = c + j < cols ? src[r * cols + c + j] : T(0.f);
+    }
+    const int64_t at = VEC ? i * 8 : r * pitch + c;
+    if constexpr (NP == 1) {
+      *reinterpret_cast<int4*>(dst + at) = *reinterpret_cast<const int4*>(in);
+    } else {
+      alignas(16) uint16_t o[NP][8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float v = in[j];
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
           __nv_bfloat16 h = __float2bfloat16_rn(v);
           // a finite value just below 2^128 rounds to infinity: cut it instead
-          if (__hisinf(h) && isfinite(v))
+          if (p == 0 && __hisinf(h) && isfinite(v))
             h = __ushort_as_bfloat16((unsigned short)(__float_as_uint(v) >> 16));
           o[p][j] = __bfloat16_as_ushort(h);
           const float f = __bfloat162float(h);
-          v = isfinite(f) ? v - f : 0.f;   // exact
+          v = p > 0 || isfinite(f) ? v - f : 0.f;   // exact
         }
       }
-    }
 #pragma unroll
-    for (int p = 0; p < NP; ++p)
-      *reinterpret_cast<int4*>(dst + (p * rows + r) * pitch + c) =
-          *reinterpret_cast<const int4*>(o[p]);
+      for (int p = 0; p < NP; ++p)
+        *reinterpret_cast<int4*>(dst + p * rows * pitch + at) = *reinterpret_cast<const int4*>(o[p]);
+    }
   }
 }
 
@@ -611,14 +643,15 @@ stade_status expert_pack(int dtype, const void* src, void* dst, int64_t rows, in
                          int64_t pitch, cudaStream_t s) {
   const int64_t n = rows * (pitch / 8);
   if (n == 0) return STADE_OK;
-  const unsigned blocks = (unsigned)std::min<int64_t>((n + 255) / 256, 148 * 16);
+  const unsigned blocks = (unsigned)std::min<int64_t>((n + 255) / 256, 148 * 32);
+  uint16_t* d = (uint16_t*)dst;
+  const bool vec = cols == pitch && row_align(16, {src}) == 16;
   if (dtype == STADE_F32)
-    pack_kernel<float, 3><<<blocks, 256, 0, s>>>((const float*)src, (uint16_t*)dst, rows, cols, pitch);
-  else
-    pack_kernel<__half, 1><<<blocks, 256, 0, s>>>((const __half*)src, (uint16_t*)dst, rows, cols,
-                                                  pitch);
-  STADE_CHECK_LAUNCH();
-  return STADE_OK;
+    return launch_next(vec ? pack_kernel<float, 3, true> : pack_kernel<float, 3, false>, blocks, 256,
+                       0, s, (const float*)src, d, rows, cols, pitch);
+  // the two 16-bit types are moved, not computed with
+  return launch_next(vec ? pack_kernel<__half, 1, true> : pack_kernel<__half, 1, false>, blocks, 256,
+                     0, s, (const __half*)src, d, rows, cols, pitch);
 }
 
 stade_status expert_tc_rows(int dtype, const ExpertOperand& in, const ExpertOperand& w, void* out,

@@ -20,6 +20,8 @@ struct ExpertOperand {
   int64_t d0, d1, d2, pitch;
 };
 
+// The calls below, and expert_pack, are launched so that they overlap the end of
+// the kernel before them; that has to be a kernel of the same call.
 // out[s, :] (+)= in[s, :] W[e] (n_i -> n_o) or in[s, :] W[e]^T (trans)
 stade_status expert_tc_rows(int dtype, const ExpertOperand& in, const ExpertOperand& w, void* out,
                             const ExpertTile* tiles, const int* count, int64_t max_tiles,
