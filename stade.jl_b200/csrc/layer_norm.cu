@@ -23,21 +23,17 @@ namespace {
 
 // ---- rows held in registers -----------------------------------------------------
 // Both sweeps are bound by memory: x in and y out, or x and yb in and xb out,
-// each once. A row lives in the registers of a group of G threads, NV vectors
-// of VEC values each (slot j of a row belongs to thread j % G), so nothing is
-// read twice; rows too long for that go through the kernels further down,
-// which read a row again from the caches.
-// VEC is 16 bytes where the rows allow it, 4 bytes (16-bit types), else one
-// value; short rows take narrower vectors so that a warp's lanes all have
-// work.
-//
-// Long rows of arrays that start on 16-byte boundaries take the ring kernels: one block
-// holds a row, the rows to come are copied by cp.async.bulk into a ring in
-// shared memory, several rows ahead of the arithmetic, and w, b and the sums
-// over rows stay in registers for all of a block's rows.
+// each once. A row lives in registers, so nothing is read twice:
+//  - rows of less than 1,536 bytes: a warp each, several rows in flight, w, b
+//    and the sums over rows in the lanes' registers for all of a warp's rows;
+//  - longer rows of arrays that start on 16-byte boundaries: the ring kernels,
+//    a block each, the rows to come copied by cp.async.bulk into a ring in
+//    shared memory, several rows ahead of the arithmetic;
+//  - other rows: a group of G threads each, NV values a thread, read directly;
+//  - rows too long for registers: read again from the caches.
 
-// Sums of two values over the group, the same in every thread. `red`: 2 x 2 x
-// 32 values, used alternately (`turn`), so that one barrier per sum is enough.
+// Sums of two values over the block, the same in every thread. `red`: 2 x 2 x 32
+// values, used alternately (`turn`), so that one barrier per sum is enough.
 template <class A>
 __device__ __forceinline__ void block_sum2(A& a, A& b, A (*red)[2][32], int turn, int warps) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -51,75 +47,45 @@ __device__ __forceinline__ void block_sum2(A& a, A& b, A (*red)[2][32], int turn
   a = warp_sum(lane < warps ? red[turn][0][lane] : A(0));
   b = warp_sum(lane < warps ? red[turn][1][lane] : A(0));
 }
-template <int G, class A>
-__device__ __forceinline__ void group_sum2(A& a, A& b, A (*red)[2][32], int turn) {
-  if constexpr (G > 32) {
-    block_sum2(a, b, red, turn, G / 32);
-  } else {
-    a = warp_sum(a);
-    b = warp_sum(b);
-  }
-}
-
-template <int G> constexpr int rows_per_block() { return G == 32 ? 4 : 1; }
-
-template <class T, int VEC, int G, int NV>
-__global__ void __launch_bounds__(G * rows_per_block<G>())
+template <class T, int G, int NV>
+__global__ void __launch_bounds__(G)
 ln_fwd_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
               const acc_t<T>* __restrict__ b, T* __restrict__ y, acc_t<T>* __restrict__ m_stack,
-              acc_t<T>* __restrict__ r_stack, double eps, int64_t n_s, int n_d) {
+              acc_t<T>* __restrict__ r_stack, double eps, int n_d) {
   using A = acc_t<T>;
   __shared__ A red[2][2][32];
-  const int t = threadIdx.x % G;
-  const int64_t s = (int64_t)blockIdx.x * rows_per_block<G>() + threadIdx.x / G;
-  if (s >= n_s) return;                       // whole warps, and then G == 32
-  const int slots = n_d / VEC;
+  const int t = threadIdx.x;
+  const int64_t s = blockIdx.x;
   const T* xr = x + s * n_d;
-  Vec<T, VEC> raw[NV];
+  A c[NV], sum = 0, zero = 0;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (i * G + t < slots) raw[i] = reinterpret_cast<const Vec<T, VEC>*>(xr)[i * G + t];
-  A sum = 0, zero = 0;
+  for (int i = 0; i < NV; ++i) c[i] = i * G + t < n_d ? load_acc<T>(xr[i * G + t]) : A(0);
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (i * G + t < slots)
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) sum += load_acc<T>(raw[i].v[k]);
-  group_sum2<G>(sum, zero, red, 0);
+  for (int i = 0; i < NV; ++i) sum += c[i];
+  block_sum2(sum, zero, red, 0, G / 32);
   const A mean = sum / (A)n_d;
   A sq = 0;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (i * G + t < slots)
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const A c = load_acc<T>(raw[i].v[k]) - mean;
-        sq += c * c;
-      }
-  group_sum2<G>(sq, zero, red, 1);
+  for (int i = 0; i < NV; ++i) {
+    c[i] -= mean;
+    if (i * G + t < n_d) sq += c[i] * c[i];
+  }
+  block_sum2(sq, zero, red, 1, G / 32);
   const A rstd = A(1) / sqrt(sq / (A)n_d + (A)eps);
   if (t == 0) {
     m_stack[s] = mean;
     r_stack[s] = rstd;
   }
-  T* yr = y + s * n_d;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (i * G + t < slots) {
-      const int d = (i * G + t) * VEC;
-      A o[VEC];
-#pragma unroll
-      for (int k = 0; k < VEC; ++k)
-        o[k] = (load_acc<T>(raw[i].v[k]) - mean) * rstd * (w ? __ldg(w + d + k) : A(1)) +
-               (b ? __ldg(b + d + k) : A(0));
-      store_vec<T, VEC>(yr + d, o);
-    }
+  for (int i = 0; i < NV; ++i) {
+    const int d = i * G + t;
+    if (d < n_d) y[s * n_d + d] = round_to<T>(c[i] * rstd * (w ? w[d] : A(1)) + (b ? b[d] : A(0)));
+  }
 }
 
-// The reverse sweep. Blocks walk the rows at a stride of the grid; a thread
-// keeps its columns of w and of the two sums over rows in registers, and the
-// next row's loads are issued before the current row's sums. Per block one
-// partial of each sum, added up in block order by ln_finish_kernel.
+// The reverse sweeps: blocks walk the rows at a stride of the grid, a thread
+// keeps its columns of w and of the two sums over rows in registers. Per block
+// one partial of each sum, added up in block order by ln_finish_kernel.
 struct BwdArgs {
   const void *x, *w, *m, *r;
   void *xb, *yb, *part;
@@ -128,118 +94,78 @@ struct BwdArgs {
   bool add, zero, sums;
 };
 
-template <class T, int VEC, int G, int NV>
-__global__ void __launch_bounds__(G * rows_per_block<G>())
+template <class T, int G, int NV>
+__global__ void __launch_bounds__(G)
 ln_bwd_kernel(BwdArgs p) {
   using A = acc_t<T>;
-  constexpr int R = rows_per_block<G>();
-  using V = Vec<T, VEC>;
   __shared__ A red[2][2][32];
-  const int t = threadIdx.x % G, slots = p.n_d / VEC;
-  const V* x = (const V*)p.x;
-  V* yb = (V*)p.yb;
-  const A* m = (const A*)p.m;
-  const A* r = (const A*)p.r;
-  A w[NV][VEC], sw[NV][VEC], sb[NV][VEC];
+  const int t = threadIdx.x;
+  const T* x = (const T*)p.x;
+  T* yb = (T*)p.yb;
+  T* xb = (T*)p.xb;
+  A w[NV], sw[NV], sb[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      w[i][k] = p.w && i * G + t < slots ? ((const A*)p.w)[(i * G + t) * VEC + k] : A(1);
-      sw[i][k] = sb[i][k] = A(0);
-    }
-  const int64_t step = (int64_t)gridDim.x * R;
-  int64_t s = (int64_t)blockIdx.x * R + threadIdx.x / G;
-  V nx[NV], ny[NV];
+  for (int i = 0; i < NV; ++i) {
+    w[i] = p.w && i * G + t < p.n_d ? ((const A*)p.w)[i * G + t] : A(1);
+    sw[i] = sb[i] = A(0);
+  }
+  T nx[NV], ny[NV];       // the next row, loaded a row ahead
   A nm = 0, nr = 0;
   auto fetch = [&](int64_t q) {
     if (q >= p.n_s) return;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (i * G + t < slots) {
-        nx[i] = x[q * slots + i * G + t];
-        ny[i] = yb[q * slots + i * G + t];
+      if (i * G + t < p.n_d) {
+        nx[i] = x[q * p.n_d + i * G + t];
+        ny[i] = yb[q * p.n_d + i * G + t];
       }
-    nm = m[q];
-    nr = r[q];
+    nm = ((const A*)p.m)[q];
+    nr = ((const A*)p.r)[q];
   };
-  fetch(s);
+  fetch(blockIdx.x);
   int turn = 0;
-  for (; s < p.n_s; s += step) {      // the same count for all threads of a group
-    V cx[NV], cy[NV];
-    const A mean = nm, rstd = nr;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) cx[i] = nx[i], cy[i] = ny[i];
-    fetch(s + step);
-    A sg = 0, sgh = 0;
+  for (int64_t s = blockIdx.x; s < p.n_s; s += gridDim.x) {
+    A h[NV], v[NV], sg = 0, sgh = 0;
+    const A rstd = nr;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (i * G + t < slots)
+      if (i * G + t < p.n_d) {
+        h[i] = (load_acc<T>(nx[i]) - nm) * rstd;
+        v[i] = load_acc<T>(ny[i]);
+      }
+    fetch(s + gridDim.x);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const A h = (load_acc<T>(cx[i].v[k]) - mean) * rstd, v = load_acc<T>(cy[i].v[k]);
-          const A g = v * w[i][k];
-          sg += g;
-          sgh += g * h;
-          sw[i][k] += v * h;
-          sb[i][k] += v;
+    for (int i = 0; i < NV; ++i)
+      if (i * G + t < p.n_d) {
+        const A g = v[i] * w[i];
+        sg += g;
+        sgh += g * h[i];
+        sw[i] += v[i] * h[i];
+        sb[i] += v[i];
+      }
+    block_sum2(sg, sgh, red, turn, G / 32);
+    turn ^= 1;
+    const A mg = sg / (A)p.n_d, mgh = sgh / (A)p.n_d;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int64_t at = s * p.n_d + i * G + t;
+      if (i * G + t < p.n_d) {
+        if (xb) {
+          const A o = rstd * (v[i] * w[i] - mg - h[i] * mgh);
+          xb[at] = round_to<T>(p.add ? load_acc<T>(xb[at]) + o : o);
         }
-    if (p.xb) {
-      group_sum2<G>(sg, sgh, red, turn);
-      turn ^= 1;
-      const A mg = sg / (A)p.n_d, mgh = sgh / (A)p.n_d;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (i * G + t < slots) {
-          T* o = (T*)p.xb + (s * slots + i * G + t) * VEC;
-          A out[VEC], old[VEC];
-          if (p.add) load_vec<T, VEC>(o, old);
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) {
-            const A h = (load_acc<T>(cx[i].v[k]) - mean) * rstd;
-            const A g = load_acc<T>(cy[i].v[k]) * w[i][k];
-            out[k] = rstd * (g - mg - h * mgh);
-            if (p.add) out[k] += old[k];
-          }
-          store_vec<T, VEC>(o, out);
-        }
+        if (p.zero) yb[at] = round_to<T>(A(0));
+      }
     }
-    if (p.zero)
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (i * G + t < slots)
-          store_zero<T, VEC>((T*)p.yb + (s * slots + i * G + t) * VEC);
   }
   if (!p.sums) return;
   A* part = (A*)p.part + (int64_t)blockIdx.x * 2 * p.n_d;
-  if constexpr (R > 1) {
-    // the block's warps, added in order
-    extern __shared__ char sm_raw[];
-    A* sm = reinterpret_cast<A*>(sm_raw);       // 2 x n_d
-    for (int q = 0; q < R; ++q) {
-      if ((int)threadIdx.x / G == q)
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (i * G + t < slots)
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-              const int d = (i * G + t) * VEC + k;
-              sm[d] = q ? sm[d] + sw[i][k] : sw[i][k];
-              sm[p.n_d + d] = q ? sm[p.n_d + d] + sb[i][k] : sb[i][k];
-            }
-      __syncthreads();
+  for (int i = 0; i < NV; ++i)
+    if (i * G + t < p.n_d) {
+      part[i * G + t] = sw[i];
+      part[p.n_d + i * G + t] = sb[i];
     }
-    for (int d = threadIdx.x; d < 2 * p.n_d; d += G * R) part[d] = sm[d];
-  } else {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (i * G + t < slots)
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          part[(i * G + t) * VEC + k] = sw[i][k];
-          part[p.n_d + (i * G + t) * VEC + k] = sb[i][k];
-        }
-  }
 }
 
 // ---- rings of rows -------------------------------------------------------------------
@@ -247,17 +173,12 @@ __device__ int g_norm_error = 0;
 
 constexpr int kMaxStages = 8;
 
-// v[i] = f(sum of v[i] over the block), the same in every thread: within a warp
-// by halving (each step adds one half of the values to the lanes that keep
-// it), then one barrier and the warps' sums; f runs once, on the lanes that
-// hold the sums, before they are spread (a division and a root per row in
-// every thread were a third of the forward's instructions). `red`: 2 x 8 x 32
-// values, zero where the block has no warp, used alternately (`turn`), so that
-// no second barrier is needed.
-template <int N, class A, class F>
-__device__ __forceinline__ void block_sums(A (&v)[N], A (*red)[8][32], int turn, F f) {
-  constexpr int kLanes = 32 / N;       // lanes per value
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Sums of N values over a warp by halving: each step adds one half of the values
+// to the lanes that keep it. v[0] of lane l is then the sum of value l / (32 /
+// N).
+template <int N, class A>
+__device__ __forceinline__ void halve(A (&v)[N]) {
+  const int lane = threadIdx.x & 31;
   int n = N, off = 16;
 #pragma unroll
   for (int step = 0; step < 5; ++step, off >>= 1) {
@@ -274,6 +195,27 @@ __device__ __forceinline__ void block_sums(A (&v)[N], A (*red)[8][32], int turn,
       v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
     }
   }
+}
+// v[i] = f(sum of v[i] over the warp), the same in every lane.
+template <int N, class A, class F>
+__device__ __forceinline__ void warp_sums(A (&v)[N], F f) {
+  halve<N>(v);
+  const A s = f(v[0]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xffffffffu, s, i * (32 / N));
+}
+
+// v[i] = f(sum of v[i] over the block), the same in every thread: within a warp
+// by halving, then one barrier and the warps' sums; f runs once, on the lanes that
+// hold the sums, before they are spread (a division and a root per row in
+// every thread were a third of the forward's instructions). `red`: 2 x 8 x 32
+// values, zero where the block has no warp, used alternately (`turn`), so that
+// no second barrier is needed.
+template <int N, class A, class F>
+__device__ __forceinline__ void block_sums(A (&v)[N], A (*red)[8][32], int turn, F f) {
+  constexpr int kLanes = 32 / N;       // lanes per value
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  halve<N>(v);
   if (lane % kLanes == 0) red[turn][lane / kLanes][warp] = v[0];
   __syncthreads();
   A s = 0;
@@ -647,6 +589,186 @@ ln_bwd_ring_kernel(BwdArgs p, int stages) {
   own.store_params(part + p.n_d, sb);
 }
 
+// ---- a warp per row --------------------------------------------------------------------
+constexpr int kRowWarps = 8;
+
+// R rows a turn, all their loads in flight; M vectors (or their worth of single
+// columns) a lane.
+template <class T, int M, bool WIDE, int R>
+__global__ void __launch_bounds__(32 * kRowWarps)
+ln_fwd_warp_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
+                   const acc_t<T>* __restrict__ b, T* __restrict__ y,
+                   acc_t<T>* __restrict__ m_stack, acc_t<T>* __restrict__ r_stack, double eps,
+                   int64_t n_s, int n_d) {
+  using A = acc_t<T>;
+  using O = Own<T, M, WIDE>;
+  constexpr int E = O::E;
+  const int t = threadIdx.x & 31;
+  const O own(t, 32, n_d);
+  const int64_t row_bytes = n_d * (int64_t)sizeof(T);
+  Pair<A> wr[E / 2], br[E / 2];
+  own.params(w, A(1), wr);
+  own.params(b, A(0), br);
+  const bool mine = own.has(0);
+  const A inv = A(1) / (A)n_d;
+  const int64_t step = (int64_t)gridDim.x * kRowWarps * R;
+  for (int64_t s = ((int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * R; s < n_s; s += step) {
+    const uint8_t* in = reinterpret_cast<const uint8_t*>(x) + s * row_bytes;
+    uint8_t* out = reinterpret_cast<uint8_t*>(y) + s * row_bytes;
+    const int rows = (int)min((int64_t)R, n_s - s);
+    Pair<A> c[R][E / 2];
+    A v[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      if (q < rows && mine) own.load(in + q * row_bytes, c[q]);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      v[q] = 0;
+      if (q < rows && mine) {
+        Pair<A> sum = c[q][0];
+#pragma unroll
+        for (int k = 1; k < E / 2; ++k) sum = add2(sum, c[q][k]);
+        v[q] = sum.lo() + sum.hi();
+      }
+    }
+    warp_sums<R>(v, [&](A z) { return z * inv; });
+    A mean[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      mean[q] = v[q];
+      v[q] = 0;
+      if (q < rows && mine) {
+        const Pair<A> minus = both(-mean[q]);
+        Pair<A> sq = both(A(0));
+#pragma unroll
+        for (int k = 0; k < E / 2; ++k) {
+          c[q][k] = add2(c[q][k], minus);
+          if constexpr (WIDE) {
+            if (M == 1 || own.has(2 * k)) sq = fma2(c[q][k], c[q][k], sq);
+          } else {
+            const Pair<A> z(own.has(2 * k) ? c[q][k].lo() : A(0),
+                            own.has(2 * k + 1) ? c[q][k].hi() : A(0));
+            sq = fma2(z, z, sq);
+          }
+        }
+        v[q] = sq.lo() + sq.hi();
+      }
+    }
+    warp_sums<R>(v, [&](A z) { return A(1) / sqrt(z * inv + (A)eps); });
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      if (q < rows) {
+        if (mine) {
+          const Pair<A> rstd = both(v[q]);
+#pragma unroll
+          for (int k = 0; k < E / 2; ++k) c[q][k] = fma2(mul2(c[q][k], rstd), wr[k], br[k]);
+          own.store(out + q * row_bytes, c[q]);
+        }
+        if (t == 0) {
+          m_stack[s + q] = mean[q];
+          r_stack[s + q] = v[q];
+        }
+      }
+  }
+}
+
+template <class T, int M, bool WIDE, int R>
+__global__ void __launch_bounds__(32 * kRowWarps, 2)
+ln_bwd_warp_kernel(BwdArgs p) {
+  using A = acc_t<T>;
+  using O = Own<T, M, WIDE>;
+  constexpr int E = O::E;
+  const int t = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const O own(t, 32, p.n_d);
+  const int64_t row_bytes = p.n_d * (int64_t)sizeof(T);
+  const A* m = (const A*)p.m;
+  const A* r = (const A*)p.r;
+  Pair<A> w[E / 2], sw[E / 2], sb[E / 2];
+  own.params((const A*)p.w, A(1), w);
+#pragma unroll
+  for (int k = 0; k < E / 2; ++k) sw[k] = sb[k] = both(A(0));
+  const bool mine = own.has(0);
+  const A inv = A(1) / (A)p.n_d;
+  const int64_t step = (int64_t)gridDim.x * kRowWarps * R;
+  for (int64_t s = ((int64_t)blockIdx.x * kRowWarps + warp) * R; s < p.n_s; s += step) {
+    const int rows = (int)min((int64_t)R, p.n_s - s);
+    const int64_t at = s * row_bytes;
+    Pair<A> cx[R][E / 2], cy[R][E / 2];     // x and yb, then h and g w
+    A rstd[R], v[2 * R];
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      if (q < rows && mine) {
+        own.load((const uint8_t*)p.x + at + q * row_bytes, cx[q]);
+        own.load((const uint8_t*)p.yb + at + q * row_bytes, cy[q]);
+      }
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      rstd[q] = q < rows ? r[s + q] : A(0);
+      const A shift = q < rows ? -m[s + q] * rstd[q] : A(0);
+      v[2 * q] = v[2 * q + 1] = A(0);
+      if (q < rows && mine) {
+        Pair<A> sg = both(A(0)), sgh = both(A(0));
+        const Pair<A> rs = both(rstd[q]), sh = both(shift);
+#pragma unroll
+        for (int k = 0; k < E / 2; ++k) {
+          // columns the lane does not have: yb = 0 there, so nothing is added
+          const Pair<A> h = fma2(cx[q][k], rs, sh), g = cy[q][k], gw = mul2(g, w[k]);
+          sg = add2(sg, gw);
+          sgh = fma2(gw, h, sgh);
+          sw[k] = fma2(g, h, sw[k]);
+          sb[k] = add2(sb[k], g);
+          cx[q][k] = h;
+          cy[q][k] = gw;
+        }
+        v[2 * q] = sg.lo() + sg.hi();
+        v[2 * q + 1] = sgh.lo() + sgh.hi();
+      }
+    }
+    warp_sums<2 * R>(v, [&](A z) { return z * inv; });
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      if (q < rows && mine) {
+        if (p.xb) {
+          uint8_t* o = (uint8_t*)p.xb + at + q * row_bytes;
+          const Pair<A> rs = both(rstd[q]);
+          const Pair<A> mg = both(-v[2 * q] * rstd[q]), mgh = both(-v[2 * q + 1] * rstd[q]);
+#pragma unroll
+          for (int k = 0; k < E / 2; ++k) cx[q][k] = fma2(cy[q][k], rs, fma2(cx[q][k], mgh, mg));
+          if (p.add) {
+            own.load(o, cy[q]);
+#pragma unroll
+            for (int k = 0; k < E / 2; ++k) cx[q][k] = add2(cx[q][k], cy[q][k]);
+          }
+          own.store(o, cx[q]);
+        }
+        if (p.zero) {
+#pragma unroll
+          for (int k = 0; k < E / 2; ++k) cy[q][k] = both(A(0));
+          own.store((uint8_t*)p.yb + at + q * row_bytes, cy[q]);
+        }
+      }
+  }
+  if (!p.sums) return;
+  // the block's warps, added in order
+  extern __shared__ __align__(128) uint8_t sm[];
+  A* part = reinterpret_cast<A*>(sm);       // 2 x n_d
+  for (int q = 0; q < kRowWarps; ++q) {
+    if (warp == q)
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (own.has(e)) {
+          const int d = own.col(e);
+          const A a = e % 2 ? sw[e / 2].hi() : sw[e / 2].lo();
+          const A z = e % 2 ? sb[e / 2].hi() : sb[e / 2].lo();
+          part[d] = q ? part[d] + a : a;
+          part[p.n_d + d] = q ? part[p.n_d + d] + z : z;
+        }
+    __syncthreads();
+  }
+  A* out = (A*)p.part + (int64_t)blockIdx.x * 2 * p.n_d;
+  for (int d = threadIdx.x; d < 2 * p.n_d; d += 32 * kRowWarps) out[d] = part[d];
+}
+
 // wb and bb from the partials [count][2][n_d]: 32 columns a block, 32 warps
 // that each add every 32nd partial, then the warps' sums in order.
 template <class A>
@@ -654,6 +776,7 @@ __global__ void __launch_bounds__(1024)
 ln_finish_kernel(const A* __restrict__ part, int count, int64_t n_d, A* __restrict__ wb,
                  A* __restrict__ bb, bool add) {
   __shared__ A sm[32][33];
+  after_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t d = (int64_t)blockIdx.x * 32 + lane;    // 0 .. 2 n_d - 1: wb, then bb
   A acc = 0;
@@ -749,25 +872,19 @@ ln_bwd_w_long_kernel(const T* __restrict__ x, T* __restrict__ yb,
 }
 
 // ---- which kernel --------------------------------------------------------------------
-// Calls f(VEC) with the widest vector the rows allow (`align` bytes) that
-// still gives each lane of a warp one.
-template <class T, class F>
-stade_status with_vec(int align, int64_t n_d, F&& f) {
-  using std::integral_constant;
-  constexpr int W = 16 / (int)sizeof(T);
-  if (align >= 16 && n_d >= 32 * W) return f(integral_constant<int, W>{});
-  if constexpr (sizeof(T) == 2)
-    if (align >= 4 && n_d >= 64) return f(integral_constant<int, 2>{});
-  return f(integral_constant<int, 1>{});
-}
-
-// Blocks of the reverse sweep, and so partials of the sums over rows: about
-// 1,024 threads an SM, but at least 32 rows a block beyond two blocks an SM (a
-// block's partials cost 16 bytes a column, its rows 6 to 12 bytes each).
+// Blocks of the reverse sweep, and so partials of the sums over rows.
 constexpr int64_t kBwdBlocks = 148 * 8;
-int64_t bwd_blocks(int64_t n_s, int threads) {
-  const int64_t fill = 148 * (1024 / threads);
-  return std::min<int64_t>(fill, std::max<int64_t>(148 * 2, n_s / 32));
+
+// Rows of less than 96 vectors of 16 bytes go to a warp each: calls f(M, WIDE).
+template <class F>
+stade_status with_row_warps(int64_t slots, bool wide, F&& f) {
+  using std::integral_constant;
+  auto m = [&](auto wd) {
+    if (slots <= 32) return f(integral_constant<int, 1>{}, wd);
+    if (slots <= 64) return f(integral_constant<int, 2>{}, wd);
+    return f(integral_constant<int, 3>{}, wd);
+  };
+  return wide ? m(std::true_type{}) : m(std::false_type{});
 }
 
 // Ring kernels: a block of `threads` threads a row (m vectors each), `rows` rows
@@ -807,46 +924,50 @@ template <class T>
 stade_status fwd(const void* x, const void* w, const void* b, void* y, void* m, void* r, double eps,
                  int64_t n_s, int64_t n_d, cudaStream_t st) {
   using A = acc_t<T>;
-  using std::integral_constant;
-  const int align = row_align(n_d * sizeof(T), {x, y});
+  const bool wide = row_align(n_d * sizeof(T), {x, y}) == 16;
+  const int64_t row_bytes = n_d * (int64_t)sizeof(T), slots = (row_bytes + 15) / 16;
+  if (slots < 96)
+    return with_row_warps(slots, wide, [&](auto mm, auto wd) {
+      constexpr int M = decltype(mm)::value, R = M == 1 ? 4 : 2;
+      const int64_t turns = (n_s + R * kRowWarps - 1) / (R * kRowWarps);
+      ln_fwd_warp_kernel<T, M, decltype(wd)::value, R>
+          <<<(unsigned)std::min<int64_t>(turns, 148 * 8), 32 * kRowWarps, 0, st>>>(
+              (const T*)x, (const A*)w, (const A*)b, (T*)y, (A*)m, (A*)r, eps, n_s, (int)n_d);
+      STADE_CHECK_LAUNCH();
+      return (stade_status)STADE_OK;
+    });
   RingPlan rp;
-  if (row_align(16, {x}) == 16 && ring_plan(n_s, n_d * sizeof(T), false, align == 16, &rp)) {
-    auto go = [&](auto wide) {
-      constexpr bool WIDE = decltype(wide)::value;
+  if (row_align(16, {x}) == 16 && ring_plan(n_s, row_bytes, false, wide, &rp)) {
+    auto go = [&](auto wd) {
+      constexpr bool WIDE = decltype(wd)::value;
       auto kern = rp.m == 2 ? ln_fwd_ring_kernel<T, 2, WIDE, 1, 768, 1>
                   : rp.threads > 512 ? (rp.rows == 2 ? ln_fwd_ring_kernel<T, 1, WIDE, 2, 1024, 1>
                                                      : ln_fwd_ring_kernel<T, 1, WIDE, 1, 1024, 1>)
                   : rp.rows == 4 ? ln_fwd_ring_kernel<T, 1, WIDE, 4, 512, 2>
                   : rp.rows == 2 ? ln_fwd_ring_kernel<T, 1, WIDE, 2, 512, 2>
                                  : ln_fwd_ring_kernel<T, 1, WIDE, 1, 512, 2>;
-      STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rp.smem));
-      kern<<<rp.blocks, rp.threads, rp.smem, st>>>((const T*)x, (const A*)w, (const A*)b, (T*)y, (A*)m,
-                                                   (A*)r, eps, n_s, (int)n_d, rp.stages);
+      STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)rp.smem));
+      kern<<<rp.blocks, rp.threads, rp.smem, st>>>((const T*)x, (const A*)w, (const A*)b, (T*)y,
+                                                   (A*)m, (A*)r, eps, n_s, (int)n_d, rp.stages);
       STADE_CHECK_LAUNCH();
       return (stade_status)STADE_OK;
     };
-    return align == 16 ? go(std::true_type{}) : go(std::false_type{});
+    return wide ? go(std::true_type{}) : go(std::false_type{});
   }
-  return with_vec<T>(align, n_d, [&](auto vec) {
-    constexpr int VEC = decltype(vec)::value;
-    const int64_t slots = n_d / VEC;
-    auto go = [&](auto g, auto nv) {
-      constexpr int G = decltype(g)::value, NV = decltype(nv)::value, R = rows_per_block<G>();
-      ln_fwd_kernel<T, VEC, G, NV><<<ceil_div_u(n_s, R), G * R, 0, st>>>(
-          (const T*)x, (const A*)w, (const A*)b, (T*)y, (A*)m, (A*)r, eps, n_s, (int)n_d);
-      STADE_CHECK_LAUNCH();
-      return (stade_status)STADE_OK;
-    };
-    if (slots <= 64) return go(integral_constant<int, 32>{}, integral_constant<int, 2>{});
-    if (slots <= 256) return go(integral_constant<int, 32>{}, integral_constant<int, 8>{});
-    if (slots <= 1024) return go(integral_constant<int, 128>{}, integral_constant<int, 8>{});
-    if (slots <= 4096) return go(integral_constant<int, 512>{}, integral_constant<int, 8>{});
-    if (slots <= 8192) return go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
+  void (*kern)(const T*, const A*, const A*, T*, A*, A*, double, int) = nullptr;
+  int threads = 0;
+  if (n_d <= 1024) kern = ln_fwd_kernel<T, 128, 8>, threads = 128;
+  else if (n_d <= 4096) kern = ln_fwd_kernel<T, 512, 8>, threads = 512;
+  else if (n_d <= 8192) kern = ln_fwd_kernel<T, 1024, 8>, threads = 1024;
+  if (kern)
+    kern<<<(unsigned)n_s, threads, 0, st>>>((const T*)x, (const A*)w, (const A*)b, (T*)y, (A*)m,
+                                            (A*)r, eps, (int)n_d);
+  else
     ln_fwd_long_kernel<T><<<(unsigned)n_s, kThreads, 0, st>>>(
         (const T*)x, (const A*)w, (const A*)b, (T*)y, (A*)m, (A*)r, eps, n_d);
-    STADE_CHECK_LAUNCH();
-    return (stade_status)STADE_OK;
-  });
+  STADE_CHECK_LAUNCH();
+  return STADE_OK;
 }
 
 template <class T>
@@ -854,50 +975,52 @@ stade_status bwd(const void* x, void* xb, const void* w, void* wb, void* bb, voi
                  const void* m, const void* r, int64_t n_s, int64_t n_d, void* ws, bool add,
                  bool zero, cudaStream_t st) {
   using A = acc_t<T>;
-  using std::integral_constant;
   const bool sums = wb || bb;
   if (!xb && !sums && !zero) return STADE_OK;
+  const bool wide = row_align(n_d * sizeof(T), {x, xb, yb}) == 16;
+  const int64_t row_bytes = n_d * (int64_t)sizeof(T), slots = (row_bytes + 15) / 16;
   int count = 0;
-  const int align = row_align(n_d * sizeof(T), {x, xb, yb});
   RingPlan rp;
   stade_status e = STADE_OK;
-  if (row_align(16, {x, yb}) == 16 && ring_plan(n_s, n_d * sizeof(T), true, align == 16, &rp)) {
+  if (slots < 96) {
+    e = with_row_warps(slots, wide, [&](auto mm, auto wd) {
+      constexpr int M = decltype(mm)::value, R = M == 1 ? 2 : 1;
+      const int64_t turns = (n_s + R * kRowWarps - 1) / (R * kRowWarps);
+      count = (int)std::min<int64_t>(turns, 148 * 2);
+      const BwdArgs p{x, w, m, r, xb, yb, ws, n_s, (int)n_d, add, zero, sums};
+      ln_bwd_warp_kernel<T, M, decltype(wd)::value, R>
+          <<<count, 32 * kRowWarps, 2 * n_d * sizeof(A), st>>>(p);
+      STADE_CHECK_LAUNCH();
+      return (stade_status)STADE_OK;
+    });
+  } else if (row_align(16, {x, yb}) == 16 && ring_plan(n_s, row_bytes, true, wide, &rp)) {
     count = rp.blocks;
     const BwdArgs p{x, w, m, r, xb, yb, ws, n_s, (int)n_d, add, zero, sums};
-    auto go = [&](auto wide) {
-      constexpr bool WIDE = decltype(wide)::value;
+    auto go = [&](auto wd) {
+      constexpr bool WIDE = decltype(wd)::value;
       void (*kern)(BwdArgs, int) = rp.threads > 512 ? ln_bwd_ring_kernel<T, 2, WIDE, 1, 768, false>
                                                    : ln_bwd_ring_kernel<T, 2, WIDE, 1, 512, true>;
       if constexpr (!WIDE)
         if (rp.m == 1)
           kern = rp.rows == 2 ? ln_bwd_ring_kernel<T, 1, false, 2, 512, true>
                               : ln_bwd_ring_kernel<T, 1, false, 1, 512, true>;
-      STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)rp.smem));
+      STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)rp.smem));
       kern<<<rp.blocks, rp.threads, rp.smem, st>>>(p, rp.stages);
       STADE_CHECK_LAUNCH();
       return (stade_status)STADE_OK;
     };
-    e = align == 16 ? go(std::true_type{}) : go(std::false_type{});
+    e = wide ? go(std::true_type{}) : go(std::false_type{});
+  } else if (n_d <= 4096) {
+    const BwdArgs p{x, w, m, r, xb, yb, ws, n_s, (int)n_d, add, zero, sums};
+    const int threads = n_d <= 512 ? 128 : n_d <= 1024 ? 256 : n_d <= 2048 ? 512 : 1024;
+    auto kern = threads == 128 ? ln_bwd_kernel<T, 128, 4>
+                : threads == 256 ? ln_bwd_kernel<T, 256, 4>
+                : threads == 512 ? ln_bwd_kernel<T, 512, 4> : ln_bwd_kernel<T, 1024, 4>;
+    count = (int)std::min<int64_t>(n_s, 148 * (1024 / threads));
+    kern<<<count, threads, 0, st>>>(p);
+    STADE_CHECK_LAUNCH();
   } else {
-    e = with_vec<T>(align, n_d, [&](auto vec) {
-    constexpr int VEC = decltype(vec)::value;
-    const int64_t slots = n_d / VEC;
-    auto go = [&](auto g, auto nv) {
-      constexpr int G = decltype(g)::value, NV = decltype(nv)::value, R = rows_per_block<G>();
-      count = (int)std::min<int64_t>((n_s + R - 1) / R, bwd_blocks(n_s, G * R));
-      const BwdArgs p{x, w, m, r, xb, yb, ws, n_s, (int)n_d, add, zero, sums};
-      ln_bwd_kernel<T, VEC, G, NV><<<count, G * R, R > 1 ? 2 * n_d * sizeof(A) : 0, st>>>(p);
-      STADE_CHECK_LAUNCH();
-      return (stade_status)STADE_OK;
-    };
-    constexpr int NV = VEC >= 4 ? 2 : 4;
-    if (slots <= 32 * NV) return go(integral_constant<int, 32>{}, integral_constant<int, NV>{});
-    if (slots <= 128 * NV) return go(integral_constant<int, 128>{}, integral_constant<int, NV>{});
-    if (slots <= 256 * NV) return go(integral_constant<int, 256>{}, integral_constant<int, NV>{});
-    if (slots <= 512 * NV) return go(integral_constant<int, 512>{}, integral_constant<int, NV>{});
-    // 1,024 threads leave 64 registers each: enough for narrow vectors only
-    if constexpr (VEC == 1)
-      if (slots <= 1024 * NV) return go(integral_constant<int, 1024>{}, integral_constant<int, NV>{});
     if (xb) {
       ln_bwd_x_long_kernel<T><<<(unsigned)n_s, kThreads, 0, st>>>(
           (const T*)x, (T*)xb, (const A*)w, (const T*)yb, (const A*)m, (const A*)r, n_d, add);
@@ -909,14 +1032,10 @@ stade_status bwd(const void* x, void* xb, const void* w, void* wb, void* bb, voi
     ln_bwd_w_long_kernel<T><<<grid, kThreads, 0, st>>>((const T*)x, (T*)yb, (const A*)m,
                                                        (const A*)r, n_s, n_d, rows, (A*)ws, zero);
     STADE_CHECK_LAUNCH();
-    return (stade_status)STADE_OK;
-    });
   }
   if (e != STADE_OK || !sums) return e;
-  ln_finish_kernel<A><<<ceil_div_u(2 * n_d, 32), 1024, 0, st>>>((const A*)ws, count, n_d, (A*)wb,
-                                                                (A*)bb, add);
-  STADE_CHECK_LAUNCH();
-  return STADE_OK;
+  return launch_next(ln_finish_kernel<A>, ceil_div_u(2 * n_d, 32), 1024, 0, st, (const A*)ws, count,
+                     n_d, (A*)wb, (A*)bb, add);
 }
 
 stade_status check_sizes(const char* who, int dtype, int64_t n_s, int64_t n_d) {
