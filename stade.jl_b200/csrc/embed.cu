@@ -400,7 +400,17 @@ window_sum_kernel(SumArgs p) {
   };
   const T* yb = (const T*)p.yb;
   const A scale = (A)p.scale;
-  A acc[kCols][VEC] = {};
+  // sums in pairs (one value a vector where rows allow no more)
+  constexpr int NP = VEC > 1 ? VEC / 2 : 1;
+  Pair<A> acc[kCols][NP];
+  bool has[kCols];
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) {
+    has[c] = col + c * 32 * VEC < p.n_d;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) acc[c][j] = both(A(0));
+  }
+  const T* mine = yb + col;
   int first = 0;                       // where the current run begins in the window
   for (int i0 = 0; i0 < len; i0 += U) {
     if (key_of(i0) == none) break;     // padding sorts last
@@ -410,10 +420,10 @@ window_sum_kernel(SumArgs p) {
       const int i = i0 + u;
       const uint32_t row = __shfl_sync(0xffffffffu, i < 32 ? at[0] : at[1], i & 31);
       if (i < len) {
-        const T* q = yb + (int64_t)row * p.n_d + col;
+        const T* q = mine + (int64_t)row * p.n_d;
 #pragma unroll
         for (int c = 0; c < kCols; ++c)
-          if (col + c * 32 * VEC < p.n_d) r[u][c] = *reinterpret_cast<const V*>(q + c * 32 * VEC);
+          if (has[c]) r[u][c] = *reinterpret_cast<const V*>(q + c * 32 * VEC);
       }
     }
 #pragma unroll
@@ -423,9 +433,13 @@ window_sum_kernel(SumArgs p) {
       if (i >= len || k == none) break;
 #pragma unroll
       for (int c = 0; c < kCols; ++c)
-        if (col + c * 32 * VEC < p.n_d)
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[c][j] += load_acc<T>(r[u][c].v[j]);
+        for (int j = 0; j < NP; ++j) {
+          if constexpr (VEC > 1)
+            acc[c][j] = add2(acc[c][j], widen2(reinterpret_cast<const Vec<T, 2>*>(&r[u][c])[j]));
+          else
+            acc[c][j] = Pair<A>(acc[c][j].lo() + load_acc<T>(r[u][c].v[0]), A(0));
+        }
       const bool edge = i + 1 == len;
       if (!edge && k1 == k) continue;
       // the run, or the window's share of it, ends here
@@ -434,12 +448,16 @@ window_sum_kernel(SumArgs p) {
       A* o = whole ? (A*)p.wb + (int64_t)k * p.n_d
                    : (A*)p.part + (2 * win + (begun ? 1 : 0)) * p.n_d;
 #pragma unroll
-      for (int c = 0; c < kCols; ++c)
-        if (col + c * 32 * VEC < p.n_d) {
-          put<A, VEC>(o + col + c * 32 * VEC, acc[c], whole ? scale : A(1), whole && p.add);
+      for (int c = 0; c < kCols; ++c) {
+        if (has[c]) {
+          A v[VEC];
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[c][j] = 0;
+          for (int j = 0; j < VEC; ++j) v[j] = j % 2 ? acc[c][j / 2].hi() : acc[c][j / 2].lo();
+          put<A, VEC>(o + col + c * 32 * VEC, v, whole ? scale : A(1), whole && p.add);
         }
+#pragma unroll
+        for (int j = 0; j < NP; ++j) acc[c][j] = both(A(0));
+      }
       first = i + 1;
     }
   }
@@ -457,10 +475,11 @@ join_kernel(SumArgs p) {
   const int64_t win = item / chunks, p1 = (win + 1) * p.width;
   if (p1 >= p.n) return;
   after_previous();
-  const uint32_t k = p.keys[p1 - 1];
-  if (k == (uint32_t)p.n_v || p.keys[p1] != k) return;
   const int64_t p0 = win * p.width;
-  if (p0 > 0 && p.keys[p0 - 1] == k) return;     // begun before this window
+  const uint32_t k = p.keys[p1 - 1], next = p.keys[p1];
+  const uint32_t before = p0 > 0 ? p.keys[p0 - 1] : 0xffffffffu;
+  // nothing goes on past the window, or what does has begun before it
+  if (k == (uint32_t)p.n_v || next != k || before == k) return;
   // heads: of window win + 1 + j while its first key is k
   int64_t heads = 0;
   for (;;) {

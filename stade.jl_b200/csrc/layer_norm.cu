@@ -290,41 +290,35 @@ struct Ring {
   }
 };
 
-// The E columns of a row that a thread owns, in pairs: WIDE, M vectors of 16
-// bytes, vector i at slot i G + t; else single columns e G + t, for rows that
-// are no multiple of 16 bytes (one 2- or 4-byte access each, still 64 or 128
-// bytes a warp).
-template <class T, int M, bool WIDE>
+// The E columns of a row that a thread owns, in pairs: E / VW vectors of VW
+// values, vector i at slot i G + t. VW is 16 bytes' worth where rows are
+// multiples of 16 bytes, else two values or one (still 64 bytes or more a warp).
+template <class T, int E_, int VW>
 struct Own {
   using A = acc_t<T>;
-  static constexpr int VEC = 16 / (int)sizeof(T), E = VEC * M;
+  static constexpr int E = E_;
+  static_assert(E % 2 == 0 && E % VW == 0, "whole pairs and vectors");
   int t, G, n_d;
-  uint32_t off, step;      // bytes: the first column, and from one vector (value) to the next
+  uint32_t off, step;      // bytes: the first column, and from one vector to the next
   __device__ __forceinline__ Own(int t_, int G_, int n_d_)
-      : t(t_), G(G_), n_d(n_d_), off(t_ * (WIDE ? 16 : (int)sizeof(T))),
-        step(G_ * (WIDE ? 16 : (int)sizeof(T))) {}
-  __device__ __forceinline__ bool has(int e) const {
-    return WIDE ? (e / VEC * G + t) * VEC < n_d : e * G + t < n_d;
-  }
-  __device__ __forceinline__ int col(int e) const {
-    return WIDE ? (e / VEC * G + t) * VEC + e % VEC : e * G + t;
-  }
-  // zeros where the thread has no column (one vector a thread: only called
-  // where it has it)
+      : t(t_), G(G_), n_d(n_d_), off(t_ * VW * (int)sizeof(T)), step(G_ * VW * (int)sizeof(T)) {}
+  __device__ __forceinline__ bool has(int e) const { return (e / VW * G + t) * VW < n_d; }
+  __device__ __forceinline__ int col(int e) const { return (e / VW * G + t) * VW + e % VW; }
+  // zeros where the thread has no column (a single vector: only called where
+  // it has it)
   __device__ __forceinline__ void load(const uint8_t* row, Pair<A> (&o)[E / 2]) const {
-    if constexpr (WIDE) {
+    if constexpr (VW > 1) {
 #pragma unroll
-      for (int i = 0; i < M; ++i) {
-        Vec<T, VEC> v;
-        if (M > 1) {
+      for (int i = 0; i < E / VW; ++i) {
+        Vec<T, VW> v;
+        if (E > VW) {
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) v.v[k] = round_to<T>(A(0));
+          for (int k = 0; k < VW; ++k) v.v[k] = round_to<T>(A(0));
         }
-        if (M == 1 || has(i * VEC))
-          v = *reinterpret_cast<const Vec<T, VEC>*>(row + off + i * step);
+        if (E == VW || has(i * VW)) v = *reinterpret_cast<const Vec<T, VW>*>(row + off + i * step);
 #pragma unroll
-        for (int k = 0; k < VEC / 2; ++k)
-          o[i * (VEC / 2) + k] = widen2(*reinterpret_cast<const Vec<T, 2>*>(&v.v[2 * k]));
+        for (int k = 0; k < VW / 2; ++k)
+          o[i * (VW / 2) + k] = widen2(*reinterpret_cast<const Vec<T, 2>*>(&v.v[2 * k]));
       }
     } else {
 #pragma unroll
@@ -336,14 +330,14 @@ struct Own {
     }
   }
   __device__ __forceinline__ void store(uint8_t* row, const Pair<A> (&o)[E / 2]) const {
-    if constexpr (WIDE) {
+    if constexpr (VW > 1) {
 #pragma unroll
-      for (int i = 0; i < M; ++i) {
-        Vec<T, VEC> v;
+      for (int i = 0; i < E / VW; ++i) {
+        Vec<T, VW> v;
 #pragma unroll
-        for (int k = 0; k < VEC / 2; ++k)
-          *reinterpret_cast<Vec<T, 2>*>(&v.v[2 * k]) = narrow2<T>(o[i * (VEC / 2) + k]);
-        if (has(i * VEC)) *reinterpret_cast<Vec<T, VEC>*>(row + off + i * step) = v;
+        for (int k = 0; k < VW / 2; ++k)
+          *reinterpret_cast<Vec<T, 2>*>(&v.v[2 * k]) = narrow2<T>(o[i * (VW / 2) + k]);
+        if (has(i * VW)) *reinterpret_cast<Vec<T, VW>*>(row + off + i * step) = v;
       }
     } else {
 #pragma unroll
@@ -353,6 +347,12 @@ struct Own {
           *reinterpret_cast<T*>(row + off + (e + 1) * step) = round_to<T>(o[e / 2].hi());
       }
     }
+  }
+  // the pair with zeros where the thread has no column
+  __device__ __forceinline__ Pair<A> only(int k, Pair<A> c) const {
+    if (E == VW) return c;
+    if (VW > 1) return has(2 * k) ? c : both(A(0));
+    return Pair<A>(has(2 * k) ? c.lo() : A(0), has(2 * k + 1) ? c.hi() : A(0));
   }
   __device__ __forceinline__ void params(const A* p, A other, Pair<A> (&o)[E / 2]) const {
 #pragma unroll
@@ -376,18 +376,17 @@ __device__ __forceinline__ void clear_red(A (*red)[8][32]) {
 
 // R rows a turn: what a turn costs beside its arithmetic (the wait, two
 // barriers, the shuffles) is shared by them.
-template <class T, int M, bool WIDE, int R, int MAXT, int MINB>
+template <class T, int E, int VW, int R, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB)
 ln_fwd_ring_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
                    const acc_t<T>* __restrict__ b, T* __restrict__ y,
                    acc_t<T>* __restrict__ m_stack, acc_t<T>* __restrict__ r_stack, double eps,
                    int64_t n_s, int n_d, int stages) {
   using A = acc_t<T>;
-  using O = Own<T, M, WIDE>;
-  constexpr int E = O::E;
+  using O = Own<T, E, VW>;
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ A red[2][8][32];
-  Ring<T, 1, WIDE> ring(sm, stages, R, n_d, n_s, x, nullptr);
+  Ring<T, 1, VW * sizeof(T) == 16> ring(sm, stages, R, n_d, n_s, x, nullptr);
   clear_red(red);
   const int t = threadIdx.x;
   const O own(t, (int)blockDim.x, n_d);
@@ -430,23 +429,13 @@ ln_fwd_ring_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
       mean[q] = v[q];
       const Pair<A> minus = both(-v[q]);
       Pair<A> sq = both(A(0));
-      if constexpr (WIDE) {
 #pragma unroll
-        for (int k = 0; k < E / 2; ++k) {
-          c[q][k] = add2(c[q][k], minus);
-          if (M == 1 || own.has(2 * k)) sq = fma2(c[q][k], c[q][k], sq);
-        }
-        v[q] = mine ? sq.lo() + sq.hi() : A(0);
-      } else {
-#pragma unroll
-        for (int k = 0; k < E / 2; ++k) {
-          c[q][k] = add2(c[q][k], minus);
-          const Pair<A> z(own.has(2 * k) ? c[q][k].lo() : A(0),
-                          own.has(2 * k + 1) ? c[q][k].hi() : A(0));
-          sq = fma2(z, z, sq);
-        }
-        v[q] = sq.lo() + sq.hi();
+      for (int k = 0; k < E / 2; ++k) {
+        c[q][k] = add2(c[q][k], minus);
+        const Pair<A> z = own.only(k, c[q][k]);
+        sq = fma2(z, z, sq);
       }
+      v[q] = mine ? sq.lo() + sq.hi() : A(0);
     }
     block_sums<R>(v, red, 1, [&](A z) { return A(1) / sqrt(z * inv + (A)eps); });
 #pragma unroll
@@ -475,15 +464,14 @@ ln_fwd_ring_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
 // turn's sums, not by memory: 16384 x 4096 takes 103 us in bf16 when the row is
 // read twice (32 instructions an element), 83 us kept, 61 us by memory alone;
 // in Float32 129 us, 0.95 of the measured copy rate.
-template <class T, int M, bool WIDE, int R, int MAXT, bool KEEP>
+template <class T, int E, int VW, int R, int MAXT, bool KEEP>
 __global__ void __launch_bounds__(MAXT, 1)
 ln_bwd_ring_kernel(BwdArgs p, int stages) {
   using A = acc_t<T>;
-  using O = Own<T, M, WIDE>;
-  constexpr int E = O::E;
+  using O = Own<T, E, VW>;
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ A red[2][8][32];
-  Ring<T, 2, WIDE> ring(sm, stages, R, p.n_d, p.n_s, p.x, p.yb);
+  Ring<T, 2, VW * sizeof(T) == 16> ring(sm, stages, R, p.n_d, p.n_s, p.x, p.yb);
   clear_red(red);
   const int t = threadIdx.x;
   const O own(t, (int)blockDim.x, p.n_d);
@@ -592,17 +580,17 @@ ln_bwd_ring_kernel(BwdArgs p, int stages) {
 // ---- a warp per row --------------------------------------------------------------------
 constexpr int kRowWarps = 8;
 
-// R rows a turn, all their loads in flight; M vectors (or their worth of single
-// columns) a lane.
-template <class T, int M, bool WIDE, int R>
-__global__ void __launch_bounds__(32 * kRowWarps)
+// R rows a turn, all their loads in flight. Lanes with more than 16 bytes of a
+// row take one row a turn and leave room for three blocks an SM (65536 x 512
+// bf16: 34 us; 44 with two rows).
+template <class T, int E, int VW, int R>
+__global__ void __launch_bounds__(32 * kRowWarps, R == 1 ? 3 : 1)
 ln_fwd_warp_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
                    const acc_t<T>* __restrict__ b, T* __restrict__ y,
                    acc_t<T>* __restrict__ m_stack, acc_t<T>* __restrict__ r_stack, double eps,
                    int64_t n_s, int n_d) {
   using A = acc_t<T>;
-  using O = Own<T, M, WIDE>;
-  constexpr int E = O::E;
+  using O = Own<T, E, VW>;
   const int t = threadIdx.x & 31;
   const O own(t, 32, n_d);
   const int64_t row_bytes = n_d * (int64_t)sizeof(T);
@@ -643,13 +631,8 @@ ln_fwd_warp_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
 #pragma unroll
         for (int k = 0; k < E / 2; ++k) {
           c[q][k] = add2(c[q][k], minus);
-          if constexpr (WIDE) {
-            if (M == 1 || own.has(2 * k)) sq = fma2(c[q][k], c[q][k], sq);
-          } else {
-            const Pair<A> z(own.has(2 * k) ? c[q][k].lo() : A(0),
-                            own.has(2 * k + 1) ? c[q][k].hi() : A(0));
-            sq = fma2(z, z, sq);
-          }
+          const Pair<A> z = own.only(k, c[q][k]);
+          sq = fma2(z, z, sq);
         }
         v[q] = sq.lo() + sq.hi();
       }
@@ -672,12 +655,15 @@ ln_fwd_warp_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
   }
 }
 
-template <class T, int M, bool WIDE, int R>
-__global__ void __launch_bounds__(32 * kRowWarps, 2)
+// blocks an SM that a lane's columns leave registers for
+template <class T, int E> constexpr int bwd_warp_blocks() {
+  return E <= 8 ? 4 : sizeof(T) == 4 ? 3 : 2;
+}
+template <class T, int E, int VW, int R>
+__global__ void __launch_bounds__(32 * kRowWarps, (bwd_warp_blocks<T, E>()))
 ln_bwd_warp_kernel(BwdArgs p) {
   using A = acc_t<T>;
-  using O = Own<T, M, WIDE>;
-  constexpr int E = O::E;
+  using O = Own<T, E, VW>;
   const int t = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const O own(t, 32, p.n_d);
   const int64_t row_bytes = p.n_d * (int64_t)sizeof(T);
@@ -875,16 +861,34 @@ ln_bwd_w_long_kernel(const T* __restrict__ x, T* __restrict__ yb,
 // Blocks of the reverse sweep, and so partials of the sums over rows.
 constexpr int64_t kBwdBlocks = 148 * 8;
 
-// Rows of less than 96 vectors of 16 bytes go to a warp each: calls f(M, WIDE).
-template <class F>
-stade_status with_row_warps(int64_t slots, bool wide, F&& f) {
+// Calls f(VW): what the rows' alignment allows an access to be.
+template <class T, class F>
+stade_status with_width(int align, F&& f) {
   using std::integral_constant;
-  auto m = [&](auto wd) {
-    if (slots <= 32) return f(integral_constant<int, 1>{}, wd);
-    if (slots <= 64) return f(integral_constant<int, 2>{}, wd);
-    return f(integral_constant<int, 3>{}, wd);
-  };
-  return wide ? m(std::true_type{}) : m(std::false_type{});
+  if (align >= 16) return f(integral_constant<int, 16 / (int)sizeof(T)>{});
+  if constexpr (sizeof(T) < 8)
+    if (align >= 2 * (int)sizeof(T)) return f(integral_constant<int, 2>{});
+  return f(integral_constant<int, 1>{});
+}
+
+// Rows of less than 96 times 16 bytes go to a warp each: calls f(E, VW), E the
+// columns of a lane. Vectors of 16 bytes only where most lanes get one.
+template <class T, class F>
+stade_status with_row_warps(int64_t n_d, int align, F&& f) {
+  using std::integral_constant;
+  constexpr int V = 16 / (int)sizeof(T);
+  if (align >= 16 && n_d < 24 * V) align = n_d < 48 ? (int)sizeof(T) : 2 * (int)sizeof(T);
+  return with_width<T>(align, [&](auto vw) {
+    constexpr int VW = decltype(vw)::value;
+    const int64_t per = (n_d + 32 * VW - 1) / (32 * VW) * VW;       // columns of a lane
+    if constexpr (VW <= 2 && V >= 4)
+      if (per <= 2) return f(integral_constant<int, 2>{}, vw);
+    if constexpr (VW <= 4 && V == 8)
+      if (per <= 4) return f(integral_constant<int, 4>{}, vw);
+    if (per <= V) return f(integral_constant<int, V>{}, vw);
+    if (per <= 2 * V) return f(integral_constant<int, 2 * V>{}, vw);
+    return f(integral_constant<int, 3 * V>{}, vw);
+  });
 }
 
 // Ring kernels: a block of `threads` threads a row (m vectors each), `rows` rows
@@ -924,36 +928,37 @@ template <class T>
 stade_status fwd(const void* x, const void* w, const void* b, void* y, void* m, void* r, double eps,
                  int64_t n_s, int64_t n_d, cudaStream_t st) {
   using A = acc_t<T>;
-  const bool wide = row_align(n_d * sizeof(T), {x, y}) == 16;
+  constexpr int V = 16 / (int)sizeof(T);
+  const int align = row_align(n_d * sizeof(T), {x, y});
   const int64_t row_bytes = n_d * (int64_t)sizeof(T), slots = (row_bytes + 15) / 16;
   if (slots < 96)
-    return with_row_warps(slots, wide, [&](auto mm, auto wd) {
-      constexpr int M = decltype(mm)::value, R = M == 1 ? 4 : 2;
+    return with_row_warps<T>(n_d, align, [&](auto ee, auto vw) {
+      constexpr int E = decltype(ee)::value, R = E <= V ? 4 : 1;
       const int64_t turns = (n_s + R * kRowWarps - 1) / (R * kRowWarps);
-      ln_fwd_warp_kernel<T, M, decltype(wd)::value, R>
-          <<<(unsigned)std::min<int64_t>(turns, 148 * 8), 32 * kRowWarps, 0, st>>>(
+      ln_fwd_warp_kernel<T, E, decltype(vw)::value, R>
+          <<<(unsigned)std::min<int64_t>(turns, 148 * (R == 1 ? 3 : 8)),
+             32 * kRowWarps, 0, st>>>(
               (const T*)x, (const A*)w, (const A*)b, (T*)y, (A*)m, (A*)r, eps, n_s, (int)n_d);
       STADE_CHECK_LAUNCH();
       return (stade_status)STADE_OK;
     });
   RingPlan rp;
-  if (row_align(16, {x}) == 16 && ring_plan(n_s, row_bytes, false, wide, &rp)) {
-    auto go = [&](auto wd) {
-      constexpr bool WIDE = decltype(wd)::value;
-      auto kern = rp.m == 2 ? ln_fwd_ring_kernel<T, 2, WIDE, 1, 768, 1>
-                  : rp.threads > 512 ? (rp.rows == 2 ? ln_fwd_ring_kernel<T, 1, WIDE, 2, 1024, 1>
-                                                     : ln_fwd_ring_kernel<T, 1, WIDE, 1, 1024, 1>)
-                  : rp.rows == 4 ? ln_fwd_ring_kernel<T, 1, WIDE, 4, 512, 2>
-                  : rp.rows == 2 ? ln_fwd_ring_kernel<T, 1, WIDE, 2, 512, 2>
-                                 : ln_fwd_ring_kernel<T, 1, WIDE, 1, 512, 2>;
+  if (row_align(16, {x}) == 16 && ring_plan(n_s, row_bytes, false, align == 16, &rp)) {
+    return with_width<T>(align, [&](auto vw) {
+      constexpr int VW = decltype(vw)::value;
+      auto kern = rp.m == 2 ? ln_fwd_ring_kernel<T, 2 * V, VW, 1, 768, 1>
+                  : rp.threads > 512 ? (rp.rows == 2 ? ln_fwd_ring_kernel<T, V, VW, 2, 1024, 1>
+                                                     : ln_fwd_ring_kernel<T, V, VW, 1, 1024, 1>)
+                  : rp.rows == 4 ? ln_fwd_ring_kernel<T, V, VW, 4, 512, 2>
+                  : rp.rows == 2 ? ln_fwd_ring_kernel<T, V, VW, 2, 512, 2>
+                                 : ln_fwd_ring_kernel<T, V, VW, 1, 512, 2>;
       STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)rp.smem));
       kern<<<rp.blocks, rp.threads, rp.smem, st>>>((const T*)x, (const A*)w, (const A*)b, (T*)y,
                                                    (A*)m, (A*)r, eps, n_s, (int)n_d, rp.stages);
       STADE_CHECK_LAUNCH();
       return (stade_status)STADE_OK;
-    };
-    return wide ? go(std::true_type{}) : go(std::false_type{});
+    });
   }
   void (*kern)(const T*, const A*, const A*, T*, A*, A*, double, int) = nullptr;
   int threads = 0;
@@ -977,40 +982,40 @@ stade_status bwd(const void* x, void* xb, const void* w, void* wb, void* bb, voi
   using A = acc_t<T>;
   const bool sums = wb || bb;
   if (!xb && !sums && !zero) return STADE_OK;
-  const bool wide = row_align(n_d * sizeof(T), {x, xb, yb}) == 16;
+  constexpr int V = 16 / (int)sizeof(T);
+  const int align = row_align(n_d * sizeof(T), {x, xb, yb});
   const int64_t row_bytes = n_d * (int64_t)sizeof(T), slots = (row_bytes + 15) / 16;
   int count = 0;
   RingPlan rp;
   stade_status e = STADE_OK;
   if (slots < 96) {
-    e = with_row_warps(slots, wide, [&](auto mm, auto wd) {
-      constexpr int M = decltype(mm)::value, R = M == 1 ? 2 : 1;
+    e = with_row_warps<T>(n_d, align, [&](auto ee, auto vw) {
+      constexpr int E = decltype(ee)::value, R = E <= V / 2 ? 2 : 1;
       const int64_t turns = (n_s + R * kRowWarps - 1) / (R * kRowWarps);
-      count = (int)std::min<int64_t>(turns, 148 * 2);
+      count = (int)std::min<int64_t>(turns, 148 * bwd_warp_blocks<T, E>());
       const BwdArgs p{x, w, m, r, xb, yb, ws, n_s, (int)n_d, add, zero, sums};
-      ln_bwd_warp_kernel<T, M, decltype(wd)::value, R>
+      ln_bwd_warp_kernel<T, E, decltype(vw)::value, R>
           <<<count, 32 * kRowWarps, 2 * n_d * sizeof(A), st>>>(p);
       STADE_CHECK_LAUNCH();
       return (stade_status)STADE_OK;
     });
-  } else if (row_align(16, {x, yb}) == 16 && ring_plan(n_s, row_bytes, true, wide, &rp)) {
+  } else if (row_align(16, {x, yb}) == 16 && ring_plan(n_s, row_bytes, true, align == 16, &rp)) {
     count = rp.blocks;
     const BwdArgs p{x, w, m, r, xb, yb, ws, n_s, (int)n_d, add, zero, sums};
-    auto go = [&](auto wd) {
-      constexpr bool WIDE = decltype(wd)::value;
-      void (*kern)(BwdArgs, int) = rp.threads > 512 ? ln_bwd_ring_kernel<T, 2, WIDE, 1, 768, false>
-                                                   : ln_bwd_ring_kernel<T, 2, WIDE, 1, 512, true>;
-      if constexpr (!WIDE)
+    e = with_width<T>(align, [&](auto vw) {
+      constexpr int VW = decltype(vw)::value;
+      void (*kern)(BwdArgs, int) = rp.threads > 512 ? ln_bwd_ring_kernel<T, 2 * V, VW, 1, 768, false>
+                                                   : ln_bwd_ring_kernel<T, 2 * V, VW, 1, 512, true>;
+      if constexpr (VW != V)
         if (rp.m == 1)
-          kern = rp.rows == 2 ? ln_bwd_ring_kernel<T, 1, false, 2, 512, true>
-                              : ln_bwd_ring_kernel<T, 1, false, 1, 512, true>;
+          kern = rp.rows == 2 ? ln_bwd_ring_kernel<T, V, VW, 2, 512, true>
+                              : ln_bwd_ring_kernel<T, V, VW, 1, 512, true>;
       STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)rp.smem));
       kern<<<rp.blocks, rp.threads, rp.smem, st>>>(p, rp.stages);
       STADE_CHECK_LAUNCH();
       return (stade_status)STADE_OK;
-    };
-    e = wide ? go(std::true_type{}) : go(std::false_type{});
+    });
   } else if (n_d <= 4096) {
     const BwdArgs p{x, w, m, r, xb, yb, ws, n_s, (int)n_d, add, zero, sums};
     const int threads = n_d <= 512 ? 128 : n_d <= 1024 ? 256 : n_d <= 2048 ? 512 : 1024;
