@@ -277,4 +277,128 @@ function mlp2_ce_hv_check_replicas(w1, b1, w2, b2, w1d, b1d, w2d, b2d, lossb, lo
     return nothing
 end
 
+# ---- operators of a token model's training step --------------------------------
+# embed, layer_norm, the 8-bit tape and expert_mm, each with its reverse sweep.
+# The element type T is the activation array's (Float32, Float64, Float16, or
+# Core.BFloat16 where CUDA.jl has it; not Float64 on the tape); parameters of
+# layer_norm, statistics and parameter adjoints are Float32, Float64 for
+# Float64. Arrays are in the library's row-major layout (rows of n_d
+# consecutive values). `accumulate = false` stores adjoints instead of adding,
+# `consume = false` leaves the seed yb.
+const STADE_ADJ_STORE = UInt32(2)
+const STADE_SEED_KEEP = UInt32(4)
+const STADE_ACT = Dict(:relu => 1, :tanh => 2, :silu => 3, :gelu => 4)
+
+function stade_dtype(T)
+    T === Float32 && return Cint(0)
+    T === Float64 && return Cint(1)
+    T === Float16 && return Cint(3)
+    nameof(T) === :BFloat16 && return Cint(2)
+    error("libstade_b200: unsupported element type $T")
+end
+adjoint_opts(accumulate, consume) =
+    opts(flags = (accumulate ? UInt32(0) : STADE_ADJ_STORE) |
+                 (consume ? UInt32(0) : STADE_SEED_KEEP))
+optional(a) = a === nothing ? CU_NULL : reinterpret(CuPtr{Cvoid}, pointer(a))
+rawptr(a) = reinterpret(CuPtr{Cvoid}, pointer(a))
+
+# ids count from 1; an id of 0 or less is padding
+function embed_cuda(w, ids, y, scale, n_s, n_v, n_d)
+    check(ccall((:stade_embed, libstade), Cint,
+        (Cint, CuPtr{Cvoid}, CuPtr{Int64}, CuPtr{Cvoid}, Float64, Int64, Int64, Int64, Int64,
+         Ref{StadeOpts}),
+        stade_dtype(eltype(y)), rawptr(w), ids, rawptr(y), scale, 1, n_s, n_v, n_d, opts()))
+    return nothing
+end
+
+function embed_b_cuda(wb, ids, yb, scale, n_s, n_v, n_d; accumulate = true, consume = true)
+    check(ccall((:stade_embed_b, libstade), Cint,
+        (Cint, CuPtr{Cvoid}, CuPtr{Int64}, CuPtr{Cvoid}, Float64, Int64, Int64, Int64, Int64,
+         Ref{StadeOpts}),
+        stade_dtype(eltype(yb)), rawptr(wb), ids, rawptr(yb), scale, 1, n_s, n_v, n_d,
+        adjoint_opts(accumulate, consume)))
+    return nothing
+end
+
+# w and b may be nothing (ones and zeros)
+function layer_norm_cuda(x, w, b, y, m_stack, r_stack, eps, n_s, n_d)
+    check(ccall((:stade_layer_norm, libstade), Cint,
+        (Cint, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid},
+         CuPtr{Cvoid}, Float64, Int64, Int64, Ref{StadeOpts}),
+        stade_dtype(eltype(x)), rawptr(x), optional(w), optional(b), rawptr(y), rawptr(m_stack),
+        rawptr(r_stack), eps, n_s, n_d, opts()))
+    return nothing
+end
+
+# xb, wb and bb may be nothing (not wanted)
+function layer_norm_b_cuda(x, xb, w, wb, bb, yb, m_stack, r_stack, n_s, n_d;
+                           accumulate = true, consume = true)
+    check(ccall((:stade_layer_norm_b, libstade), Cint,
+        (Cint, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid},
+         CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, Int64, Int64, Ref{StadeOpts}),
+        stade_dtype(eltype(x)), rawptr(x), optional(xb), optional(w), optional(wb), optional(bb),
+        rawptr(yb), rawptr(m_stack), rawptr(r_stack), n_s, n_d,
+        adjoint_opts(accumulate, consume)))
+    return nothing
+end
+
+function initstacks_tape8_cuda(n_s, n_d)
+    m = ccall((:stade_initstacks_tape8, libstade), Int64, (Int64, Int64), n_s, n_d)
+    return CuArray{Int8}(undef, max(n_s * n_d, 1)), CuArray{UInt8}(undef, max(m, 1))
+end
+
+function tape8_push_cuda(x, q_stack, e_stack, n_s, n_d)
+    check(ccall((:stade_tape8_push, libstade), Cint,
+        (Cint, CuPtr{Cvoid}, CuPtr{Int8}, CuPtr{UInt8}, Int64, Int64, Ref{StadeOpts}),
+        stade_dtype(eltype(x)), rawptr(x), q_stack, e_stack, n_s, n_d, opts()))
+    return nothing
+end
+
+function tape8_pop_cuda(x, q_stack, e_stack, n_s, n_d)
+    check(ccall((:stade_tape8_pop, libstade), Cint,
+        (Cint, CuPtr{Cvoid}, CuPtr{Int8}, CuPtr{UInt8}, Int64, Int64, Ref{StadeOpts}),
+        stade_dtype(eltype(x)), rawptr(x), q_stack, e_stack, n_s, n_d, opts()))
+    return nothing
+end
+
+# act: :relu, :tanh, :silu or :gelu
+function act_tape8_cuda(act, x, y, q_stack, e_stack, n_s, n_d)
+    check(ccall((:stade_act_tape8, libstade), Cint,
+        (Cint, Cint, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Int8}, CuPtr{UInt8}, Int64, Int64,
+         Ref{StadeOpts}),
+        stade_dtype(eltype(x)), STADE_ACT[act], rawptr(x), rawptr(y), q_stack, e_stack, n_s, n_d,
+        opts()))
+    return nothing
+end
+
+function act_tape8_b_cuda(act, xb, yb, q_stack, e_stack, n_s, n_d;
+                          accumulate = true, consume = true)
+    check(ccall((:stade_act_tape8_b, libstade), Cint,
+        (Cint, Cint, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Int8}, CuPtr{UInt8}, Int64, Int64,
+         Ref{StadeOpts}),
+        stade_dtype(eltype(yb)), STADE_ACT[act], rawptr(xb), rawptr(yb), q_stack, e_stack, n_s,
+        n_d, adjoint_opts(accumulate, consume)))
+    return nothing
+end
+
+# off: n_e + 1 row counts from 0 (off[e] rows come before expert e's)
+function expert_mm_cuda(x, w, y, off, n_s, n_e, n_i, n_o)
+    check(ccall((:stade_expert_mm, libstade), Cint,
+        (Cint, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Int64}, Int64, Int64, Int64, Int64,
+         Ref{StadeOpts}),
+        stade_dtype(eltype(x)), rawptr(x), rawptr(w), rawptr(y), off, n_s, n_e, n_i, n_o, opts()))
+    return nothing
+end
+
+# xb or wb may be nothing (not wanted)
+function expert_mm_b_cuda(x, xb, w, wb, yb, off, n_s, n_e, n_i, n_o;
+                          accumulate = true, consume = true)
+    check(ccall((:stade_expert_mm_b, libstade), Cint,
+        (Cint, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Int64},
+         Int64, Int64, Int64, Int64, Ref{StadeOpts}),
+        stade_dtype(eltype(yb)), rawptr(x), optional(xb), rawptr(w), optional(wb), rawptr(yb), off,
+        n_s, n_e, n_i, n_o, adjoint_opts(accumulate, consume)))
+    return nothing
+end
+
 end # module
