@@ -22,10 +22,10 @@
 // products down to 2^-16 of it, each an ordinary K loop over its two planes.
 //
 // The tensor cores' Float32 sums truncate: their error grows with the number
-// of MMAs into one accumulator, by about 2^-25 of it each. Where the result is
-// Float32 an accumulator takes at most kChain blocks of 64 before the epilogue
-// warps add it to round-to-nearest sums in registers; where it is rounded to
-// 16 bits the whole K stays in one.
+// of MMAs into one accumulator, by about 2^-25 of it each. An accumulator takes
+// a few blocks of 64 where the result is Float32 (kChain, kChain16), many where
+// it is rounded to 16 bits (kChainRound), before the epilogue warps add it to
+// round-to-nearest sums in registers.
 //
 // Warp roles per CTA: 0 TMA loads, 1 (of the leader) MMAs, 2 .. 17 epilogue, 18
 // zeroes the K tail. Every wait is bounded; one that runs out sets the device
@@ -71,6 +71,7 @@ static_assert(kBars * 8 + 4 <= 256, "barrier block");
 // 4096 in bf16: 365, 298, 285, 278 us. Float32 operands keep the tighter sums.
 constexpr int kChain = 4, kChain16 = 8;
 constexpr int kChainSmall = 64;  // the same for the plane products below 2^-7 of the result
+constexpr int kChainRound = 256; // where it is rounded to 16 bits: 3e-5, whatever K is
 
 struct Geom {
   int M;           // output's contiguous extent
@@ -663,7 +664,7 @@ stade_status expert_tc_rows(int dtype, const ExpertOperand& in, const ExpertOper
   g.m_tiles = (g.M + 2 * kHalfM - 1) / (2 * kHalfM);
   g.n_tiles = 1;
   g.planes = (int)expert_planes(dtype);
-  g.chain = dtype == STADE_F32 ? kChain : 1 << 20;
+  g.chain = dtype == STADE_F32 ? kChain : kChainRound;
   g.a_mn = !trans;
   g.b_mn = false;
   g.bf16 = dtype != STADE_F16;

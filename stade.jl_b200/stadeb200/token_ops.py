@@ -21,7 +21,7 @@ import torch
 
 from ._lib import (STADE_ADJ_STORE, STADE_BF16, STADE_F16, STADE_F32, STADE_F64, STADE_OK,
                    STADE_SEED_KEEP, check, lib, stade_opts)
-from .kernels import _arr
+from . import kernels
 
 _DTYPES = {torch.float32: STADE_F32, torch.float64: STADE_F64, torch.bfloat16: STADE_BF16,
            torch.float16: STADE_F16}
@@ -39,10 +39,17 @@ def _dtype(t, name: str):
     types = _TYPES.get(t.dtype)
     if types is None:
         raise TypeError(f"{name}: unsupported dtype {t.dtype}")
-    if t.is_cuda and t.get_device() != torch.cuda.current_device():
+    return types
+
+
+def _arr(t, dtype, n: int, name: str) -> int:
+    """Address of an array after its checks: CUDA, type, contiguity, length,
+    and the current device, on which the call runs."""
+    p = kernels._arr(t, dtype, n, name)
+    if t.get_device() != torch.cuda.current_device():
         raise ValueError(f"{name}: tensor lives on {t.device}, the current device is "
                          f"cuda:{torch.cuda.current_device()}")
-    return types
+    return p
 
 
 # The current stream's handle without building a Stream object, which costs as

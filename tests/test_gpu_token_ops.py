@@ -355,6 +355,21 @@ def test_act_tape8(n_s, n_d, off, act, dt):
     assert not yb.any()
 
 
+@pytest.mark.parametrize("dt", NO64)
+@pytest.mark.parametrize("n_d", [64, 61])
+def test_act_tape8_b_in_place(n_d, dt):
+    """xb and yb may be one array when adjoints are stored and the seed kept."""
+    dt = R.DTYPES[dt]
+    x, yb = _dev(_rand(1, 9, n_d), dt), _dev(_rand(2, 9, n_d), dt)
+    q, e = sb.initstacks_tape8_cuda(9, n_d)
+    sb.act_tape8_cuda("gelu", x, torch.empty_like(x), q, e, 9, n_d)
+    xb = torch.empty_like(x)
+    new = dict(accumulate=False, consume=False)
+    sb.act_tape8_b_cuda("gelu", xb, yb, q, e, 9, n_d, **new)
+    sb.act_tape8_b_cuda("gelu", yb, yb, q, e, 9, n_d, **new)
+    assert torch.equal(xb, yb)
+
+
 @pytest.mark.parametrize("act", list(T.ACTIVATIONS))
 def test_act_tape8_slope_against_differences(act):
     """Where the tape holds x exactly (whole sixty-fourths below one), the
