@@ -11,7 +11,9 @@
 // every group into row tiles, and the product kernels walk that list. Bounds
 // that fall or leave 0 .. n_s are clamped and set the device error word.
 
+#include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
 #include "expert_tc.cuh"
 #include "token_ops.cuh"
@@ -173,6 +175,146 @@ expert_wgrad_kernel(const T* __restrict__ x, const T* __restrict__ yb, acc_t<T>*
                          (int)min((int64_t)kTile, n_o - o0), b - a, add);
 }
 
+// ---- few rows, Float32 ------------------------------------------------------------
+// With a handful of rows a group the time is one read of the weights. The
+// tensor cores' path writes them out as three planes first and reads those: six
+// times the bytes (6 rows, 2 experts, 2328 -> 3688: 107 us, of which 10 us is
+// the read). Here tiles of kFew rows multiply on the CUDA cores, the rows in
+// shared memory, the weights read once per tile straight into registers.
+constexpr int kFew = 8;
+constexpr int kFewK = 512;      // depth of one block's share of y = x W
+constexpr int kFewWarps = 8;
+
+// y = x W: a block takes 32 V columns of a tile and kFewK of the depth, a warp
+// an eighth of that; the warps' sums are added in order. part: [slice][row][n_o]
+// where the depth takes several blocks, else y itself.
+template <int V>
+__global__ void __launch_bounds__(32 * kFewWarps)
+few_forward_kernel(const float* __restrict__ x, const float* __restrict__ w,
+                   float* __restrict__ part, const Tile* __restrict__ tiles,
+                   const int* __restrict__ count, int n_i, int n_o, int64_t n_s) {
+  __shared__ __align__(16) float xs[kFewK][kFew];
+  __shared__ float red[kFewWarps][kFew][32 * V];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  after_previous();
+  if ((int)blockIdx.x >= *count) return;
+  const Tile t = tiles[blockIdx.x];
+  const int k0 = blockIdx.z * kFewK, depth = t.expert < 0 ? 0 : min(kFewK, n_i - k0);
+  const int o = (blockIdx.y * 32 + lane) * V;
+  for (int i = threadIdx.x; i < kFew * depth; i += 32 * kFewWarps) {
+    const int r = i / depth, k = i - r * depth;
+    xs[k][r] = r < t.rows ? x[(int64_t)(t.row + r) * n_i + k0 + k] : 0.f;
+  }
+  __syncthreads();
+  float acc[kFew][V] = {};
+  if (o < n_o) {
+    const float* wp = w + ((int64_t)max(t.expert, 0) * n_i + k0) * n_o + o;
+    const int per = (depth + kFewWarps - 1) / kFewWarps, a = warp * per, z = min(depth, a + per);
+    constexpr int U = 8;
+    for (int k = a; k < z; k += U) {
+      Vec<float, V> r[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (k + u < z) r[u] = *reinterpret_cast<const Vec<float, V>*>(wp + (int64_t)(k + u) * n_o);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (k + u < z)
+#pragma unroll
+          for (int q = 0; q < kFew; ++q)
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[q][v] = fmaf(xs[k + u][q], r[u].v[v], acc[q][v]);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < kFew; ++q)
+#pragma unroll
+    for (int v = 0; v < V; ++v) red[warp][q][v * 32 + lane] = acc[q][v];
+  __syncthreads();
+  // warp q adds up row q
+  if (warp < t.rows && o < n_o) {
+    float* out = part + ((int64_t)blockIdx.z * n_s + t.row + warp) * n_o + o;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < kFewWarps; ++j) s += red[j][warp][v * 32 + lane];
+      out[v] = s;
+    }
+  }
+}
+// y = the slices' sums, in order
+__global__ void __launch_bounds__(256)
+few_join_kernel(const float* __restrict__ part, float* __restrict__ y, int64_t n, int slices) {
+  after_previous();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) y[i] = ordered_sum(part + i, slices, n);
+}
+
+// xb (+)= yb W^T: a warp takes four rows of W, its lanes V columns each; four
+// times kFew sums met by halving, one a lane.
+template <int V>
+__global__ void __launch_bounds__(32 * kFewWarps)
+few_input_kernel(const float* __restrict__ yb, const float* __restrict__ w, float* __restrict__ xb,
+                 const Tile* __restrict__ tiles, const int* __restrict__ count, int n_i, int n_o,
+                 bool add) {
+  constexpr int kCols = 1024;
+  __shared__ __align__(16) float ys[kFew][kCols];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  after_previous();
+  if ((int)blockIdx.x >= *count) return;
+  const Tile t = tiles[blockIdx.x];
+  const int i0 = (blockIdx.y * kFewWarps + warp) * 4;
+  float acc[32] = {};            // [row of W][row of the tile]
+  const float* wp = w + (int64_t)max(t.expert, 0) * n_i * n_o;
+  for (int c0 = 0; c0 < (t.expert < 0 ? 0 : n_o); c0 += kCols) {
+    const int cols = min(kCols, n_o - c0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kFew * cols; i += 32 * kFewWarps) {
+      const int r = i / cols, c = i - r * cols;
+      ys[r][c] = r < t.rows ? yb[(int64_t)(t.row + r) * n_o + c0 + c] : 0.f;
+    }
+    __syncthreads();
+#pragma unroll 2
+    for (int c = lane * V; c < cols; c += 32 * V) {
+      Vec<float, V> r[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i0 + j < n_i)
+          r[j] = *reinterpret_cast<const Vec<float, V>*>(wp + (int64_t)(i0 + j) * n_o + c0 + c);
+#pragma unroll
+      for (int q = 0; q < kFew; ++q) {
+        const Vec<float, V> g = *reinterpret_cast<const Vec<float, V>*>(&ys[q][c]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i0 + j < n_i)
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+              acc[j * kFew + q] = fmaf(g.v[v], r[j].v[v], acc[j * kFew + q]);
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 16; n > 0; n >>= 1) {
+    const bool up = lane & n;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float send = up ? acc[i] : acc[i + n], keep = up ? acc[i + n] : acc[i];
+      acc[i] = keep + __shfl_xor_sync(0xffffffffu, send, n);
+    }
+  }
+  const int i = i0 + lane / kFew, q = lane % kFew;       // lane l has sum l
+  if (i < n_i && q < t.rows) {
+    float* o = xb + (int64_t)(t.row + q) * n_i + i;
+    *o = add ? *o + acc[0] : acc[0];
+  }
+}
+
+// Whether the rows are few enough: no more than kFew a group on average.
+bool few_rows(int dtype, int64_t n_s, int64_t n_e, int64_t n_i, int64_t n_o) {
+  return dtype == STADE_F32 && n_s <= kFew * n_e && std::max(n_i, n_o) < (int64_t(1) << 20);
+}
+int64_t few_slices(int64_t n_i) { return (n_i + kFewK - 1) / kFewK; }
+
 int64_t max_tiles(int64_t n_s, int64_t n_e, int tile) { return n_s / tile + n_e + 2; }
 
 // Which path a call takes. The tensor cores read 16-bit operands whose rows
@@ -194,6 +336,7 @@ struct Plan {
   Tile* tiles;
   int* count;
   uint16_t *x, *w, *yb;      // packed planes, where needed
+  float* part;               // few rows: the depth slices' sums
 };
 // S: Sizer or Carver
 template <class S>
@@ -205,12 +348,14 @@ Plan layout(S& z, int dtype, int64_t n_s, int64_t n_e, int64_t n_i, int64_t n_o,
     else *to = z.template take<E>(n);
   };
   take(&p.bounds, n_e + 1);
-  take(&p.tiles, max_tiles(n_s, n_e, kTile));
+  const bool few = few_rows(dtype, n_s, n_e, n_i, n_o);
+  take(&p.tiles, max_tiles(n_s, n_e, few ? kFew : kTile));
   take(&p.count, 1);
+  if (few && !reverse && few_slices(n_i) > 1) take(&p.part, few_slices(n_i) * n_s * n_o);
   if (dtype != STADE_F64 && packs(dtype, n_i, n_o)) {
     const int64_t np = expert_planes(dtype);
-    take(&p.x, np * n_s * pitch8(n_i));
-    take(&p.w, np * n_e * n_i * pitch8(n_o));
+    if (!few || reverse) take(&p.x, np * n_s * pitch8(n_i));
+    if (!few) take(&p.w, np * n_e * n_i * pitch8(n_o));
     if (reverse) take(&p.yb, np * n_s * pitch8(n_o));
   }
   return p;
@@ -291,9 +436,21 @@ extern "C" stade_status stade_expert_mm(int dtype, const void* x, const void* w,
   PhaseScope ph("expert_mm", s);
   Carver c(ws);
   const Plan p = layout(c, dtype, n_s, n_e, n_i, n_o, false);
-  const bool tc = on_tensor_cores(dtype, n_i, n_o, {x, w});
-  st = make_plan(p, off, n_s, n_e, tc ? kExpertTcRows : kTile, s);
+  const bool few = few_rows(dtype, n_s, n_e, n_i, n_o);
+  const bool tc = !few && on_tensor_cores(dtype, n_i, n_o, {x, w});
+  st = make_plan(p, off, n_s, n_e, few ? kFew : tc ? kExpertTcRows : kTile, s);
   if (st != STADE_OK) return st;
+  if (few) {
+    const bool vec = row_align(n_o * 4, {w}) == 16;
+    const int slices = (int)few_slices(n_i);
+    const dim3 grid((unsigned)max_tiles(n_s, n_e, kFew), ceil_div_u(n_o, vec ? 128 : 32), slices);
+    st = launch_next(vec ? few_forward_kernel<4> : few_forward_kernel<1>, grid, 32 * kFewWarps, 0, s,
+                     (const float*)x, (const float*)w, slices > 1 ? p.part : (float*)y, p.tiles,
+                     p.count, (int)n_i, (int)n_o, n_s);
+    if (st != STADE_OK || slices == 1) return st;
+    return launch_next(few_join_kernel, ceil_div_u(n_s * n_o, 256), 256, 0, s, p.part, (float*)y,
+                       n_s * n_o, slices);
+  }
   if (tc) {
     ExpertOperand xo, wo;
     st = operand(dtype, x, p.x, n_i, n_s, 1, &xo, s);
@@ -342,13 +499,21 @@ extern "C" stade_status stade_expert_mm_b(int dtype, const void* x, void* xb, co
   PhaseScope ph("expert_mm_b", s);
   Carver c(ws);
   const Plan p = layout(c, dtype, n_s, n_e, n_i, n_o, true);
+  const bool few = few_rows(dtype, n_s, n_e, n_i, n_o);
   const bool tc = on_tensor_cores(dtype, n_i, n_o, {wb ? x : yb, xb ? w : yb, yb});
-  st = make_plan(p, off, n_s, n_e, tc ? kExpertTcRows : kTile, s);
+  st = make_plan(p, off, n_s, n_e, few ? kFew : tc ? kExpertTcRows : kTile, s);
   if (st != STADE_OK) return st;
   if (tc) {
     ExpertOperand xo, wo, yo;
-    st = operand(dtype, yb, p.yb, n_o, n_s, 1, &yo, s);
-    if (st == STADE_OK && xb) {
+    if (few && xb) {
+      const bool vec = row_align(n_o * 4, {w}) == 16;
+      const dim3 grid((unsigned)max_tiles(n_s, n_e, kFew), ceil_div_u(n_i, 4 * kFewWarps));
+      st = launch_next(vec ? few_input_kernel<4> : few_input_kernel<1>, grid, 32 * kFewWarps, 0, s,
+                       (const float*)yb, (const float*)w, (float*)xb, p.tiles, p.count, (int)n_i,
+                       (int)n_o, add);
+    }
+    if (st == STADE_OK && (wb || (xb && !few))) st = operand(dtype, yb, p.yb, n_o, n_s, 1, &yo, s);
+    if (st == STADE_OK && xb && !few) {
       st = operand(dtype, w, p.w, n_o, n_i, n_e, &wo, s);
       if (st == STADE_OK)
         st = expert_tc_rows(dtype, yo, wo, xb, p.tiles, p.count,

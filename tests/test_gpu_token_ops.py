@@ -408,7 +408,9 @@ EXPERT_SIZES = [  # off, n_i, n_o
     ([0, 1], 1, 1), ([0, 1], 64, 64), ([0, 0, 3, 3, 8], 16, 24), ([0, 5, 5, 133], 72, 200),
     ([0, 300, 301, 700], 264, 136), ([0, 1, 2, 3, 4, 5, 6, 7, 8], 128, 512), ([0, 0, 0], 32, 32),
     ([0, 130, 260], 33, 47), ([0, 257, 1000], 784, 512), ([0, 64, 128, 640], 520, 264),
-    ([0, 17, 17, 80], 200, 10), ([0, 24], 1024, 8), ([0, 2000], 64, 96), ([0, 31, 500], 40, 1030)]
+    ([0, 17, 17, 80], 200, 10), ([0, 24], 1024, 8), ([0, 2000], 64, 96), ([0, 31, 500], 40, 1030),
+    # few rows a group over wide weights
+    ([0, 3, 3, 9, 10], 1100, 72), ([0, 5], 1500, 33), ([0, 1, 16], 515, 2100), ([0, 8, 16], 2049, 130)]
 
 
 def _expert_case(off, n_i, n_o, dt, shift=0, n_s=None):
@@ -459,9 +461,10 @@ def test_expert_mm_b(off, n_i, n_o, dt):
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("shift", [1, 4])
-def test_expert_mm_unaligned(shift, dt):
+@pytest.mark.parametrize("off", [[0, 70, 200], [0, 3, 11]])
+def test_expert_mm_unaligned(off, shift, dt):
     dt = R.DTYPES[dt]
-    off, n_i, n_o = [0, 70, 200], 72, 136
+    n_i, n_o = 72, 136
     x, w, yb, o, n = _expert_case(off, n_i, n_o, dt, shift)
     y, xb = _dev(torch.zeros(n[0], n_o), dt, shift), _dev(torch.zeros(n[0], n_i), dt, shift)
     wb = _dev(torch.zeros(2, n_i, n_o), R.par(dt), shift)
