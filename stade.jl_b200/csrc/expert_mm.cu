@@ -250,68 +250,108 @@ few_join_kernel(const float* __restrict__ part, float* __restrict__ y, int64_t n
   if (i < n) y[i] = ordered_sum(part + i, slices, n);
 }
 
-// xb (+)= yb W^T: a warp takes four rows of W, its lanes V columns each; four
-// times kFew sums met by halving, one a lane.
+// xb (+)= yb W^T: a block takes eight rows of W, its warps every eighth stretch
+// of 32 V columns; the 64 sums of a warp are halved down to two a lane, and the
+// warps' added in order.
 template <int V>
 __global__ void __launch_bounds__(32 * kFewWarps)
 few_input_kernel(const float* __restrict__ yb, const float* __restrict__ w, float* __restrict__ xb,
                  const Tile* __restrict__ tiles, const int* __restrict__ count, int n_i, int n_o,
                  bool add) {
-  constexpr int kCols = 1024;
-  __shared__ __align__(16) float ys[kFew][kCols];
+  constexpr int kRows = 8;
+  __shared__ float red[kFewWarps][kRows * kFew];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   after_previous();
   if ((int)blockIdx.x >= *count) return;
   const Tile t = tiles[blockIdx.x];
-  const int i0 = (blockIdx.y * kFewWarps + warp) * 4;
-  float acc[32] = {};            // [row of W][row of the tile]
-  const float* wp = w + (int64_t)max(t.expert, 0) * n_i * n_o;
-  for (int c0 = 0; c0 < (t.expert < 0 ? 0 : n_o); c0 += kCols) {
-    const int cols = min(kCols, n_o - c0);
-    __syncthreads();
-    for (int i = threadIdx.x; i < kFew * cols; i += 32 * kFewWarps) {
-      const int r = i / cols, c = i - r * cols;
-      ys[r][c] = r < t.rows ? yb[(int64_t)(t.row + r) * n_o + c0 + c] : 0.f;
-    }
-    __syncthreads();
-#pragma unroll 2
-    for (int c = lane * V; c < cols; c += 32 * V) {
-      Vec<float, V> r[4];
+  const int i0 = blockIdx.y * kRows;
+  float acc[kRows * kFew] = {};            // [row of W][row of the tile]
+  const float* wp = w + ((int64_t)max(t.expert, 0) * n_i + i0) * n_o;
+  const float* yp = yb + (int64_t)t.row * n_o;
+  for (int c = (warp * 32 + lane) * V; c < (t.expert < 0 ? 0 : n_o); c += kFewWarps * 32 * V) {
+    Vec<float, V> r[kRows];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i0 + j < n_i)
-          r[j] = *reinterpret_cast<const Vec<float, V>*>(wp + (int64_t)(i0 + j) * n_o + c0 + c);
+    for (int j = 0; j < kRows; ++j)
+      if (i0 + j < n_i) r[j] = *reinterpret_cast<const Vec<float, V>*>(wp + (int64_t)j * n_o + c);
 #pragma unroll
-      for (int q = 0; q < kFew; ++q) {
-        const Vec<float, V> g = *reinterpret_cast<const Vec<float, V>*>(&ys[q][c]);
+    for (int q = 0; q < kFew; ++q)
+      if (q < t.rows) {
+        const Vec<float, V> g = *reinterpret_cast<const Vec<float, V>*>(yp + (int64_t)q * n_o + c);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < kRows; ++j)
           if (i0 + j < n_i)
 #pragma unroll
             for (int v = 0; v < V; ++v)
               acc[j * kFew + q] = fmaf(g.v[v], r[j].v[v], acc[j * kFew + q]);
       }
-    }
   }
 #pragma unroll
-  for (int n = 16; n > 0; n >>= 1) {
-    const bool up = lane & n;
+  for (int n = 32; n > 1; n >>= 1) {
+    const bool up = lane & (n / 2);
 #pragma unroll
     for (int i = 0; i < n; ++i) {
       const float send = up ? acc[i] : acc[i + n], keep = up ? acc[i + n] : acc[i];
-      acc[i] = keep + __shfl_xor_sync(0xffffffffu, send, n);
+      acc[i] = keep + __shfl_xor_sync(0xffffffffu, send, n / 2);
     }
   }
-  const int i = i0 + lane / kFew, q = lane % kFew;       // lane l has sum l
-  if (i < n_i && q < t.rows) {
+  red[warp][2 * lane] = acc[0];        // lane l has sums 2 l and 2 l + 1
+  red[warp][2 * lane + 1] = acc[1];
+  __syncthreads();
+  const int i = i0 + (int)threadIdx.x / kFew, q = threadIdx.x % kFew;
+  if (threadIdx.x < kRows * kFew && i < n_i && q < t.rows) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < kFewWarps; ++j) s += red[j][threadIdx.x];
     float* o = xb + (int64_t)(t.row + q) * n_i + i;
-    *o = add ? *o + acc[0] : acc[0];
+    *o = add ? *o + s : s;
   }
+}
+
+// wb[e] (+)= sum over the group's rows of x^T yb: one write of the gradient. A
+// warp takes four rows and 32 V columns of it and walks the group's rows.
+template <int V>
+__global__ void __launch_bounds__(32 * kFewWarps)
+few_weight_kernel(const float* __restrict__ x, const float* __restrict__ yb, float* __restrict__ wb,
+                  const int64_t* __restrict__ bounds, int n_i, int n_o, bool add) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  after_previous();
+  const int64_t e = blockIdx.z, a = bounds[e], z = bounds[e + 1];
+  const int i0 = (blockIdx.y * kFewWarps + warp) * 4, o = (blockIdx.x * 32 + lane) * V;
+  if (i0 >= n_i || o >= n_o || (add && a == z)) return;
+  float acc[4][V] = {};
+  for (int64_t s = a; s < z; s += 4) {
+    Vec<float, V> g[4];
+    float f[4][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool in = s + u < z;
+      if (in) g[u] = *reinterpret_cast<const Vec<float, V>*>(yb + (s + u) * n_o + o);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[u][j] = in && i0 + j < n_i ? x[(s + u) * n_i + i0 + j] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (s + u < z)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int v = 0; v < V; ++v) acc[j][v] = fmaf(f[u][j], g[u].v[v], acc[j][v]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (i0 + j < n_i) {
+      float* p = wb + (e * n_i + i0 + j) * n_o + o;
+      Vec<float, V> r;
+      if (add) r = *reinterpret_cast<const Vec<float, V>*>(p);
+#pragma unroll
+      for (int v = 0; v < V; ++v) r.v[v] = add ? r.v[v] + acc[j][v] : acc[j][v];
+      *reinterpret_cast<Vec<float, V>*>(p) = r;
+    }
 }
 
 // Whether the rows are few enough: no more than kFew a group on average.
 bool few_rows(int dtype, int64_t n_s, int64_t n_e, int64_t n_i, int64_t n_o) {
-  return dtype == STADE_F32 && n_s <= kFew * n_e && std::max(n_i, n_o) < (int64_t(1) << 20);
+  return dtype == STADE_F32 && n_s <= kFew * n_e && std::max(n_i, n_o) < (int64_t(1) << 18);
 }
 int64_t few_slices(int64_t n_i) { return (n_i + kFewK - 1) / kFewK; }
 
@@ -352,10 +392,10 @@ Plan layout(S& z, int dtype, int64_t n_s, int64_t n_e, int64_t n_i, int64_t n_o,
   take(&p.tiles, max_tiles(n_s, n_e, few ? kFew : kTile));
   take(&p.count, 1);
   if (few && !reverse && few_slices(n_i) > 1) take(&p.part, few_slices(n_i) * n_s * n_o);
-  if (dtype != STADE_F64 && packs(dtype, n_i, n_o)) {
+  if (!few && dtype != STADE_F64 && packs(dtype, n_i, n_o)) {
     const int64_t np = expert_planes(dtype);
-    if (!few || reverse) take(&p.x, np * n_s * pitch8(n_i));
-    if (!few) take(&p.w, np * n_e * n_i * pitch8(n_o));
+    take(&p.x, np * n_s * pitch8(n_i));
+    take(&p.w, np * n_e * n_i * pitch8(n_o));
     if (reverse) take(&p.yb, np * n_s * pitch8(n_o));
   }
   return p;
@@ -500,20 +540,29 @@ extern "C" stade_status stade_expert_mm_b(int dtype, const void* x, void* xb, co
   Carver c(ws);
   const Plan p = layout(c, dtype, n_s, n_e, n_i, n_o, true);
   const bool few = few_rows(dtype, n_s, n_e, n_i, n_o);
-  const bool tc = on_tensor_cores(dtype, n_i, n_o, {wb ? x : yb, xb ? w : yb, yb});
+  const bool tc = !few && on_tensor_cores(dtype, n_i, n_o, {wb ? x : yb, xb ? w : yb, yb});
   st = make_plan(p, off, n_s, n_e, few ? kFew : tc ? kExpertTcRows : kTile, s);
   if (st != STADE_OK) return st;
-  if (tc) {
-    ExpertOperand xo, wo, yo;
-    if (few && xb) {
-      const bool vec = row_align(n_o * 4, {w}) == 16;
-      const dim3 grid((unsigned)max_tiles(n_s, n_e, kFew), ceil_div_u(n_i, 4 * kFewWarps));
+  if (few) {
+    if (xb) {
+      const bool vec = row_align(n_o * 4, {w, yb}) == 16;
+      const dim3 grid((unsigned)max_tiles(n_s, n_e, kFew), ceil_div_u(n_i, 8));
       st = launch_next(vec ? few_input_kernel<4> : few_input_kernel<1>, grid, 32 * kFewWarps, 0, s,
                        (const float*)yb, (const float*)w, (float*)xb, p.tiles, p.count, (int)n_i,
                        (int)n_o, add);
     }
-    if (st == STADE_OK && (wb || (xb && !few))) st = operand(dtype, yb, p.yb, n_o, n_s, 1, &yo, s);
-    if (st == STADE_OK && xb && !few) {
+    if (st == STADE_OK && wb) {
+      const bool vec = row_align(n_o * 4, {yb, wb}) == 16;
+      const dim3 grid(ceil_div_u(n_o, vec ? 128 : 32), ceil_div_u(n_i, 4 * kFewWarps),
+                      (unsigned)n_e);
+      st = launch_next(vec ? few_weight_kernel<4> : few_weight_kernel<1>, grid, 32 * kFewWarps, 0,
+                       s, (const float*)x, (const float*)yb, (float*)wb, p.bounds, (int)n_i,
+                       (int)n_o, add);
+    }
+  } else if (tc) {
+    ExpertOperand xo, wo, yo;
+    st = operand(dtype, yb, p.yb, n_o, n_s, 1, &yo, s);
+    if (st == STADE_OK && xb) {
       st = operand(dtype, w, p.w, n_o, n_i, n_e, &wo, s);
       if (st == STADE_OK)
         st = expert_tc_rows(dtype, yo, wo, xb, p.tiles, p.count,
