@@ -33,23 +33,26 @@ _TYPES = {t: (code, t, torch.float64 if t == torch.float64 else torch.float32)
 
 
 def _dtype(t, name: str):
-    """(dtype code, element type, parameter type) by an activation array."""
+    """(dtype code, element type, parameter type, current device) by an
+    activation array."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a CUDA tensor, got {type(t).__name__}")
     types = _TYPES.get(t.dtype)
     if types is None:
         raise TypeError(f"{name}: unsupported dtype {t.dtype}")
-    return types
+    if not t.is_cuda:
+        raise ValueError(f"{name}: tensor must live on a CUDA device")
+    return *types, torch.cuda.current_device()
 
 
-def _arr(t, dtype, n: int, name: str) -> int:
+def _arr(d: int, t, dtype, n: int, name: str) -> int:
     """Address of an array after its checks: CUDA, type, contiguity, length,
-    and the current device, on which the call runs."""
-    p = kernels._arr(t, dtype, n, name)
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{name}: tensor lives on {t.device}, the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
-    return p
+    and the current device d, on which the call runs."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_contiguous() and t.numel() >= n
+            and t.get_device() == d):
+        return t.data_ptr()
+    kernels._arr(t, dtype, n, name)
+    raise ValueError(f"{name}: tensor lives on {t.device}, the current device is cuda:{d}")
 
 
 # The current stream's handle without building a Stream object, which costs as
@@ -74,8 +77,8 @@ def _run(fn, *args, stream=None, workspace=None, flags=0) -> None:
         check(code)
 
 
-def _opt(t, dtype, n, name):
-    return None if t is None else _arr(t, dtype, n, name)
+def _opt(d, t, dtype, n, name):
+    return None if t is None else _arr(d, t, dtype, n, name)
 
 
 def _flags(accumulate: bool, consume: bool) -> int:
@@ -98,9 +101,10 @@ def embed_cuda(w, ids, y, scale, n_s, n_v, n_d, *, base=0, stream=None):
     """y[s] = scale w[ids[s] - base]; ids below base are padding (zero rows).
     ids: int64. Gathers rows of any n_v x n_d array by an index list."""
     _sizes(n_s, n_v, n_d)
-    code, T, _ = _dtype(y, "y")
-    _run(lib().stade_embed, code, _arr(w, T, n_v * n_d, "w"), _arr(ids, torch.int64, n_s, "ids"),
-         _arr(y, T, n_s * n_d, "y"), float(scale), base, n_s, n_v, n_d, stream=stream)
+    code, T, _, d = _dtype(y, "y")
+    _run(lib().stade_embed, code, _arr(d, w, T, n_v * n_d, "w"),
+         _arr(d, ids, torch.int64, n_s, "ids"), _arr(d, y, T, n_s * n_d, "y"), float(scale), base,
+         n_s, n_v, n_d, stream=stream)
 
 
 def embed_b_cuda(wb, ids, yb, scale, n_s, n_v, n_d, *, base=0, accumulate=True, consume=True,
@@ -108,10 +112,11 @@ def embed_b_cuda(wb, ids, yb, scale, n_s, n_v, n_d, *, base=0, accumulate=True, 
     """wb[v] += scale * sum of yb[s] over the positions s that hold id v, in
     increasing s (bit-identical from call to call)."""
     _sizes(n_s, n_v, n_d)
-    code, T, P = _dtype(yb, "yb")
-    _run(lib().stade_embed_b, code, _arr(wb, P, n_v * n_d, "wb"),
-         _arr(ids, torch.int64, n_s, "ids"), _arr(yb, T, n_s * n_d, "yb"), float(scale), base, n_s,
-         n_v, n_d, stream=stream, workspace=workspace, flags=_flags(accumulate, consume))
+    code, T, P, d = _dtype(yb, "yb")
+    _run(lib().stade_embed_b, code, _arr(d, wb, P, n_v * n_d, "wb"),
+         _arr(d, ids, torch.int64, n_s, "ids"), _arr(d, yb, T, n_s * n_d, "yb"), float(scale),
+         base, n_s, n_v, n_d, stream=stream, workspace=workspace,
+         flags=_flags(accumulate, consume))
 
 
 def embed_b_workspace(n_s, n_v, n_d) -> int:
@@ -123,10 +128,11 @@ def layer_norm_cuda(x, w, b, y, m_stack, r_stack, eps, n_s, n_d, *, stream=None)
     """y = (x - mean) rstd w + b over rows of n_d; w and b may be None. The
     tape m_stack, r_stack (n_s each) receives mean and rstd."""
     _sizes(n_s, n_d)
-    code, T, P = _dtype(x, "x")
-    _run(lib().stade_layer_norm, code, _arr(x, T, n_s * n_d, "x"), _opt(w, P, n_d, "w"),
-         _opt(b, P, n_d, "b"), _arr(y, T, n_s * n_d, "y"), _arr(m_stack, P, n_s, "m_stack"),
-         _arr(r_stack, P, n_s, "r_stack"), float(eps), n_s, n_d, stream=stream)
+    code, T, P, d = _dtype(x, "x")
+    _run(lib().stade_layer_norm, code, _arr(d, x, T, n_s * n_d, "x"), _opt(d, w, P, n_d, "w"),
+         _opt(d, b, P, n_d, "b"), _arr(d, y, T, n_s * n_d, "y"),
+         _arr(d, m_stack, P, n_s, "m_stack"), _arr(d, r_stack, P, n_s, "r_stack"), float(eps), n_s,
+         n_d, stream=stream)
 
 
 def layer_norm_b_cuda(x, xb, w, wb, bb, yb, m_stack, r_stack, n_s, n_d, *, accumulate=True,
@@ -134,12 +140,12 @@ def layer_norm_b_cuda(x, xb, w, wb, bb, yb, m_stack, r_stack, n_s, n_d, *, accum
     """Reverse sweep of layer_norm from x and the tape; xb, wb and bb may be
     None (not wanted)."""
     _sizes(n_s, n_d)
-    code, T, P = _dtype(x, "x")
-    _run(lib().stade_layer_norm_b, code, _arr(x, T, n_s * n_d, "x"), _opt(xb, T, n_s * n_d, "xb"),
-         _opt(w, P, n_d, "w"), _opt(wb, P, n_d, "wb"), _opt(bb, P, n_d, "bb"),
-         _arr(yb, T, n_s * n_d, "yb"), _arr(m_stack, P, n_s, "m_stack"),
-         _arr(r_stack, P, n_s, "r_stack"), n_s, n_d, stream=stream, workspace=workspace,
-         flags=_flags(accumulate, consume))
+    code, T, P, d = _dtype(x, "x")
+    _run(lib().stade_layer_norm_b, code, _arr(d, x, T, n_s * n_d, "x"),
+         _opt(d, xb, T, n_s * n_d, "xb"), _opt(d, w, P, n_d, "w"), _opt(d, wb, P, n_d, "wb"),
+         _opt(d, bb, P, n_d, "bb"), _arr(d, yb, T, n_s * n_d, "yb"),
+         _arr(d, m_stack, P, n_s, "m_stack"), _arr(d, r_stack, P, n_s, "r_stack"), n_s, n_d,
+         stream=stream, workspace=workspace, flags=_flags(accumulate, consume))
 
 
 def layer_norm_b_workspace(dtype, n_s, n_d) -> int:
@@ -156,44 +162,45 @@ def initstacks_tape8_cuda(n_s, n_d, device=None):
     return q, e
 
 
-def _tape(q, e, n_s, n_d):
-    return (_arr(q, torch.int8, n_s * n_d, "q_stack"),
-            _arr(e, torch.uint8, lib().stade_initstacks_tape8(n_s, n_d), "e_stack"))
+def _tape(d, q, e, n_s, n_d):
+    return (_arr(d, q, torch.int8, n_s * n_d, "q_stack"),
+            _arr(d, e, torch.uint8, lib().stade_initstacks_tape8(n_s, n_d), "e_stack"))
 
 
 def tape8_push_cuda(x, q_stack, e_stack, n_s, n_d, *, stream=None):
     """Writes x to the 8-bit tape."""
     _sizes(n_s, n_d)
-    code, T, _ = _dtype(x, "x")
-    _run(lib().stade_tape8_push, code, _arr(x, T, n_s * n_d, "x"),
-         *_tape(q_stack, e_stack, n_s, n_d), n_s, n_d, stream=stream)
+    code, T, _, d = _dtype(x, "x")
+    _run(lib().stade_tape8_push, code, _arr(d, x, T, n_s * n_d, "x"),
+         *_tape(d, q_stack, e_stack, n_s, n_d), n_s, n_d, stream=stream)
 
 
 def tape8_pop_cuda(x, q_stack, e_stack, n_s, n_d, *, stream=None):
     """Restores x from the 8-bit tape (overwrites x)."""
     _sizes(n_s, n_d)
-    code, T, _ = _dtype(x, "x")
-    _run(lib().stade_tape8_pop, code, _arr(x, T, n_s * n_d, "x"),
-         *_tape(q_stack, e_stack, n_s, n_d), n_s, n_d, stream=stream)
+    code, T, _, d = _dtype(x, "x")
+    _run(lib().stade_tape8_pop, code, _arr(d, x, T, n_s * n_d, "x"),
+         *_tape(d, q_stack, e_stack, n_s, n_d), n_s, n_d, stream=stream)
 
 
 def act_tape8_cuda(act, x, y, q_stack, e_stack, n_s, n_d, *, stream=None):
     """y = f(x), f one of relu, tanh, silu, gelu (erf form); x goes to the
     8-bit tape for act_tape8_b."""
     _sizes(n_s, n_d)
-    code, T, _ = _dtype(x, "x")
-    _run(lib().stade_act_tape8, code, _act(act), _arr(x, T, n_s * n_d, "x"),
-         _arr(y, T, n_s * n_d, "y"), *_tape(q_stack, e_stack, n_s, n_d), n_s, n_d, stream=stream)
+    code, T, _, d = _dtype(x, "x")
+    _run(lib().stade_act_tape8, code, _act(act), _arr(d, x, T, n_s * n_d, "x"),
+         _arr(d, y, T, n_s * n_d, "y"), *_tape(d, q_stack, e_stack, n_s, n_d), n_s, n_d,
+         stream=stream)
 
 
 def act_tape8_b_cuda(act, xb, yb, q_stack, e_stack, n_s, n_d, *, accumulate=True, consume=True,
                      stream=None):
     """xb += yb f'(x^), x^ the input as the 8-bit tape holds it."""
     _sizes(n_s, n_d)
-    code, T, _ = _dtype(yb, "yb")
-    _run(lib().stade_act_tape8_b, code, _act(act), _arr(xb, T, n_s * n_d, "xb"),
-         _arr(yb, T, n_s * n_d, "yb"), *_tape(q_stack, e_stack, n_s, n_d), n_s, n_d, stream=stream,
-         flags=_flags(accumulate, consume))
+    code, T, _, d = _dtype(yb, "yb")
+    _run(lib().stade_act_tape8_b, code, _act(act), _arr(d, xb, T, n_s * n_d, "xb"),
+         _arr(d, yb, T, n_s * n_d, "yb"), *_tape(d, q_stack, e_stack, n_s, n_d), n_s, n_d,
+         stream=stream, flags=_flags(accumulate, consume))
 
 
 # ---------------------------------------------------------------------------
@@ -202,10 +209,11 @@ def expert_mm_cuda(x, w, y, off, n_s, n_e, n_i, n_o, *, stream=None, workspace=N
     n_e x n_i x n_o, off: n_e + 1 rising bounds (int64, on the device). Rows in
     no group get y = 0."""
     _sizes(n_s, n_e, n_i, n_o)
-    code, T, _ = _dtype(x, "x")
-    _run(lib().stade_expert_mm, code, _arr(x, T, n_s * n_i, "x"), _arr(w, T, n_e * n_i * n_o, "w"),
-         _arr(y, T, n_s * n_o, "y"), _arr(off, torch.int64, n_e + 1, "off"), n_s, n_e, n_i, n_o,
-         stream=stream, workspace=workspace)
+    code, T, _, d = _dtype(x, "x")
+    _run(lib().stade_expert_mm, code, _arr(d, x, T, n_s * n_i, "x"),
+         _arr(d, w, T, n_e * n_i * n_o, "w"), _arr(d, y, T, n_s * n_o, "y"),
+         _arr(d, off, torch.int64, n_e + 1, "off"), n_s, n_e, n_i, n_o, stream=stream,
+         workspace=workspace)
 
 
 def expert_mm_workspace(dtype, n_s, n_e, n_i, n_o) -> int:
@@ -217,11 +225,12 @@ def expert_mm_b_cuda(x, xb, w, wb, yb, off, n_s, n_e, n_i, n_o, *, accumulate=Tr
     """xb[s] += yb[s] w[e]^T and wb[e] += x^T yb over the rows of expert e; xb
     or wb may be None (not wanted)."""
     _sizes(n_s, n_e, n_i, n_o)
-    code, T, P = _dtype(yb, "yb")
-    _run(lib().stade_expert_mm_b, code, _opt(x, T, n_s * n_i, "x"), _opt(xb, T, n_s * n_i, "xb"),
-         _opt(w, T, n_e * n_i * n_o, "w"), _opt(wb, P, n_e * n_i * n_o, "wb"),
-         _arr(yb, T, n_s * n_o, "yb"), _arr(off, torch.int64, n_e + 1, "off"), n_s, n_e, n_i, n_o,
-         stream=stream, workspace=workspace, flags=_flags(accumulate, consume))
+    code, T, P, d = _dtype(yb, "yb")
+    _run(lib().stade_expert_mm_b, code, _opt(d, x, T, n_s * n_i, "x"),
+         _opt(d, xb, T, n_s * n_i, "xb"), _opt(d, w, T, n_e * n_i * n_o, "w"),
+         _opt(d, wb, P, n_e * n_i * n_o, "wb"), _arr(d, yb, T, n_s * n_o, "yb"),
+         _arr(d, off, torch.int64, n_e + 1, "off"), n_s, n_e, n_i, n_o, stream=stream,
+         workspace=workspace, flags=_flags(accumulate, consume))
 
 
 def expert_mm_b_workspace(dtype, n_s, n_e, n_i, n_o) -> int:
