@@ -894,9 +894,12 @@ stade_status with_row_warps(int64_t n_d, int align, F&& f) {
 // Ring kernels: a block of `threads` threads a row (m vectors each), `rows` rows
 // a turn, `stages` turns in flight, as many blocks an SM as registers and 200
 // KB of shared memory allow.
-//  - Forward: one vector a thread and several rows a turn, 1,024 threads an SM
-//    at 64 registers; two vectors where a row would take 513 to 672 threads and
-//    leave the SM a third empty (8192 x 5000 f16: 49.6 -> 41.9 us).
+//  - Forward: rows of up to 256 vectors one a thread and up to four rows a turn,
+//    1,024 threads an SM at 64 registers; longer ones two vectors a thread and
+//    two rows a turn, 640 threads at 96 (16384 x 4096 bf16: 49.6 us against 55.8
+//    with one vector; 16384 x 2048: 34.9 against 31.0). Two blocks of 257 to 384
+//    threads with whole vectors do better a row a turn (8192 x 5000 f16: 43.8
+//    against 46.3 us; single columns, 8192 x 4999: 76 against 64).
 //  - Reverse: the row's h and g w stay in registers, 512 threads at 128, so two
 //    vectors a thread and two or more blocks an SM rather than several rows a
 //    turn, which left one block and its barriers alone on the SM (16384 x 4096
@@ -910,14 +913,16 @@ struct RingPlan {
 bool ring_plan(int64_t n_s, int64_t row_bytes, bool rev, bool wide, RingPlan* p) {
   const int64_t slots = (row_bytes + 15) / 16;   // a thread owns 16 bytes of a row, or 32
   if (slots < 96 || slots > 2 * 768) return false;
-  p->m = rev ? (wide || slots > 512 ? 2 : 1) : slots <= 512 || (slots > 672 && slots <= 1024) ? 1 : 2;
+  p->m = rev ? (wide || slots > 512 ? 2 : 1) : slots <= 256 ? 1 : 2;
   p->threads = (int)(((slots + p->m - 1) / p->m + 31) / 32 * 32);
-  const int per_sm = std::max(1, (rev ? 512 : p->m == 2 ? 768 : 1024) / p->threads);
+  const int per_sm = std::max(1, (rev ? 512 : p->m == 2 ? 640 : 1024) / p->threads);
   const int arrays = rev ? 2 : 1;
   const int64_t room = 200 * 1024 / (per_sm * row_bytes * arrays);   // rows in flight a block
   // several rows a turn where every block still gets two turns
-  p->rows = p->m > 1 || n_s < 4 * 148 * per_sm || room < 4 ? 1
-            : !rev && p->threads <= 512 && room >= 8 && n_s >= 8 * 148 * per_sm ? 4 : 2;
+  const bool two_blocks = wide && p->threads > 256 && p->threads <= 384;
+  const bool one = n_s < 4 * 148 * per_sm || room < 4 ||
+                   (p->m > 1 && (rev || p->threads > 512 || two_blocks));
+  p->rows = one ? 1 : p->m == 1 && !rev && room >= 8 && n_s >= 8 * 148 * per_sm ? 4 : 2;
   p->stages = (int)std::min<int64_t>(kMaxStages, std::max<int64_t>(2, room / p->rows));
   p->smem = 128 + p->stages * arrays * ((p->rows * row_bytes + 31) & ~int64_t(15));
   p->blocks = (int)std::min<int64_t>((n_s + p->rows - 1) / p->rows, 148 * per_sm);
@@ -946,12 +951,12 @@ stade_status fwd(const void* x, const void* w, const void* b, void* y, void* m, 
   if (row_align(16, {x}) == 16 && ring_plan(n_s, row_bytes, false, align == 16, &rp)) {
     return with_width<T>(align, [&](auto vw) {
       constexpr int VW = decltype(vw)::value;
-      auto kern = rp.m == 2 ? ln_fwd_ring_kernel<T, 2 * V, VW, 1, 768, 1>
-                  : rp.threads > 512 ? (rp.rows == 2 ? ln_fwd_ring_kernel<T, V, VW, 2, 1024, 1>
-                                                     : ln_fwd_ring_kernel<T, V, VW, 1, 1024, 1>)
-                  : rp.rows == 4 ? ln_fwd_ring_kernel<T, V, VW, 4, 512, 2>
-                  : rp.rows == 2 ? ln_fwd_ring_kernel<T, V, VW, 2, 512, 2>
-                                 : ln_fwd_ring_kernel<T, V, VW, 1, 512, 2>;
+      auto kern = rp.threads > 512 ? ln_fwd_ring_kernel<T, 2 * V, VW, 1, 768, 1>
+                  : rp.m == 2 ? (rp.rows == 2 ? ln_fwd_ring_kernel<T, 2 * V, VW, 2, 512, 1>
+                                              : ln_fwd_ring_kernel<T, 2 * V, VW, 1, 512, 1>)
+                  : rp.rows == 4 ? ln_fwd_ring_kernel<T, V, VW, 4, 256, 4>
+                  : rp.rows == 2 ? ln_fwd_ring_kernel<T, V, VW, 2, 256, 4>
+                                 : ln_fwd_ring_kernel<T, V, VW, 1, 256, 4>;
       STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)rp.smem));
       kern<<<rp.blocks, rp.threads, rp.smem, st>>>((const T*)x, (const A*)w, (const A*)b, (T*)y,
@@ -1004,8 +1009,8 @@ stade_status bwd(const void* x, void* xb, const void* w, void* wb, void* bb, voi
     const BwdArgs p{x, w, m, r, xb, yb, ws, n_s, (int)n_d, add, zero, sums};
     e = with_width<T>(align, [&](auto vw) {
       constexpr int VW = decltype(vw)::value;
-      void (*kern)(BwdArgs, int) = rp.threads > 512 ? ln_bwd_ring_kernel<T, 2 * V, VW, 1, 768, false>
-                                                   : ln_bwd_ring_kernel<T, 2 * V, VW, 1, 512, true>;
+      void (*kern)(BwdArgs, int) = ln_bwd_ring_kernel<T, 2 * V, VW, 1, 512, true>;
+      if (rp.threads > 512) kern = ln_bwd_ring_kernel<T, 2 * V, VW, 1, 768, false>;
       if constexpr (VW != V)
         if (rp.m == 1)
           kern = rp.rows == 2 ? ln_bwd_ring_kernel<T, V, VW, 2, 512, true>
