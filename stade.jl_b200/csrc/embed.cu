@@ -13,10 +13,11 @@
 //
 // The lookup is bound by memory: 32768 rows of 1024 bf16 in 20.6 us, 0.99 of the
 // measured copy rate by the bytes moved. The gradient of the same rows into a
-// table of 50021 (205 MB of Float32) takes 85 us, 41 by its bytes: the sort's
-// three launches (14 to 20 us each under the profiler, with a third of the
-// clearing in each), the sums (21 us) and the parts' join (11 us) wait for one
-// another.
+// table of 50021 (205 MB of Float32) takes 65 us, 41 by its bytes: the sort, with
+// the clearing beside it (34 us under the profiler), the sums (21 us) and the
+// parts' join (11 us) wait for one another.
+
+#include <cooperative_groups.h>
 
 #include <algorithm>
 #include <initializer_list>
@@ -121,7 +122,11 @@ __device__ __forceinline__ bool fill_block(const Fill& f, int first) {
   const int64_t n = f.bytes / 16, a = n * f.part / f.parts, z = n * (f.part + 1) / f.parts;
   const int64_t step = (int64_t)(gridDim.x - first) * blockDim.x;
   const int64_t t = (int64_t)(blockIdx.x - first) * blockDim.x + threadIdx.x;
-  for (int64_t i = a + t; i < z; i += step) f.p[i] = make_int4(0, 0, 0, 0);
+  int64_t i = a + t;
+  for (; i + 3 * step < z; i += 4 * step)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) f.p[i + u * step] = make_int4(0, 0, 0, 0);
+  for (; i < z; i += step) f.p[i] = make_int4(0, 0, 0, 0);
   if (f.part == 0 && t < f.bytes % 16) reinterpret_cast<char*>(f.p + n)[t] = 0;
   return true;
 }
@@ -342,6 +347,117 @@ small_sort_kernel(SortIn in, int n, int passes, int bits, uint32_t* __restrict__
   for (int i = threadIdx.x; i < n; i += kSmallThreads) {
     keys_out[i] = keys[i];
     pos_out[i] = pos[i];
+  }
+}
+
+// The whole sort for n up to kClusterSort in one cluster of kSortCtas blocks (the
+// other clusters clear): each block holds its share of the keys in shared
+// memory, a pass adds the blocks' digit counts up over distributed shared
+// memory and stores every key where it belongs, in whichever block that is.
+// The embedding gradient of 32768 x 1024 bf16 into 50021 rows takes 85 us with
+// three launches for the sort, 65 us so; the sort alone 25 us, with the clearing
+// of 205 MB beside it 34.
+constexpr int kSortCtas = 8;
+constexpr int kSortWarps = 32;
+constexpr int kLaneItems = 8;               // keys a lane holds, at most
+constexpr int kClusterSort = kSortCtas * kSortWarps * 32 * kLaneItems;
+
+__global__ void __launch_bounds__(32 * kSortWarps)
+cluster_sort_kernel(SortIn in, int n, int passes, int bits, int lane_items,
+                    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out, Fill fill) {
+  namespace cg = cooperative_groups;
+  extern __shared__ uint32_t sm[];
+  __shared__ uint32_t total[kMaxBins];
+  __shared__ uint32_t sums[32];
+  before_next();
+  if (fill_block(fill, kSortCtas)) return;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bins = 1 << bits;
+  const int per_warp = 32 * lane_items, share = kSortWarps * per_warp;
+  uint32_t* keys = sm;
+  uint32_t* pos = sm + share;
+  uint32_t* h = sm + 2 * share;               // [kSortWarps][bins]
+  const int mine = warp * per_warp;           // of the block's share
+  const int valid = n - rank * share;         // keys of the block's share that exist
+  uint32_t key[kLaneItems], p[kLaneItems];
+#pragma unroll
+  for (int u = 0; u < kLaneItems; ++u) {
+    const int i = mine + u * 32 + lane;
+    const bool has = u < lane_items && i < valid;
+    key[u] = has ? id_key(in, (int64_t)rank * share + i) : 0xffffffffu;
+    p[u] = rank * share + i;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * bits;
+    for (int b = threadIdx.x; b < kSortWarps * bins; b += 32 * kSortWarps) h[b] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kLaneItems; ++u)
+      if (u < lane_items && mine + u * 32 + lane < valid)
+        atomicAdd(&h[warp * bins + ((key[u] >> shift) & (bins - 1))], 1u);
+    __syncthreads();
+    if ((int)threadIdx.x < bins) {
+      uint32_t t = 0;
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) t += h[w * bins + threadIdx.x];
+      total[threadIdx.x] = t;
+    }
+    cluster.sync();       // every block's counts are there, and its keys in registers
+    uint32_t all = 0, before = 0;
+    if ((int)threadIdx.x < bins) {
+      uint32_t c[kSortCtas];
+#pragma unroll
+      for (int r = 0; r < kSortCtas; ++r) c[r] = *cluster.map_shared_rank(&total[threadIdx.x], r);
+#pragma unroll
+      for (int r = 0; r < kSortCtas; ++r) {
+        all += c[r];
+        if (r < rank) before += c[r];
+      }
+    }
+    uint32_t sum;
+    const uint32_t ahead = block_exclusive(all, sums, &sum);
+    if ((int)threadIdx.x < bins) {
+      uint32_t at = ahead + before;
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = h[w * bins + threadIdx.x];
+        h[w * bins + threadIdx.x] = at;
+        at += c;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kLaneItems; ++u) {
+      const bool in_range = u < lane_items && mine + u * 32 + lane < valid;
+      const uint32_t bin = in_range ? (key[u] >> shift) & (bins - 1) : 0xffffffffu;
+      const uint32_t peers = __match_any_sync(0xffffffffu, bin);
+      const int before_me = __popc(peers & ((1u << lane) - 1u));
+      uint32_t to = 0;
+      if (in_range) to = h[warp * bins + bin] + before_me;
+      __syncwarp();
+      if (in_range && before_me == 0) h[warp * bins + bin] += __popc(peers);
+      __syncwarp();
+      if (in_range) {
+        const uint32_t owner = to / share, at = to - owner * share;
+        *cluster.map_shared_rank(&keys[at], owner) = key[u];
+        *cluster.map_shared_rank(&pos[at], owner) = p[u];
+      }
+    }
+    cluster.sync();
+#pragma unroll
+    for (int u = 0; u < kLaneItems; ++u) {
+      const int i = mine + u * 32 + lane;
+      if (u < lane_items && i < valid) key[u] = keys[i], p[u] = pos[i];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kLaneItems; ++u) {
+    const int i = mine + u * 32 + lane;
+    if (u < lane_items && i < valid) {
+      keys_out[(int64_t)rank * share + i] = key[u];
+      pos_out[(int64_t)rank * share + i] = p[u];
+    }
   }
 }
 
@@ -682,6 +798,33 @@ extern "C" stade_status stade_embed_b(int dtype, void* wb, const int64_t* ids, v
               SortIn{ids, nullptr, nullptr, base, n_v}, (int)n_s, p.passes, p.bits, sc.keys[0],
               sc.pos[0], fill);
           STADE_CHECK_LAUNCH();
+        } else if (n_s <= kClusterSort) {
+          const int lane_items = (int)((n_s + kClusterSort / kLaneItems - 1) /
+                                       (kClusterSort / kLaneItems));
+          const size_t smem =
+              (2 * (size_t)kSortWarps * 32 * lane_items + (size_t)kSortWarps * bins) * 4;
+          STADE_CUDA(cudaFuncSetAttribute(cluster_sort_kernel,
+                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+          cudaLaunchConfig_t cfg = {};
+          // clusters that clear: with the sort's no more than can be on the GPU at
+          // once (two of eight blocks in each of eight groups of SMs), since one
+          // that starts late would end late
+          const int clearing = (std::min(clearers, kSortCtas * 14) + kSortCtas - 1) / kSortCtas;
+          cfg.gridDim = dim3(kSortCtas * (1 + clearing));
+          cfg.blockDim = dim3(32 * kSortWarps);
+          cfg.dynamicSmemBytes = smem;
+          cfg.stream = s;
+          cudaLaunchAttribute attr[1];
+          attr[0].id = cudaLaunchAttributeClusterDimension;
+          attr[0].val.clusterDim.x = kSortCtas;
+          attr[0].val.clusterDim.y = 1;
+          attr[0].val.clusterDim.z = 1;
+          cfg.attrs = attr;
+          cfg.numAttrs = 1;
+          STADE_CUDA(cudaLaunchKernelEx(&cfg, cluster_sort_kernel,
+                                        SortIn{ids, nullptr, nullptr, base, n_v}, (int)n_s, p.passes,
+                                        p.bits, lane_items, sc.keys[0], sc.pos[0], fill));
+          count_launch();
         } else {
           const int64_t per_pass = p.blocks << p.bits;
           const bool scan = p.blocks > kFusedScan;

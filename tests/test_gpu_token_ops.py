@@ -167,7 +167,8 @@ def test_layer_norm_b_against_differences():
 EMBED_SIZES = [(1, 1, 1, 0), (1, 1000, 784, 0), (5, 3, 32, 0), (96, 1000, 784, 0), (257, 50, 33, 1),
                (3000, 7, 64, 0), (2048, 512, 40, 0), (2049, 511, 100, 3), (5000, 100000, 24, 0),
                (9000, 3000, 17, 0), (300, 20, 4100, 0), (4096, 70000, 8, 0), (4097, 300, 24, 0),
-               (140000, 600, 3, 0), (20000, 20, 260, 0)]
+               (140000, 600, 3, 0), (20000, 20, 260, 0),
+               (65536, 70000, 5, 0), (65537, 3000, 4, 1), (8193, 2 ** 18, 2, 0)]
 
 
 def _ids(seed, n_s, n_v, base):
