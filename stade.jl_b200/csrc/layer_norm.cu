@@ -897,31 +897,36 @@ stade_status with_row_warps(int64_t n_d, int align, F&& f) {
 //  - Forward: rows of up to 256 vectors one a thread and up to four rows a turn,
 //    1,024 threads an SM at 64 registers; longer ones two vectors a thread and
 //    two rows a turn, 640 threads at 96 (16384 x 4096 bf16: 49.6 us against 55.8
-//    with one vector; 16384 x 2048: 34.9 against 31.0). Two blocks of 257 to 384
-//    threads with whole vectors do better a row a turn (8192 x 5000 f16: 43.8
-//    against 46.3 us; single columns, 8192 x 4999: 76 against 64).
+//    with one vector; 16384 x 2048: 34.9 against 31.0). Where that leaves blocks
+//    of 257 to 384 threads with whole vectors, two of them and a row a turn do
+//    better (8192 x 5000 f16: 43.8 against 46.3 us; single columns, 8192 x 4999:
+//    76 against 64).
 //  - Reverse: the row's h and g w stay in registers, 512 threads at 128, so two
 //    vectors a thread and two or more blocks an SM rather than several rows a
 //    turn, which left one block and its barriers alone on the SM (16384 x 4096
 //    bf16: 83 us against 106 with four rows a turn; 32768 x 1024: 48 against
-//    56). Single columns spill at two vectors' worth: two rows a turn there
-//    (32768 x 1023 bf16: 63 us against 93).
+//    56). Narrower columns spill at two vectors' worth: one vector's and two rows
+//    a turn there (32768 x 1023 bf16: 63 us against 93); 16-bit rows of 513 to
+//    768 vectors' length one vector's and one row (8192 x 4999 f16: 94 against
+//    133).
 struct RingPlan {
   int m, rows, threads, stages, blocks;
   size_t smem;
 };
-bool ring_plan(int64_t n_s, int64_t row_bytes, bool rev, bool wide, RingPlan* p) {
+bool ring_plan(int64_t n_s, int64_t row_bytes, int size, bool rev, bool wide, RingPlan* p) {
   const int64_t slots = (row_bytes + 15) / 16;   // a thread owns 16 bytes of a row, or 32
   if (slots < 96 || slots > 2 * 768) return false;
-  p->m = rev ? (wide || slots > 512 ? 2 : 1) : slots <= 256 ? 1 : 2;
+  const int64_t single = rev ? (wide ? 0 : size == 2 ? 768 : 512) : 256;
+  p->m = slots <= single ? 1 : 2;
   p->threads = (int)(((slots + p->m - 1) / p->m + 31) / 32 * 32);
-  const int per_sm = std::max(1, (rev ? 512 : p->m == 2 ? 640 : 1024) / p->threads);
+  const bool two_blocks = !rev && wide && p->threads > 256 && p->threads <= 384;
+  const int per_sm =
+      two_blocks ? 2 : std::max(1, (rev ? 512 : p->m == 2 ? 640 : 1024) / p->threads);
   const int arrays = rev ? 2 : 1;
   const int64_t room = 200 * 1024 / (per_sm * row_bytes * arrays);   // rows in flight a block
   // several rows a turn where every block still gets two turns
-  const bool two_blocks = wide && p->threads > 256 && p->threads <= 384;
-  const bool one = n_s < 4 * 148 * per_sm || room < 4 ||
-                   (p->m > 1 && (rev || p->threads > 512 || two_blocks));
+  const bool one = n_s < 4 * 148 * per_sm || room < 4 || two_blocks || p->threads > 512 ||
+                   (p->m > 1 && rev);
   p->rows = one ? 1 : p->m == 1 && !rev && room >= 8 && n_s >= 8 * 148 * per_sm ? 4 : 2;
   p->stages = (int)std::min<int64_t>(kMaxStages, std::max<int64_t>(2, room / p->rows));
   p->smem = 128 + p->stages * arrays * ((p->rows * row_bytes + 31) & ~int64_t(15));
@@ -948,12 +953,13 @@ stade_status fwd(const void* x, const void* w, const void* b, void* y, void* m, 
       return (stade_status)STADE_OK;
     });
   RingPlan rp;
-  if (row_align(16, {x}) == 16 && ring_plan(n_s, row_bytes, false, align == 16, &rp)) {
+  if (row_align(16, {x}) == 16 && ring_plan(n_s, row_bytes, sizeof(T), false, align == 16, &rp)) {
     return with_width<T>(align, [&](auto vw) {
       constexpr int VW = decltype(vw)::value;
       auto kern = rp.threads > 512 ? ln_fwd_ring_kernel<T, 2 * V, VW, 1, 768, 1>
                   : rp.m == 2 ? (rp.rows == 2 ? ln_fwd_ring_kernel<T, 2 * V, VW, 2, 512, 1>
-                                              : ln_fwd_ring_kernel<T, 2 * V, VW, 1, 512, 1>)
+                                 : rp.threads <= 384 ? ln_fwd_ring_kernel<T, 2 * V, VW, 1, 384, 2>
+                                                     : ln_fwd_ring_kernel<T, 2 * V, VW, 1, 512, 1>)
                   : rp.rows == 4 ? ln_fwd_ring_kernel<T, V, VW, 4, 256, 4>
                   : rp.rows == 2 ? ln_fwd_ring_kernel<T, V, VW, 2, 256, 4>
                                  : ln_fwd_ring_kernel<T, V, VW, 1, 256, 4>;
@@ -1004,7 +1010,7 @@ stade_status bwd(const void* x, void* xb, const void* w, void* wb, void* bb, voi
       STADE_CHECK_LAUNCH();
       return (stade_status)STADE_OK;
     });
-  } else if (row_align(16, {x, yb}) == 16 && ring_plan(n_s, row_bytes, true, align == 16, &rp)) {
+  } else if (row_align(16, {x, yb}) == 16 && ring_plan(n_s, row_bytes, sizeof(T), true, align == 16, &rp)) {
     count = rp.blocks;
     const BwdArgs p{x, w, m, r, xb, yb, ws, n_s, (int)n_d, add, zero, sums};
     e = with_width<T>(align, [&](auto vw) {
@@ -1013,8 +1019,9 @@ stade_status bwd(const void* x, void* xb, const void* w, void* wb, void* bb, voi
       if (rp.threads > 512) kern = ln_bwd_ring_kernel<T, 2 * V, VW, 1, 768, false>;
       if constexpr (VW != V)
         if (rp.m == 1)
-          kern = rp.rows == 2 ? ln_bwd_ring_kernel<T, V, VW, 2, 512, true>
-                              : ln_bwd_ring_kernel<T, V, VW, 1, 512, true>;
+          kern = rp.threads > 512 ? ln_bwd_ring_kernel<T, V, VW, 1, 768, true>
+                 : rp.rows == 2   ? ln_bwd_ring_kernel<T, V, VW, 2, 512, true>
+                                  : ln_bwd_ring_kernel<T, V, VW, 1, 512, true>;
       STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                       (int)rp.smem));
       kern<<<rp.blocks, rp.threads, rp.smem, st>>>(p, rp.stages);
