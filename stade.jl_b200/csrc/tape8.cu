@@ -167,8 +167,8 @@ template <int ACT, bool FAST> __device__ __forceinline__ P2 act_d_pair(P2 x) {
 // Adding 1.5 2^23 rounds a value of less than 2^22 to the nearest whole number,
 // ties to even, and leaves it in the low bits: the code's byte is the low one.
 constexpr float kMagic = 12582912.f;
-__device__ __forceinline__ P2 code_bits2(P2 v, float inv) {
-  const P2 r = mul2(v, both(inv));
+__device__ __forceinline__ P2 code_bits2(P2 v, P2 inv) {
+  const P2 r = mul2(v, inv);
   return add2(P2(fminf(fmaxf(r.lo(), -127.f), 127.f), fminf(fmaxf(r.hi(), -127.f), 127.f)),
               both(kMagic));
 }
@@ -189,7 +189,7 @@ __device__ __forceinline__ P2 code_value2(uint32_t w, int k, P2 step) {
 // of x a load, 8 bytes of codes a store, and the group's largest magnitude by
 // two shuffles. Rows that are no multiple of 8 values, or arrays that do not
 // start on the boundary such accesses need, go through the kernels further
-// down, one value a thread.
+// down.
 constexpr int kV = 8;
 
 template <class T>
@@ -276,7 +276,7 @@ push8_kernel(const T* __restrict__ x, T* __restrict__ y, int8_t* __restrict__ q,
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       p[k] = pair_of<T>(v, k);
-      c[k] = code_bits2(p[k], inv);
+      c[k] = code_bits2(p[k], both(inv));
     }
     uint2 w = make_uint2(pack4(c[0], c[1]), pack4(c[2], c[3]));
     if (code == 255) w = make_uint2(0, 0);
@@ -333,80 +333,130 @@ pop8_kernel(T* __restrict__ xb, T* __restrict__ yb, const int8_t* __restrict__ q
   }
 }
 
-// Any row length and alignment: a warp takes kGroups groups of a row, a value a
-// lane of each, all of them in flight.
+// Other row lengths and alignments: a warp takes kGroups groups of a row, all of
+// them in flight. W = 2 (rows of an even number of values): half a warp a
+// group, two neighbours a lane; W = 1: a warp a group, a value a lane, two
+// groups at a time, so that arithmetic runs in pairs either way.
 constexpr int kGroups = 8;
+constexpr int kPairs = kGroups / 2;
 
-template <class T, int ACT>
+// Where a lane's pair k lies in a row, from the first of the groups on: its two
+// values, and the two groups they belong to.
+template <int W>
+struct Place {
+  int lane;
+  __device__ __forceinline__ int group(int k, int v) const {
+    return W == 2 ? 2 * k + (lane >> 4) : 2 * k + v;
+  }
+  __device__ __forceinline__ int value(int k, int v) const {
+    return group(k, v) * kGroup + (W == 2 ? 2 * (lane & 15) + v : lane);
+  }
+};
+template <int W, class E>
+__device__ __forceinline__ Vec<E, 2> load_pair(const E* p, const Place<W>& pl, int k,
+                                               int64_t left) {
+  Vec<E, 2> r{};
+  if constexpr (W == 2) {
+    if (pl.value(k, 0) < left) r = *reinterpret_cast<const Vec<E, 2>*>(p + pl.value(k, 0));
+  } else {
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+      if (pl.value(k, v) < left) r.v[v] = p[pl.value(k, v)];
+  }
+  return r;
+}
+template <int W, class E>
+__device__ __forceinline__ void store_pair(E* p, const Place<W>& pl, int k, int64_t left,
+                                           Vec<E, 2> r) {
+  if constexpr (W == 2) {
+    if (pl.value(k, 0) < left) *reinterpret_cast<Vec<E, 2>*>(p + pl.value(k, 0)) = r;
+  } else {
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+      if (pl.value(k, v) < left) p[pl.value(k, v)] = r.v[v];
+  }
+}
+
+template <class T, int ACT, int W>
 __global__ void __launch_bounds__(kThreads)
 push_kernel(const T* __restrict__ x, T* __restrict__ y, int8_t* __restrict__ q,
             uint8_t* __restrict__ e, int64_t n_g, int64_t segs, int64_t count, int64_t n_d) {
   const int lane = threadIdx.x & 31;
+  const Place<W> pl{lane};
   for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < count;
        i += (int64_t)gridDim.x * (kThreads / 32)) {
     const int64_t s = i / segs, g0 = (i - s * segs) * kGroups;
-    const int64_t at = s * n_d + g0 * kGroup + lane;
-    const int64_t left = n_d - g0 * kGroup - lane;     // values of the row from this lane's on
-    float v[kGroups];
-    int mine = 0;
+    const int64_t at = s * n_d + g0 * kGroup, left = n_d - g0 * kGroup;
+    Vec<T, 2> raw[kPairs];
 #pragma unroll
-    for (int j = 0; j < kGroups; ++j)
-      v[j] = j * kGroup < left ? (float)load_acc<T>(x[at + j * kGroup]) : 0.f;
+    for (int k = 0; k < kPairs; ++k) raw[k] = load_pair<W>(x + at, pl, k, left);
 #pragma unroll
-    for (int j = 0; j < kGroups; ++j) {
-      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(v[j]) & 0x7fffffffu);
-      const int code = scale_code(__uint_as_float(top));
-      if (lane == j) mine = code;
-      const uint32_t c =
-          code == 255 ? 0u
-                      : __float_as_uint(code_bits2(both(v[j]), pow2f(127 - min(code, 253))).lo());
-      if (j * kGroup < left) {
-        q[at + j * kGroup] = (int8_t)(c & 255u);
-        if constexpr (ACT != STADE_ACT_NONE)
-          y[at + j * kGroup] = round_to<T>(act_pair<ACT, sizeof(T) == 2>(both(v[j])).lo());
+    for (int k = 0; k < kPairs; ++k) {
+      const P2 v = widen2(raw[k]);
+      int code[2];
+      if constexpr (W == 2) {
+        float top = larger(v.lo(), v.hi());
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = larger(top, __shfl_xor_sync(0xffffffffu, top, o));
+        code[0] = code[1] = scale_code(top);
+      } else {
+        code[0] = scale_code(__uint_as_float(
+            __reduce_max_sync(0xffffffffu, __float_as_uint(v.lo()) & 0x7fffffffu)));
+        code[1] = scale_code(__uint_as_float(
+            __reduce_max_sync(0xffffffffu, __float_as_uint(v.hi()) & 0x7fffffffu)));
       }
+      const P2 inv(pow2f(127 - min(code[0], 253)), pow2f(127 - min(code[1], 253)));
+      const P2 c = code_bits2(v, inv);
+      Vec<int8_t, 2> w;
+      w.v[0] = code[0] == 255 ? 0 : (int8_t)(__float_as_uint(c.lo()) & 255u);
+      w.v[1] = code[1] == 255 ? 0 : (int8_t)(__float_as_uint(c.hi()) & 255u);
+      store_pair<W>(q + at, pl, k, left, w);
+      if constexpr (ACT != STADE_ACT_NONE)
+        store_pair<W>(y + at, pl, k, left, narrow2<T>(act_pair<ACT, sizeof(T) == 2>(v)));
+      // one lane a group: the half warp's first, or lanes 0 and 1
+      const int v1 = W == 2 ? 0 : lane & 1;
+      const int g = pl.group(k, v1);
+      if ((W == 2 ? (lane & 15) == 0 : lane < 2) && g0 + g < n_g)
+        e[s * n_g + g0 + g] = (uint8_t)(v1 ? code[1] : code[0]);
     }
-    if (lane < kGroups && g0 + lane < n_g) e[s * n_g + g0 + lane] = (uint8_t)mine;
   }
 }
 
 // ACT none: x = x^ (pop). Otherwise xb (+)= yb f'(x^).
-template <class T, int ACT>
+template <class T, int ACT, int W>
 __global__ void __launch_bounds__(kThreads)
 pop_kernel(T* __restrict__ xb, T* __restrict__ yb, const int8_t* __restrict__ q,
            const uint8_t* __restrict__ e, int64_t n_g, int64_t segs, int64_t count, int64_t n_d,
            bool add, bool zero) {
   const int lane = threadIdx.x & 31;
+  const Place<W> pl{lane};
   for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < count;
        i += (int64_t)gridDim.x * (kThreads / 32)) {
     const int64_t s = i / segs, g0 = (i - s * segs) * kGroups;
-    const int64_t at = s * n_d + g0 * kGroup + lane;
-    const int64_t left = n_d - g0 * kGroup - lane;
+    const int64_t at = s * n_d + g0 * kGroup, left = n_d - g0 * kGroup;
     const int codes = lane < kGroups && g0 + lane < n_g ? e[s * n_g + g0 + lane] : 0;
-    int8_t c[kGroups];
-    float g[kGroups], old[kGroups];
+    Vec<int8_t, 2> c[kPairs];
+    Vec<T, 2> g[kPairs], old[kPairs];
 #pragma unroll
-    for (int j = 0; j < kGroups; ++j)
-      if (j * kGroup < left) {
-        c[j] = q[at + j * kGroup];
-        if constexpr (ACT != STADE_ACT_NONE) {
-          g[j] = (float)load_acc<T>(yb[at + j * kGroup]);
-          if (add) old[j] = (float)load_acc<T>(xb[at + j * kGroup]);
-        }
+    for (int k = 0; k < kPairs; ++k) {
+      c[k] = load_pair<W>(q + at, pl, k, left);
+      if constexpr (ACT != STADE_ACT_NONE) {
+        g[k] = load_pair<W>((const T*)yb + at, pl, k, left);
+        if (add) old[k] = load_pair<W>((const T*)xb + at, pl, k, left);
       }
+    }
 #pragma unroll
-    for (int j = 0; j < kGroups; ++j) {
-      const int code = __shfl_sync(0xffffffffu, codes, j);
-      if (j * kGroup < left) {
-        const float v = restore(c[j], code);
-        if constexpr (ACT == STADE_ACT_NONE) {
-          xb[at + j * kGroup] = round_to<T>(v);
-        } else {
-          float r = g[j] * act_d_pair<ACT, sizeof(T) == 2>(both(v)).lo();
-          if (add) r += old[j];
-          xb[at + j * kGroup] = round_to<T>(r);
-          if (zero) yb[at + j * kGroup] = round_to<T>(0.f);
-        }
+    for (int k = 0; k < kPairs; ++k) {
+      const int code0 = __shfl_sync(0xffffffffu, codes, pl.group(k, 0));
+      const int code1 = W == 2 ? code0 : __shfl_sync(0xffffffffu, codes, pl.group(k, 1));
+      const P2 v(restore(c[k].v[0], code0), restore(c[k].v[1], code1));
+      if constexpr (ACT == STADE_ACT_NONE) {
+        store_pair<W>(xb + at, pl, k, left, narrow2<T>(v));
+      } else {
+        P2 r = mul2(widen2(g[k]), act_d_pair<ACT, sizeof(T) == 2>(v));
+        if (add) r = add2(r, widen2(old[k]));
+        store_pair<W>(xb + at, pl, k, left, narrow2<T>(r));
+        if (zero) store_pair<W>(yb + at, pl, k, left, narrow2<T>(both(0.f)));
       }
     }
   }
@@ -473,8 +523,12 @@ stade_status push(const char* who, int dtype, int act, const void* x, void* y, i
         return (stade_status)STADE_OK;
       }
       const int64_t segs = (n_g + kGroups - 1) / kGroups;
-      push_kernel<T, decltype(a)::value><<<blocks_for(n_s * segs), kThreads, 0, s>>>(
-          (const T*)x, (T*)y, q, e, n_g, segs, n_s * segs, n_d);
+      const bool even = n_d % 2 == 0 && row_align(2 * sizeof(T), {x, y}) >= 2 * (int)sizeof(T) &&
+                        row_align(2, {q}) >= 2;
+      constexpr int ACT = decltype(a)::value;
+      auto kern = even ? push_kernel<T, ACT, 2> : push_kernel<T, ACT, 1>;
+      kern<<<blocks_for(n_s * segs), kThreads, 0, s>>>((const T*)x, (T*)y, q, e, n_g, segs,
+                                                       n_s * segs, n_d);
       STADE_CHECK_LAUNCH();
       return (stade_status)STADE_OK;
     });
@@ -504,8 +558,12 @@ stade_status pop(const char* who, int dtype, int act, void* xb, void* yb, const 
         return (stade_status)STADE_OK;
       }
       const int64_t segs = (n_g + kGroups - 1) / kGroups;
-      pop_kernel<T, decltype(a)::value><<<blocks_for(n_s * segs), kThreads, 0, s>>>(
-          (T*)xb, (T*)yb, q, e, n_g, segs, n_s * segs, n_d, accumulates(opts), consumes(opts));
+      const bool even = n_d % 2 == 0 && row_align(2 * sizeof(T), {xb, yb}) >= 2 * (int)sizeof(T) &&
+                        row_align(2, {q}) >= 2;
+      constexpr int ACT = decltype(a)::value;
+      auto kern = even ? pop_kernel<T, ACT, 2> : pop_kernel<T, ACT, 1>;
+      kern<<<blocks_for(n_s * segs), kThreads, 0, s>>>((T*)xb, (T*)yb, q, e, n_g, segs, n_s * segs,
+                                                       n_d, accumulates(opts), consumes(opts));
       STADE_CHECK_LAUNCH();
       return (stade_status)STADE_OK;
     });
