@@ -654,6 +654,26 @@ def test_calls_inside_a_captured_graph():
     assert all(torch.equal(a, b) for a, b in zip(got, (y, q, xb, wb, tb)))
 
 
+def test_embed_b_of_a_long_batch_in_a_graph():
+    """The sort that runs in a cluster, and what overlaps it, replayed."""
+    n_s, n_v, n_d = 9000, 3000, 36
+    yb = _rand(1, n_s, n_d).bfloat16().cuda()
+    ids = torch.from_numpy(_ids(2, n_s, n_v, 0)).cuda()
+    wb, again = torch.empty(n_v, n_d, device="cuda"), torch.empty(n_v, n_d, device="cuda")
+    args = (1.5, n_s, n_v, n_d)
+    sb.embed_b_cuda(again, ids, yb, *args, accumulate=False, consume=False)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        sb.embed_b_cuda(wb, ids, yb, *args, accumulate=False, consume=False)
+    ids.copy_(torch.from_numpy(_ids(7, n_s, n_v, 0)))
+    for _ in range(3):
+        wb.fill_(math.nan)
+        g.replay()
+    sb.embed_b_cuda(again, ids, yb, *args, accumulate=False, consume=False)
+    assert torch.equal(wb, again)
+
+
 def test_zero_sizes():
     e = torch.empty(0, device="cuda")
     ids = torch.empty(0, dtype=torch.int64, device="cuda")
