@@ -67,9 +67,9 @@ plan_kernel(const int64_t* __restrict__ off, int64_t n_s, int64_t n_e, int tile,
   before_next();
   auto larger = [](long long a, long long b) { return a > b ? a : b; };
   auto sum = [](long long a, long long b) { return a + b; };
-  long long low = 0, low_end = 0;     // the bound before this round's first, the first of all
+  long long low = 0, low_end = 0;     // the bound before this pass's first, the first of all
   int done = 0;                       // tiles so far
-  // round r: entries 1023 r .. 1023 r + 1023, the last of them the next round's first
+  // pass r: entries 1023 r .. 1023 r + 1023, the last of them the next pass's first
   for (int64_t e0 = 0; e0 <= n_e; e0 += 1023) {
     const int64_t e = e0 + t;
     long long v = 0;
