@@ -499,11 +499,13 @@ ln_bwd_ring_kernel(BwdArgs p, int stages) {
   const bool mine = own.has(0);
   for (int64_t s = first; s < p.n_s; s += step, out += step * ring.row_bytes) {
     const int rows = (int)min((int64_t)R, p.n_s - s);
-    A rstd[R], shift[R], v[2 * R];     // h = x rstd + shift
+    // h = (x - mean) rstd: one product with -mean rstd added is an instruction
+    // less, but its rounding does not cancel where the mean is large for the row
+    A rstd[R], less[R], v[2 * R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       rstd[q] = nr[q];
-      shift[q] = -nm[q] * nr[q];
+      less[q] = -nm[q];
       v[2 * q] = v[2 * q + 1] = A(0);
     }
     stats(s + step);
@@ -517,11 +519,11 @@ ln_bwd_ring_kernel(BwdArgs p, int stages) {
         Pair<A> cx[E / 2], cy[E / 2], sg = both(A(0)), sgh = both(A(0));
         own.load(in + q * ring.row_bytes, cx);
         own.load(in + ring.array_bytes + q * ring.row_bytes, cy);
-        const Pair<A> rs = both(rstd[q]), sh = both(shift[q]);
+        const Pair<A> rs = both(rstd[q]), mn = both(less[q]);
 #pragma unroll
         for (int k = 0; k < E / 2; ++k) {
           // columns the thread does not have: yb = 0 there, so nothing is added
-          const Pair<A> h = fma2(cx[k], rs, sh), gw = mul2(cy[k], w[k]);
+          const Pair<A> h = mul2(add2(cx[k], mn), rs), gw = mul2(cy[k], w[k]);
           sg = add2(sg, gw);
           sgh = fma2(gw, h, sgh);
           sw[k] = fma2(cy[k], h, sw[k]);
@@ -543,7 +545,7 @@ ln_bwd_ring_kernel(BwdArgs p, int stages) {
         if (p.xb) {
           uint8_t* o = (uint8_t*)p.xb + out + q * ring.row_bytes;
           // rstd (g - mean(g) - h mean(g h))
-          const Pair<A> rs = both(rstd[q]), sh = both(shift[q]);
+          const Pair<A> rs = both(rstd[q]), mn = both(less[q]);
           const Pair<A> mg = both(-v[2 * q] * rstd[q]), mgh = both(-v[2 * q + 1] * rstd[q]);
           if (!KEEP) {
             own.load(in + q * ring.row_bytes, cx);
@@ -551,7 +553,7 @@ ln_bwd_ring_kernel(BwdArgs p, int stages) {
           }
 #pragma unroll
           for (int k = 0; k < E / 2; ++k) {
-            const Pair<A> h = KEEP ? kh[KEEP ? q : 0][k] : fma2(cx[k], rs, sh);
+            const Pair<A> h = KEEP ? kh[KEEP ? q : 0][k] : mul2(add2(cx[k], mn), rs);
             const Pair<A> gw = KEEP ? kg[KEEP ? q : 0][k] : mul2(cy[k], w[k]);
             cx[k] = fma2(gw, rs, fma2(h, mgh, mg));
           }
@@ -690,15 +692,15 @@ ln_bwd_warp_kernel(BwdArgs p) {
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       rstd[q] = q < rows ? r[s + q] : A(0);
-      const A shift = q < rows ? -m[s + q] * rstd[q] : A(0);
+      const A less = q < rows ? -m[s + q] : A(0);
       v[2 * q] = v[2 * q + 1] = A(0);
       if (q < rows && mine) {
         Pair<A> sg = both(A(0)), sgh = both(A(0));
-        const Pair<A> rs = both(rstd[q]), sh = both(shift);
+        const Pair<A> rs = both(rstd[q]), mn = both(less);
 #pragma unroll
         for (int k = 0; k < E / 2; ++k) {
           // columns the lane does not have: yb = 0 there, so nothing is added
-          const Pair<A> h = fma2(cx[q][k], rs, sh), g = cy[q][k], gw = mul2(g, w[k]);
+          const Pair<A> h = mul2(add2(cx[q][k], mn), rs), g = cy[q][k], gw = mul2(g, w[k]);
           sg = add2(sg, gw);
           sgh = fma2(gw, h, sgh);
           sw[k] = fma2(g, h, sw[k]);

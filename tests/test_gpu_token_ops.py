@@ -142,6 +142,26 @@ def test_layer_norm_mean_far_from_zero():
     assert np.abs(R.f64(r) / rstd - 1).max() < 1e-4
 
 
+@pytest.mark.parametrize("dt", ALL)
+@pytest.mark.parametrize("n_s,n_d,off", [(1300, 1, 0), (300, 64, 0), (37, 96, 0), (40, 1000, 0), (9, 1024, 1),
+                                         (700, 4096, 0), (40, 5001, 0), (3, 20000, 0)])
+def test_layer_norm_b_rows_at_their_mean(n_s, n_d, off, dt):
+    """Where every x is its row's mean, h is 0 whatever rstd is: wb is exactly
+    0 and xb is rstd (g - mean(g))."""
+    dt = R.DTYPES[dt]
+    P = R.par(dt)
+    at = (torch.arange(n_s, dtype=torch.float64) * 37 % 255 - 127)
+    x = _dev(at[:, None].expand(n_s, n_d), dt, off)
+    yb = _dev(_rand(1, n_s, n_d), dt, off)
+    m, r = at.to(P).cuda(), torch.full((n_s,), 1e-5 ** -0.5, dtype=P, device="cuda")
+    xb = torch.full((n_s, n_d), math.nan, dtype=dt, device="cuda")
+    wb, bb = torch.full((n_d,), math.nan, dtype=P, device="cuda"), torch.zeros(n_d, dtype=P, device="cuda")
+    (want, _, _), (mag, _, _) = R.layer_norm_b(R.f64(x), None, R.f64(yb), R.f64(m), R.f64(r))
+    sb.layer_norm_b_cuda(x, xb, None, wb, bb, yb, m, r, n_s, n_d, accumulate=False, consume=False)
+    assert torch.equal(wb, torch.zeros_like(wb))
+    R.assert_close(xb, want, mag, 3 * n_d + 32, "xb")
+
+
 def test_layer_norm_b_against_differences():
     n_s, n_d, h = 5, 41, 1e-6
     x, w, b, yb = _rand(1, n_s, n_d), _rand(2, n_d), _rand(3, n_d), _rand(4, n_s, n_d)
