@@ -104,10 +104,10 @@ __device__ __forceinline__ P2 tail2(P2 x, P2* g) {
   p = fma2(p, t, both(0.5f * 0.254829592f));
   return mul2(mul2(p, t), *g);
 }
-// 1 / (1 + exp(-x))
+// 1 / (1 + exp(-x)), which reaches 0 where exp(-x) passes Float32's range: x
+// times any floor would not vanish for the largest x
 __device__ __forceinline__ P2 sigmoid2(P2 x) {
-  return P2(rcp(1.f + ex2(fminf(x.lo() * -kLog2e, 120.f))),
-            rcp(1.f + ex2(fminf(x.hi() * -kLog2e, 120.f))));
+  return P2(rcp(1.f + ex2(x.lo() * -kLog2e)), rcp(1.f + ex2(x.hi() * -kLog2e)));
 }
 // 1 - 2 / (1 + exp 2x), and the Taylor polynomial near 0, where that cancels
 __device__ __forceinline__ P2 tanh2(P2 x) {

@@ -1,0 +1,57 @@
+"""The token-model operators where their values and their callers leave the
+ordinary range."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import stadeb200 as sb
+import token_ref as R
+from stadeb200 import token_ops as T
+
+pytestmark = pytest.mark.gpu
+
+NO64 = ["f32", "bf16", "f16"]
+NEW = dict(accumulate=False, consume=False)
+
+
+def _rand(seed, *shape, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=g, dtype=torch.float64) * scale
+
+
+# ---- activations -------------------------------------------------------------------
+# widths of the kernels for whole eights, for pairs and for single values
+WIDTHS = [32, 30, 31]
+
+
+def _act_both(act, x, yb):
+    """y, and xb for the seed yb, through the tape."""
+    n_s, n_d = x.shape
+    y, xb = torch.full_like(x, math.nan), torch.full_like(x, math.nan)
+    q, e = sb.initstacks_tape8_cuda(n_s, n_d)
+    sb.act_tape8_cuda(act, x, y, q, e, n_s, n_d)
+    sb.act_tape8_b_cuda(act, xb, yb, q, e, n_s, n_d, **NEW)
+    return y, xb
+
+
+@pytest.mark.parametrize("dt", NO64)
+@pytest.mark.parametrize("act", list(T.ACTIVATIONS))
+@pytest.mark.parametrize("n_d", WIDTHS)
+def test_act_tape8_far_out(n_d, act, dt):
+    """From 60 on every activation is 0 (tanh: -1) to the left with slope 0
+    and x (tanh: 1) to the right with slope 1 (tanh: 0), to the type's largest
+    value: sigmoid(-60) and the tails of tanh and Phi there are below 1e-25."""
+    dt = R.DTYPES[dt]
+    far = [60.0, 96.0, 150.0, 1000.0, 6e4] + ([1e15, 1e30, 1e36] if dt != torch.float16 else [])
+    far.append(torch.finfo(dt).max)
+    x = torch.tensor([-v for v in far] + far, dtype=torch.float64).to(dt)
+    n = len(far)
+    x = x[:, None].expand(2 * n, n_d).contiguous().cuda()       # a group of one value each
+    yb = _rand(1, 2 * n, n_d).to(dt).cuda()
+    y, xb = (R.f64(t) for t in _act_both(act, x, yb))
+    X, seed = R.f64(x), R.f64(yb)
+    left, right, slope = (-1.0, 1.0, 0.0) if act == "tanh" else (0.0, X[n:], 1.0)
+    assert np.abs(y[:n] - left).max() < 1e-20 and np.all(y[n:] == right)
+    assert np.abs(xb[:n]).max() < 1e-20 and np.abs(xb[n:] - slope * seed[n:]).max() < 1e-20
