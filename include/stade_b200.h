@@ -508,7 +508,9 @@ stade_status stade_layer_norm_b(int dtype, const void* x, void* xb, const void* 
  * largest magnitude; a group that held an infinity or NaN reads back as NaN.
  * push writes the tape, pop restores x from it. act_tape8 also computes
  * y = f(x); act_tape8_b adds yb f'(x^) to xb, x^ from the tape. relu'(0) =
- * 1/2, as in the generated sweeps. */
+ * 1/2, as in the generated sweeps. y at an infinity is what the formula gives:
+ * silu and gelu of -infinity are NaN (infinity over infinity, infinity times
+ * 0), in every type; finite x, to the type's lowest value, give 0 there. */
 #define STADE_ACT_NONE 0
 #define STADE_ACT_RELU 1
 #define STADE_ACT_TANH 2

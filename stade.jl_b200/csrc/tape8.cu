@@ -128,12 +128,13 @@ __device__ __forceinline__ P2 act_f2(P2 x) {
     return mul2(x, sigmoid2(x));
   }
   if constexpr (ACT == STADE_ACT_GELU) {
-    // x Phi(x) = max(x, 0) - |x| (1 - Phi(|x|)); the product is 0 from 14 on, also
-    // for an infinity, and NaN for a NaN
+    // x Phi(x) = max(x, 0) - |x| (1 - Phi(|x|)). The product is 0 from 14 on; to
+    // the right also for an infinity, to the left it is NaN there, as x times
+    // (1 + erf) is in the Float32 form.
     P2 g;
     const P2 q = tail2(x, &g);
-    return P2(fmaf(-fminf(fabsf(x.lo()), 14.f), q.lo(), fmaxf(x.lo(), 0.f)),
-              fmaf(-fminf(fabsf(x.hi()), 14.f), q.hi(), fmaxf(x.hi(), 0.f)));
+    return P2(fmaf(-fabsf(fminf(x.lo(), 14.f)), q.lo(), fmaxf(x.lo(), 0.f)),
+              fmaf(-fabsf(fminf(x.hi(), 14.f)), q.hi(), fmaxf(x.hi(), 0.f)));
   }
   return P2(act_f<ACT>(x.lo()), act_f<ACT>(x.hi()));
 }

@@ -55,3 +55,23 @@ def test_act_tape8_far_out(n_d, act, dt):
     left, right, slope = (-1.0, 1.0, 0.0) if act == "tanh" else (0.0, X[n:], 1.0)
     assert np.abs(y[:n] - left).max() < 1e-20 and np.all(y[n:] == right)
     assert np.abs(xb[:n]).max() < 1e-20 and np.abs(xb[n:] - slope * seed[n:]).max() < 1e-20
+
+
+@pytest.mark.parametrize("dt", NO64)
+@pytest.mark.parametrize("act", list(T.ACTIVATIONS))
+@pytest.mark.parametrize("n_d", WIDTHS)
+def test_act_tape8_infinities(n_d, act, dt):
+    """Infinities and NaN give what the formulas in 64 bits give, in every type:
+    x / (1 + exp(-x)) and x (1 + erf) / 2 are NaN at -infinity. Their groups
+    come back as NaN."""
+    dt = R.DTYPES[dt]
+    x = _rand(2, 3, n_d).to(dt)
+    x[0, 3], x[1, 7], x[2, 0] = math.inf, -math.inf, math.nan
+    with np.errstate(all="ignore"):
+        ref = R.act(act, R.f64(x))
+    y, xb = _act_both(act, x.cuda(), torch.ones(3, n_d, dtype=dt, device="cuda"))
+    got = R.f64(y)
+    assert np.array_equal(np.isnan(got), np.isnan(ref))
+    assert np.array_equal(got[np.isinf(ref)], ref[np.isinf(ref)])
+    assert np.isfinite(got).sum() >= 3 * n_d - 3
+    assert torch.isnan(xb).all()
