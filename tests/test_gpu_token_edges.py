@@ -75,3 +75,36 @@ def test_act_tape8_infinities(n_d, act, dt):
     assert np.array_equal(got[np.isinf(ref)], ref[np.isinf(ref)])
     assert np.isfinite(got).sum() >= 3 * n_d - 3
     assert torch.isnan(xb).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("act", list(T.ACTIVATIONS))
+@pytest.mark.parametrize("n_d", WIDTHS)
+def test_act_tape8_tails(n_d, act, dt):
+    """The tails of the 16-bit forms, where values and slopes fall off as
+    exp(-x) or exp(-x^2 / 2), keep the type's relative precision: a quarter
+    of a rounding beside the one of the result."""
+    dt = R.DTYPES[dt]
+    at = torch.linspace(2.0, 12.0 if dt == torch.bfloat16 else 5.0, 41).to(dt)
+    x = torch.cat([-at, at])[:, None].expand(82, n_d).contiguous().cuda()
+    yb = torch.ones_like(x)
+    y, xb = _act_both(act, x, yb)
+    X = R.f64(x)
+    V = R.tape8_values(*R.tape8(X))
+    for name, out, ref in (("y", y, _act64(act, X)), ("slope", xb, _slope64(act, V))):
+        tol = 1.25 * R.UNIT[dt] * np.abs(ref) + R.TINY[dt]
+        err = np.abs(R.f64(out) - ref)
+        assert np.all(err <= tol), f"{name}: {(err / tol).max():.2f} x bound at x = {X.flat[(err / tol).argmax()]}"
+
+
+_erfc = np.vectorize(math.erfc)
+
+
+def _act64(act, x):
+    return 0.5 * x * _erfc(-x / math.sqrt(2)) if act == "gelu" else R.act(act, x)
+
+
+def _slope64(act, x):
+    if act == "gelu":
+        return 0.5 * _erfc(-x / math.sqrt(2)) + x * np.exp(-x * x / 2) / math.sqrt(2 * math.pi)
+    return R.act_slope(act, x)
