@@ -280,6 +280,10 @@ sort_scatter_kernel(SortIn in, int64_t n, int shift, int bins, int blocks,
 constexpr int kSmallItems = 256;              // elements of a warp
 constexpr int kSmallWarps = kSmallSort / kSmallItems;
 constexpr int kSmallThreads = kSmallWarps * 32;
+// A launch's shared memory, at most. The sorts' limits are set to these whatever
+// a call needs: the limit is the kernel's, and a host thread with another size
+// must not lower it between this call's setting and its launch.
+constexpr int kSmallSmem = (2 * kSmallSort + kSmallWarps * kMaxBins) * 4;
 __global__ void __launch_bounds__(kSmallThreads)
 small_sort_kernel(SortIn in, int n, int passes, int bits, uint32_t* __restrict__ keys_out,
                   uint32_t* __restrict__ pos_out, Fill fill) {
@@ -361,6 +365,7 @@ constexpr int kSortCtas = 8;
 constexpr int kSortWarps = 32;
 constexpr int kLaneItems = 8;               // keys a lane holds, at most
 constexpr int kClusterSort = kSortCtas * kSortWarps * 32 * kLaneItems;
+constexpr int kClusterSmem = (2 * kSortWarps * 32 * kLaneItems + kSortWarps * kMaxBins) * 4;
 
 __global__ void __launch_bounds__(32 * kSortWarps)
 cluster_sort_kernel(SortIn in, int n, int passes, int bits, int lane_items,
@@ -793,7 +798,7 @@ extern "C" stade_status stade_embed_b(int dtype, void* wb, const int64_t* ids, v
         if (n_s <= kSmallSort) {
           const size_t smem = (2 * kSmallSort + (size_t)kSmallWarps * bins) * 4;
           STADE_CUDA(cudaFuncSetAttribute(small_sort_kernel,
-                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+                                          cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallSmem));
           small_sort_kernel<<<1 + clearers, kSmallThreads, smem, s>>>(
               SortIn{ids, nullptr, nullptr, base, n_v}, (int)n_s, p.passes, p.bits, sc.keys[0],
               sc.pos[0], fill);
@@ -804,7 +809,7 @@ extern "C" stade_status stade_embed_b(int dtype, void* wb, const int64_t* ids, v
           const size_t smem =
               (2 * (size_t)kSortWarps * 32 * lane_items + (size_t)kSortWarps * bins) * 4;
           STADE_CUDA(cudaFuncSetAttribute(cluster_sort_kernel,
-                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+                                          cudaFuncAttributeMaxDynamicSharedMemorySize, kClusterSmem));
           cudaLaunchConfig_t cfg = {};
           // clusters that clear: with the sort's no more than can be on the GPU at
           // once (two of eight blocks in each of eight groups of SMs), since one

@@ -911,6 +911,7 @@ stade_status with_row_warps(int64_t n_d, int align, F&& f) {
 //    a turn there (32768 x 1023 bf16: 63 us against 93); 16-bit rows of 513 to
 //    768 vectors' length one vector's and one row (8192 x 4999 f16: 94 against
 //    133).
+constexpr int kRingSmem = 205 * 1024;   // a block's ring, at most
 struct RingPlan {
   int m, rows, threads, stages, blocks;
   size_t smem;
@@ -933,7 +934,15 @@ bool ring_plan(int64_t n_s, int64_t row_bytes, int size, bool rev, bool wide, Ri
   p->stages = (int)std::min<int64_t>(kMaxStages, std::max<int64_t>(2, room / p->rows));
   p->smem = 128 + p->stages * arrays * ((p->rows * row_bytes + 31) & ~int64_t(15));
   p->blocks = (int)std::min<int64_t>((n_s + p->rows - 1) / p->rows, 148 * per_sm);
-  return p->smem <= 205 * 1024;
+  return p->smem <= kRingSmem;
+}
+// The limit of a kernel's shared memory is the kernel's, not the launch's: always
+// the same value, so that host threads with rows of other lengths do not lower
+// it between this call's setting and its launch.
+template <class K>
+stade_status allow_ring(K kern) {
+  STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
+  return STADE_OK;
 }
 
 template <class T>
@@ -965,8 +974,8 @@ stade_status fwd(const void* x, const void* w, const void* b, void* y, void* m, 
                   : rp.rows == 4 ? ln_fwd_ring_kernel<T, V, VW, 4, 256, 4>
                   : rp.rows == 2 ? ln_fwd_ring_kernel<T, V, VW, 2, 256, 4>
                                  : ln_fwd_ring_kernel<T, V, VW, 1, 256, 4>;
-      STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)rp.smem));
+      const stade_status ok = allow_ring(kern);
+      if (ok != STADE_OK) return ok;
       kern<<<rp.blocks, rp.threads, rp.smem, st>>>((const T*)x, (const A*)w, (const A*)b, (T*)y,
                                                    (A*)m, (A*)r, eps, n_s, (int)n_d, rp.stages);
       STADE_CHECK_LAUNCH();
@@ -1024,8 +1033,8 @@ stade_status bwd(const void* x, void* xb, const void* w, void* wb, void* bb, voi
           kern = rp.threads > 512 ? ln_bwd_ring_kernel<T, V, VW, 1, 768, true>
                  : rp.rows == 2   ? ln_bwd_ring_kernel<T, V, VW, 2, 512, true>
                                   : ln_bwd_ring_kernel<T, V, VW, 1, 512, true>;
-      STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)rp.smem));
+      const stade_status ok = allow_ring(kern);
+      if (ok != STADE_OK) return ok;
       kern<<<rp.blocks, rp.threads, rp.smem, st>>>(p, rp.stages);
       STADE_CHECK_LAUNCH();
       return (stade_status)STADE_OK;

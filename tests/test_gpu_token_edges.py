@@ -1,6 +1,8 @@
 """The token-model operators where their values and their callers leave the
 ordinary range."""
+import ctypes as C
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -8,6 +10,7 @@ import torch
 
 import stadeb200 as sb
 import token_ref as R
+from stadeb200 import _lib
 from stadeb200 import token_ops as T
 
 pytestmark = pytest.mark.gpu
@@ -108,3 +111,58 @@ def _slope64(act, x):
     if act == "gelu":
         return 0.5 * _erfc(-x / math.sqrt(2)) + x * np.exp(-x * x / 2) / math.sqrt(2 * math.pi)
     return R.act_slope(act, x)
+
+
+# ---- threads, streams, workspaces ----------------------------------------------------
+@pytest.mark.parametrize("op", ["fwd", "bwd", "sort", "cluster"])
+def test_host_threads(op):
+    """Calls that share a kernel but want different amounts of shared memory, from
+    four threads on streams of their own: none takes another's limit for its
+    launch. Two sizes of each kernel, 98 KB and 26 KB in reverse for instance."""
+    L, failed = _lib.lib(), []
+
+    def calls(k, s):
+        """(C function, arguments, a check of the results)"""
+        o = _lib.make_opts(s.cuda_stream, None, 0, _lib.STADE_ADJ_STORE | _lib.STADE_SEED_KEEP)
+        if op in ("sort", "cluster"):
+            n_s, n_v, n_d = (100, 400 if k else 12, 4) if op == "sort" else (65536 if k else 5000, 500 if k else 12, 1)
+            ids = torch.arange(n_s, device="cuda") % n_v
+            yb, wb = torch.ones(n_s, n_d, device="cuda"), torch.zeros(n_v, n_d, device="cuda")
+            ws = torch.empty(T.embed_b_workspace(n_s, n_v, n_d), dtype=torch.uint8, device="cuda")
+            o.workspace, o.workspace_bytes = ws.data_ptr(), ws.numel()
+            args = (_lib.STADE_F32, wb.data_ptr(), ids.data_ptr(), yb.data_ptr(), 1.0, 0, n_s, n_v, n_d)
+            want = torch.bincount(ids, minlength=n_v).float()[:, None].expand(n_v, n_d)
+            return L.stade_embed_b, args, o, lambda: torch.equal(wb, want), (ids, yb, ws)
+        n_s, n_d = 64, 2048 if k else (1100 if op == "fwd" else 400)
+        x = _rand(k, n_s, n_d).float().cuda()
+        y, m, r = torch.empty_like(x), torch.empty(n_s, device="cuda"), torch.empty(n_s, device="cuda")
+        ref = torch.from_numpy(R.layer_norm(R.f64(x), None, None, 1e-5)[0])
+        if op == "fwd":
+            args = (_lib.STADE_F32, x.data_ptr(), None, None, y.data_ptr(), m.data_ptr(), r.data_ptr(), 1e-5, n_s, n_d)
+            return L.stade_layer_norm, args, o, lambda: (y.cpu() - ref).abs().max() < 1e-5, (x, m, r)
+        T.layer_norm_cuda(x, None, None, y, m, r, 1e-5, n_s, n_d)
+        torch.cuda.synchronize()
+        bb = torch.zeros(n_d, device="cuda")
+        ws = torch.empty(T.layer_norm_b_workspace(torch.float32, n_s, n_d), dtype=torch.uint8, device="cuda")
+        o.workspace, o.workspace_bytes = ws.data_ptr(), ws.numel()
+        args = (_lib.STADE_F32, x.data_ptr(), None, None, None, bb.data_ptr(), y.data_ptr(), m.data_ptr(), r.data_ptr(), n_s, n_d)
+        return L.stade_layer_norm_b, args, o, lambda: (bb.cpu() - ref.sum(0)).abs().max() < 1e-4, (x, y, m, r, ws)
+
+    def work(k):
+        torch.cuda.set_device(0)
+        s = torch.cuda.Stream()
+        fn, args, o, good, _keep = calls(k, s)
+        torch.cuda.synchronize()
+        ready.wait()
+        codes = {fn(*args, C.byref(o)) for _ in range(4000 if op != "cluster" else 1000)}
+        s.synchronize()
+        if codes != {_lib.STADE_OK} or not good():
+            failed.append((k, codes, L.stade_last_error()))
+
+    ready = threading.Barrier(4)
+    threads = [threading.Thread(target=work, args=(k % 2,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
