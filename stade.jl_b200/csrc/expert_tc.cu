@@ -19,7 +19,11 @@
 //
 // A Float32 operand is held as three bf16 planes whose sum is the value (8
 // bits of mantissa each, rounded to nearest); the product is the six plane
-// products down to 2^-16 of it, each an ordinary K loop over its two planes.
+// products down to 2^-16 of it, each an ordinary K loop over its two planes. The
+// planes reach down to bf16's smallest value, 2^-133: operands below 2^-110 lose
+// their last bits, below 2^-134 they count as 0. Where the five minor products'
+// sum is not finite, an operand is infinite or NaN and the leading product
+// gives the result alone: an infinity then stays one, as in a plain product.
 //
 // The tensor cores' Float32 sums truncate: their error grows with the number
 // of MMAs into one accumulator, by about 2^-25 of it each. An accumulator takes
@@ -523,6 +527,14 @@ expert_tc_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant
 #pragma unroll
               for (int j = 0; j < 16; ++j) sum[q][j] += v[j];
             }
+          }
+          // an infinity's lower planes are 0, and the other operand's mostly, so
+          // the minor products make NaN of it: the leading one alone has it right
+          if (sizeof(Out) == 4 && c + 1 == lp.n_small) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int j = 0; j < 16; ++j) sum[q][j] = isfinite(sum[q][j]) ? sum[q][j] : 0.f;
           }
         }
         tc5::fence_before();

@@ -113,6 +113,48 @@ def _slope64(act, x):
     return R.act_slope(act, x)
 
 
+# ---- expert_mm ---------------------------------------------------------------------
+def _same(out, ref, scale, k, name):
+    """Infinities and NaN in the same places, the rest within the bound."""
+    o = R.f64(out).reshape(ref.shape)
+    inf = np.isinf(ref)
+    assert np.array_equal(np.isnan(o), np.isnan(ref)), f"{name}: NaN in other places"
+    assert np.array_equal(np.isinf(o), inf) and np.array_equal(o[inf], ref[inf]), name
+    ok = np.isfinite(ref)
+    tol = (R.UNIT[out.dtype] * 1.001 * np.abs(ref) + R.TINY[out.dtype] + k * R.UNIT[R.par(out.dtype)] * scale)
+    assert np.all(np.abs(o - ref)[ok] <= tol[ok]), name
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("whole", [False, True])
+@pytest.mark.parametrize("off", [[0, 3, 3, 9], [0, 130, 131, 400]])
+def test_expert_mm_infinities(off, whole, dt):
+    """An infinity in x, w or yb reaches every result its row or column has a
+    part in, as in a plain product; whatever the number of rows. whole: values
+    of few bits, whose lower planes are 0."""
+    dt = R.DTYPES[dt]
+    n_s, n_e, n_i, n_o = off[-1], 3, 72, 136
+    x, w, yb = _rand(1, n_s, n_i), _rand(2, n_e, n_i, n_o), _rand(3, n_s, n_o)
+    if whole:
+        x, w, yb = (torch.sign(t) * torch.ceil(t.abs()) for t in (x, w, yb))
+    x, w, yb = (t.to(dt).cuda() for t in (x, w, yb))
+    x[1, 5], x[off[2] + 2, 71] = math.inf, -math.inf
+    w[2, 70, 9] = math.inf
+    yb[2, 0], yb[off[2] + 1, 130] = -math.inf, math.inf
+    o = torch.tensor(off).cuda()
+    X, W, Y = R.f64(x), R.f64(w), R.f64(yb)
+    with np.errstate(all="ignore"):
+        ref, mag = R.expert_mm(X, W, off)
+        xr, wr, mx, mw = R.expert_mm_b(X, W, Y, off)
+    y, xb = torch.zeros(n_s, n_o, dtype=dt, device="cuda"), torch.zeros(n_s, n_i, dtype=dt, device="cuda")
+    wb = torch.zeros(n_e, n_i, n_o, device="cuda")
+    sb.expert_mm_cuda(x, w, y, o, n_s, n_e, n_i, n_o)
+    sb.expert_mm_b_cuda(x, xb, w, wb, yb, o, n_s, n_e, n_i, n_o, **NEW)
+    _same(y, ref, mag, 2 * n_i + 8, "y")
+    _same(xb, xr, mx, 2 * n_o + 8, "xb")
+    _same(wb, wr, mw, 2 * n_s + 8, "wb")
+
+
 # ---- threads, streams, workspaces ----------------------------------------------------
 @pytest.mark.parametrize("op", ["fwd", "bwd", "sort", "cluster"])
 def test_host_threads(op):
