@@ -184,7 +184,16 @@ expert_wgrad_kernel(const T* __restrict__ x, const T* __restrict__ yb, acc_t<T>*
 // tensor cores' path writes them out as three planes first and reads those: six
 // times the bytes (6 rows, 2 experts, 2328 -> 3688: 107 us, of which 10 us is
 // the read). Here tiles of kFew rows multiply on the CUDA cores, the rows in
-// shared memory, the weights read once per tile straight into registers.
+// shared memory, the weights read once per tile straight into registers: once in
+// all when no group has more than kFew rows.
+//
+// The bounds are on the device, so the path goes by the average. Measured with
+// eight rows a group, spread evenly and all in one group (whose weights are then
+// read once per eight rows, and whose gradient few warps add up), against the
+// tensor cores' path; y, xb, wb in us:
+//   512 rows, 512 x 512     even 30, 92, 30    69, 71, 55     one 30, 92, 74     59, 58, 48
+//   4096 rows, 64 x 64      even 14, 90, 14    36, 36, 67     one 23, 99, 481    19, 20, 180
+//   32768 rows, 64 x 64     even 59, 704, 69   219, 220, 463  one 126, 739, 5220 64, 64, 1364
 constexpr int kFew = 8;
 constexpr int kFewK = 512;      // depth of one block's share of y = x W
 constexpr int kFewWarps = 8;
@@ -312,7 +321,13 @@ few_input_kernel(const float* __restrict__ yb, const float* __restrict__ w, floa
 }
 
 // wb[e] (+)= sum over the group's rows of x^T yb: one write of the gradient. A
-// warp takes four rows and 32 V columns of it and walks the group's rows.
+// warp takes four rows and 32 V columns of it and walks the group's rows. A
+// group can hold all rows: after kFewChain of them the sums go to the gradient
+// and begin anew, so that the error grows with the root of a chain's length and
+// of their number, not of the rows'. (Kept in a second set of registers they cost
+// a quarter of the time of groups of eight rows: 1,024 experts of 512 x 512, 441
+// us so, 582.)
+constexpr int kFewChain = 64;
 template <int V>
 __global__ void __launch_bounds__(32 * kFewWarps)
 few_weight_kernel(const float* __restrict__ x, const float* __restrict__ yb, float* __restrict__ wb,
@@ -322,35 +337,40 @@ few_weight_kernel(const float* __restrict__ x, const float* __restrict__ yb, flo
   const int64_t e = blockIdx.z, a = bounds[e], z = bounds[e + 1];
   const int i0 = (blockIdx.y * kFewWarps + warp) * 4, o = (blockIdx.x * 32 + lane) * V;
   if (i0 >= n_i || o >= n_o || (add && a == z)) return;
-  float acc[4][V] = {};
-  for (int64_t s = a; s < z; s += 4) {
-    Vec<float, V> g[4];
-    float f[4][4];
+  int64_t s = a;
+  do {
+    const int64_t upto = min(z, s + kFewChain);
+    float acc[4][V] = {};
+    for (; s < upto; s += 4) {
+      Vec<float, V> g[4];
+      float f[4][4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const bool in = s + u < z;
-      if (in) g[u] = *reinterpret_cast<const Vec<float, V>*>(yb + (s + u) * n_o + o);
+      for (int u = 0; u < 4; ++u) {
+        const bool in = s + u < upto;
+        if (in) g[u] = *reinterpret_cast<const Vec<float, V>*>(yb + (s + u) * n_o + o);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) f[u][j] = in && i0 + j < n_i ? x[(s + u) * n_i + i0 + j] : 0.f;
+        for (int j = 0; j < 4; ++j) f[u][j] = in && i0 + j < n_i ? x[(s + u) * n_i + i0 + j] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (s + u < upto)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[j][v] = fmaf(f[u][j], g[u].v[v], acc[j][v]);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (s + u < z)
+    for (int j = 0; j < 4; ++j)
+      if (i0 + j < n_i) {
+        float* p = wb + (e * n_i + i0 + j) * n_o + o;
+        Vec<float, V> r;
+        if (add) r = *reinterpret_cast<const Vec<float, V>*>(p);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int v = 0; v < V; ++v) acc[j][v] = fmaf(f[u][j], g[u].v[v], acc[j][v]);
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (i0 + j < n_i) {
-      float* p = wb + (e * n_i + i0 + j) * n_o + o;
-      Vec<float, V> r;
-      if (add) r = *reinterpret_cast<const Vec<float, V>*>(p);
-#pragma unroll
-      for (int v = 0; v < V; ++v) r.v[v] = add ? r.v[v] + acc[j][v] : acc[j][v];
-      *reinterpret_cast<Vec<float, V>*>(p) = r;
-    }
+        for (int v = 0; v < V; ++v) r.v[v] = add ? r.v[v] + acc[j][v] : acc[j][v];
+        *reinterpret_cast<Vec<float, V>*>(p) = r;
+      }
+    add = true;
+  } while (s < z);
 }
 
 // Whether the rows are few enough: no more than kFew a group on average.
