@@ -32,6 +32,12 @@ __device__ int g_embed_error = 0;
 
 constexpr int kThreads = 256;
 
+// Table row of an id, negative for padding; compared before the difference, which
+// can pass 64 bits.
+__device__ __forceinline__ int64_t table_row(int64_t id, int64_t base) {
+  return id < base ? -1 : (int64_t)min((uint64_t)id - (uint64_t)base, (uint64_t)INT64_MAX);
+}
+
 // A warp takes kFwdRows consecutive positions: their ids first, then column by
 // column one vector of each row, so that several rows' reads are in flight.
 constexpr int kFwdRows = 4;
@@ -48,7 +54,7 @@ embed_fwd_kernel(const T* __restrict__ w, const int64_t* __restrict__ ids, T* __
   bool ok[kFwdRows];
 #pragma unroll
   for (int q = 0; q < kFwdRows; ++q) {
-    const int64_t v = s0 + q < n_s ? ids[s0 + q] - base : -1;
+    const int64_t v = s0 + q < n_s ? table_row(ids[s0 + q], base) : -1;
     ok[q] = v >= 0 && v < n_v;
     if (v >= n_v && lane == 0) g_embed_error = 1;
     row[q] = reinterpret_cast<const V*>(w + (ok[q] ? v : 0) * n_d);
@@ -93,7 +99,7 @@ struct SortIn {
   int64_t base, n_v;
 };
 __device__ __forceinline__ uint32_t id_key(const SortIn& in, int64_t i) {
-  const int64_t v = in.ids[i] - in.base;
+  const int64_t v = table_row(in.ids[i], in.base);
   if (v >= in.n_v) g_embed_error = 1;
   return (uint32_t)(v >= 0 && v < in.n_v ? v : in.n_v);
 }

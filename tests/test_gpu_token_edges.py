@@ -175,6 +175,22 @@ def test_expert_mm_f32_one_expert_takes_all(n_s, n_e, n_i, n_o):
     assert not wb.any()
 
 
+# ---- ids -----------------------------------------------------------------------
+def test_embed_smallest_id_is_padding():
+    """Ids down to the type's smallest value are padding, not past the table."""
+    L = _lib.lib()
+    L.stade_device_error()
+    w = _rand(1, 10, 8).float().cuda()
+    ids = torch.tensor([1, -2 ** 63, 10, -2 ** 63 + 5, 0]).cuda()
+    y = torch.full((5, 8), math.nan, device="cuda")
+    sb.embed_cuda(w, ids, y, 1.0, 5, 10, 8, base=1)
+    wb = torch.zeros(10, 8, device="cuda")
+    sb.embed_b_cuda(wb, ids, torch.ones(5, 8, device="cuda"), 1.0, 5, 10, 8, base=1)
+    assert L.stade_device_error() == 0
+    assert torch.equal(y[0], w[0]) and torch.equal(y[2], w[9]) and not y[1].any() and not y[3:].any()
+    assert (wb[0] == 1).all() and (wb[9] == 1).all() and not wb[1:9].any()
+
+
 # ---- threads, streams, workspaces ----------------------------------------------------
 @pytest.mark.parametrize("op", ["fwd", "bwd", "sort", "cluster"])
 def test_host_threads(op):
