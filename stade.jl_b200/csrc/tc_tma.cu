@@ -1208,8 +1208,11 @@ extern "C" stade_status stade_check_bounded_wait(int64_t wait_cycles, const stad
 // The library's device error word: set when a bounded wait inside a
 // tensor-core kernel ran out (the kernel then skipped its remaining work and
 // returned), or when a token-model operator met an id or a group bound that
-// is out of range. Reading clears it.
+// is out of range. Reading clears it. The words are read by copies on the legacy
+// default stream, which waits for no stream created non-blocking: the wait for
+// the device is its own.
 extern "C" int stade_device_error(void) {
+  if (cudaDeviceSynchronize() != cudaSuccess) return -1;
   const int t = stade::tma_take_error();
   const int c = stade::conv_tc_take_error();
   const int h = stade::heat_take_error();

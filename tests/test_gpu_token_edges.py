@@ -244,3 +244,17 @@ def test_host_threads(op):
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+def test_device_error_waits_for_other_streams():
+    """The error word of a call that is still queued on another stream."""
+    L = _lib.lib()
+    L.stade_device_error()
+    w, ids, y = torch.ones(4, 8, device="cuda"), torch.tensor([9]).cuda(), torch.empty(1, 8, device="cuda")
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(100_000_000)
+        sb.embed_cuda(w, ids, y, 1.0, 1, 4, 8)
+    assert L.stade_device_error() != 0
+    assert L.stade_device_error() == 0
