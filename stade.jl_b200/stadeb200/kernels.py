@@ -41,10 +41,21 @@ def _arr(t: torch.Tensor, dtype: torch.dtype, n: int, name: str) -> int:
     return t.data_ptr()
 
 
+def _workspace(t):
+    """(address, bytes) of a caller's workspace: a contiguous tensor on the
+    current device, since the kernels write to it. An empty one is a workspace
+    of 0 bytes, not the absence of one (address 0)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"workspace: expected a CUDA tensor, got {type(t).__name__}")
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"workspace: tensor must live on the current CUDA device, not {t.device}")
+    if not t.is_contiguous():
+        raise ValueError("workspace: tensor must be contiguous")
+    return t.data_ptr() or 256, t.numel() * t.element_size()
+
+
 def _opts(stream, workspace, flags=0):
-    ws_ptr, ws_bytes = None, 0
-    if workspace is not None:
-        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    ws_ptr, ws_bytes = (None, 0) if workspace is None else _workspace(workspace)
     return make_opts(_stream_ptr(stream), ws_ptr, ws_bytes, flags)
 
 

@@ -70,8 +70,7 @@ def _run(fn, *args, stream=None, workspace=None, flags=0) -> None:
     if workspace is None:
         o = stade_opts(handle, None, 0, flags)
     else:
-        o = stade_opts(handle, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                       flags)
+        o = stade_opts(handle, *kernels._workspace(workspace), flags)
     code = fn(*args, C.byref(o))
     if code != STADE_OK:
         check(code)

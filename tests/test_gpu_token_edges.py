@@ -258,3 +258,16 @@ def test_device_error_waits_for_other_streams():
         sb.embed_cuda(w, ids, y, 1.0, 1, 4, 8)
     assert L.stade_device_error() != 0
     assert L.stade_device_error() == 0
+
+
+def test_workspace_refusals():
+    """Host memory, gaps between elements and an empty tensor are no workspace."""
+    n_s, n_v, n_d = 64, 10, 8
+    ids, yb, wb = torch.arange(n_s).cuda() % n_v, torch.ones(n_s, n_d, device="cuda"), torch.zeros(n_v, n_d, device="cuda")
+    need = T.embed_b_workspace(n_s, n_v, n_d)
+    for bad in (torch.empty(need, dtype=torch.uint8), torch.empty(2 * need, dtype=torch.uint8, device="cuda")[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            T.embed_b_cuda(wb, ids, yb, 1.0, n_s, n_v, n_d, workspace=bad)
+    with pytest.raises(sb.StadeError, match="workspace"):
+        T.embed_b_cuda(wb, ids, yb, 1.0, n_s, n_v, n_d, workspace=torch.empty(0, device="cuda"))
+    assert not wb.any() and (yb == 1).all()
