@@ -78,7 +78,9 @@ int         stade_kernel_launches(void);     /* kernels this thread launched sin
 void        stade_reset_kernel_launches(void);
 /* Bytes of the library-managed workspace cache on the current device (0 when
  * no entry point has needed one there: every call so far passed its own
- * workspace or needed none). */
+ * workspace or needed none). The cache grows to the largest call's needs; a
+ * buffer that a captured call uses is not freed then, so the graph stays
+ * valid. */
 size_t      stade_workspace_cached_bytes(void);
 /* Phase profiler (tracing): when enabled, entry points bracket each phase
  * with CUDA events on their stream; stade_profile_read waits for them and

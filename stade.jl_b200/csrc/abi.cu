@@ -17,6 +17,7 @@ thread_local int g_launches = 0;
 struct CachedWorkspace {
   void* ptr = nullptr;
   size_t bytes = 0;
+  bool captured = false;   // a graph may hold its address
 };
 std::mutex g_ws_mutex;
 std::vector<CachedWorkspace> g_ws;  // indexed by device ordinal
@@ -89,6 +90,15 @@ void phase_end(cudaStream_t s) {
   g_open_ev.pop_back();
 }
 
+namespace {
+bool capturing(cudaStream_t s) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(s, &st) == cudaSuccess) return st != cudaStreamCaptureStatusNone;
+  cudaGetLastError();      // the legacy stream while another one captures
+  return false;
+}
+}  // namespace
+
 stade_status get_workspace(const stade_opts* o, size_t bytes, void** p) {
   *p = nullptr;
   if (bytes == 0) return STADE_OK;
@@ -109,15 +119,17 @@ stade_status get_workspace(const stade_opts* o, size_t bytes, void** p) {
   if (w.bytes < bytes) {
     // Growth happens once per size class; a caller that must not allocate
     // passes its own workspace instead.
-    if (w.ptr) {
+    if (w.ptr && !w.captured) {
       STADE_CUDA(cudaDeviceSynchronize());
       STADE_CUDA(cudaFree(w.ptr));
-      w.ptr = nullptr;
-      w.bytes = 0;
     }
+    // a captured call writes to the buffer whenever its graph is replayed, so
+    // that one stays
+    w = CachedWorkspace();
     STADE_CUDA(cudaMalloc(&w.ptr, bytes));
     w.bytes = bytes;
   }
+  w.captured = w.captured || capturing(stream_of(o));
   *p = w.ptr;
   return STADE_OK;
 }

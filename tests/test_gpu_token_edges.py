@@ -2,6 +2,9 @@
 ordinary range."""
 import ctypes as C
 import math
+import os
+import subprocess
+import sys
 import threading
 
 import numpy as np
@@ -271,3 +274,46 @@ def test_workspace_refusals():
     with pytest.raises(sb.StadeError, match="workspace"):
         T.embed_b_cuda(wb, ids, yb, 1.0, n_s, n_v, n_d, workspace=torch.empty(0, device="cuda"))
     assert not wb.any() and (yb == 1).all()
+
+
+_GROWN = r"""
+import sys
+sys.path[:0] = [{pkg!r}]
+import torch
+import stadeb200 as sb
+from stadeb200 import _lib
+cached = _lib.lib().stade_workspace_cached_bytes
+n_s, n_v, n_d = 3000, 500, 64
+ids = torch.arange(n_s).cuda() * 7 % n_v
+yb = torch.randn(n_s, n_d, generator=torch.Generator().manual_seed(1)).cuda()
+wb, want = torch.empty(n_v, n_d, device="cuda"), torch.empty(n_v, n_d, device="cuda")
+new = dict(accumulate=False, consume=False)
+sb.embed_b_cuda(want, ids, yb, 1.0, n_s, n_v, n_d, **new)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    sb.embed_b_cuda(wb, ids, yb, 1.0, n_s, n_v, n_d, **new)
+before = cached()
+big = 200000
+sb.embed_b_cuda(torch.empty(n_v, 8, device="cuda"), torch.arange(big).cuda() % n_v, torch.ones(big, 8, device="cuda"),
+                1.0, big, n_v, 8, **new)
+assert cached() > before, "the second call has to want more"
+# what has been freed is handed out again, and filled
+fill = [torch.full((before // 4,), 7, dtype=torch.int32, device="cuda") for _ in range(8)]
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(wb, want)
+assert all((t == 7).all() for t in fill)
+sb.embed_b_cuda(wb, ids, yb, 1.0, n_s, n_v, n_d, **new)
+assert torch.equal(wb, want)
+print("ok")
+"""
+
+
+def test_graph_outlives_the_growth_of_the_cached_workspace():
+    """A graph whose call used the library's workspace is replayed after a larger
+    call has made the cache grow. In a process of its own, whose cache starts
+    empty."""
+    pkg = os.path.dirname(os.path.dirname(os.path.abspath(sb.__file__)))
+    r = subprocess.run([sys.executable, "-c", _GROWN.format(pkg=pkg)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "ok" in r.stdout, r.stderr[-2000:]
