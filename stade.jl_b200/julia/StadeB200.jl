@@ -299,12 +299,13 @@ end
 adjoint_opts(accumulate, consume) =
     opts(flags = (accumulate ? UInt32(0) : STADE_ADJ_STORE) |
                  (consume ? UInt32(0) : STADE_SEED_KEEP))
+# addresses of arrays that may be of several types: taken inside GC.@preserve
 optional(a) = a === nothing ? CU_NULL : reinterpret(CuPtr{Cvoid}, pointer(a))
 rawptr(a) = reinterpret(CuPtr{Cvoid}, pointer(a))
 
 # ids count from 1; an id of 0 or less is padding
 function embed_cuda(w, ids, y, scale, n_s, n_v, n_d)
-    check(ccall((:stade_embed, libstade), Cint,
+    GC.@preserve w y check(ccall((:stade_embed, libstade), Cint,
         (Cint, CuPtr{Cvoid}, CuPtr{Int64}, CuPtr{Cvoid}, Float64, Int64, Int64, Int64, Int64,
          Ref{StadeOpts}),
         stade_dtype(eltype(y)), rawptr(w), ids, rawptr(y), scale, 1, n_s, n_v, n_d, opts()))
@@ -312,7 +313,7 @@ function embed_cuda(w, ids, y, scale, n_s, n_v, n_d)
 end
 
 function embed_b_cuda(wb, ids, yb, scale, n_s, n_v, n_d; accumulate = true, consume = true)
-    check(ccall((:stade_embed_b, libstade), Cint,
+    GC.@preserve wb yb check(ccall((:stade_embed_b, libstade), Cint,
         (Cint, CuPtr{Cvoid}, CuPtr{Int64}, CuPtr{Cvoid}, Float64, Int64, Int64, Int64, Int64,
          Ref{StadeOpts}),
         stade_dtype(eltype(yb)), rawptr(wb), ids, rawptr(yb), scale, 1, n_s, n_v, n_d,
@@ -322,7 +323,7 @@ end
 
 # w and b may be nothing (ones and zeros)
 function layer_norm_cuda(x, w, b, y, m_stack, r_stack, eps, n_s, n_d)
-    check(ccall((:stade_layer_norm, libstade), Cint,
+    GC.@preserve x w b y m_stack r_stack check(ccall((:stade_layer_norm, libstade), Cint,
         (Cint, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid},
          CuPtr{Cvoid}, Float64, Int64, Int64, Ref{StadeOpts}),
         stade_dtype(eltype(x)), rawptr(x), optional(w), optional(b), rawptr(y), rawptr(m_stack),
@@ -333,7 +334,7 @@ end
 # xb, wb and bb may be nothing (not wanted)
 function layer_norm_b_cuda(x, xb, w, wb, bb, yb, m_stack, r_stack, n_s, n_d;
                            accumulate = true, consume = true)
-    check(ccall((:stade_layer_norm_b, libstade), Cint,
+    GC.@preserve x xb w wb bb yb m_stack r_stack check(ccall((:stade_layer_norm_b, libstade), Cint,
         (Cint, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid},
          CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, Int64, Int64, Ref{StadeOpts}),
         stade_dtype(eltype(x)), rawptr(x), optional(xb), optional(w), optional(wb), optional(bb),
@@ -348,14 +349,14 @@ function initstacks_tape8_cuda(n_s, n_d)
 end
 
 function tape8_push_cuda(x, q_stack, e_stack, n_s, n_d)
-    check(ccall((:stade_tape8_push, libstade), Cint,
+    GC.@preserve x check(ccall((:stade_tape8_push, libstade), Cint,
         (Cint, CuPtr{Cvoid}, CuPtr{Int8}, CuPtr{UInt8}, Int64, Int64, Ref{StadeOpts}),
         stade_dtype(eltype(x)), rawptr(x), q_stack, e_stack, n_s, n_d, opts()))
     return nothing
 end
 
 function tape8_pop_cuda(x, q_stack, e_stack, n_s, n_d)
-    check(ccall((:stade_tape8_pop, libstade), Cint,
+    GC.@preserve x check(ccall((:stade_tape8_pop, libstade), Cint,
         (Cint, CuPtr{Cvoid}, CuPtr{Int8}, CuPtr{UInt8}, Int64, Int64, Ref{StadeOpts}),
         stade_dtype(eltype(x)), rawptr(x), q_stack, e_stack, n_s, n_d, opts()))
     return nothing
@@ -363,7 +364,7 @@ end
 
 # act: :relu, :tanh, :silu or :gelu
 function act_tape8_cuda(act, x, y, q_stack, e_stack, n_s, n_d)
-    check(ccall((:stade_act_tape8, libstade), Cint,
+    GC.@preserve x y check(ccall((:stade_act_tape8, libstade), Cint,
         (Cint, Cint, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Int8}, CuPtr{UInt8}, Int64, Int64,
          Ref{StadeOpts}),
         stade_dtype(eltype(x)), STADE_ACT[act], rawptr(x), rawptr(y), q_stack, e_stack, n_s, n_d,
@@ -373,7 +374,7 @@ end
 
 function act_tape8_b_cuda(act, xb, yb, q_stack, e_stack, n_s, n_d;
                           accumulate = true, consume = true)
-    check(ccall((:stade_act_tape8_b, libstade), Cint,
+    GC.@preserve xb yb check(ccall((:stade_act_tape8_b, libstade), Cint,
         (Cint, Cint, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Int8}, CuPtr{UInt8}, Int64, Int64,
          Ref{StadeOpts}),
         stade_dtype(eltype(yb)), STADE_ACT[act], rawptr(xb), rawptr(yb), q_stack, e_stack, n_s,
@@ -383,7 +384,7 @@ end
 
 # off: n_e + 1 row counts from 0 (off[e] rows come before expert e's)
 function expert_mm_cuda(x, w, y, off, n_s, n_e, n_i, n_o)
-    check(ccall((:stade_expert_mm, libstade), Cint,
+    GC.@preserve x w y check(ccall((:stade_expert_mm, libstade), Cint,
         (Cint, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Int64}, Int64, Int64, Int64, Int64,
          Ref{StadeOpts}),
         stade_dtype(eltype(x)), rawptr(x), rawptr(w), rawptr(y), off, n_s, n_e, n_i, n_o, opts()))
@@ -393,7 +394,7 @@ end
 # xb or wb may be nothing (not wanted)
 function expert_mm_b_cuda(x, xb, w, wb, yb, off, n_s, n_e, n_i, n_o;
                           accumulate = true, consume = true)
-    check(ccall((:stade_expert_mm_b, libstade), Cint,
+    GC.@preserve x xb w wb yb check(ccall((:stade_expert_mm_b, libstade), Cint,
         (Cint, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Cvoid}, CuPtr{Int64},
          Int64, Int64, Int64, Int64, Ref{StadeOpts}),
         stade_dtype(eltype(yb)), rawptr(x), optional(xb), rawptr(w), optional(wb), rawptr(yb), off,
