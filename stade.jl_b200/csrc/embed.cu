@@ -15,7 +15,10 @@
 // measured copy rate by the bytes moved. The gradient of the same rows into a
 // table of 50021 (205 MB of Float32) takes 65 us, 41 by its bytes: the sort, with
 // the clearing beside it (34 us under the profiler), the sums (21 us) and the
-// parts' join (11 us) wait for one another.
+// parts' join (11 us) wait for one another. Past 65,536 positions the sort no
+// longer fits one cluster and takes five launches or more, whose digit counts one
+// block scans: 65536 x 256 bf16 into 50021 rows 67 us, 65537 83, 262144 198 (28 by
+// bytes), 1048576 x 64 639.
 
 #include <cooperative_groups.h>
 

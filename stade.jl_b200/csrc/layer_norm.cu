@@ -30,7 +30,11 @@ namespace {
 //    a block each, the rows to come copied by cp.async.bulk into a ring in
 //    shared memory, several rows ahead of the arithmetic;
 //  - other rows: a group of G threads each, NV values a thread, read directly;
-//  - rows too long for registers: read again from the caches.
+//  - rows too long for registers: read again from the caches. In reverse these
+//    are rows past 24 KB, in two kernels of one value an access (4096 x 8192
+//    Float32: 157 us, 61 by memory); clearing the seed in the second one's loop
+//    keeps a thread to one row in flight (1,113 us with the default flags, 102
+//    for the bytes that then move).
 
 // Sums of two values over the block, the same in every thread. `red`: 2 x 2 x 32
 // values, used alternately (`turn`), so that one barrier per sum is enough.
@@ -460,10 +464,11 @@ ln_fwd_ring_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,
 
 // KEEP: h and g w stay in registers over the sums; otherwise the row is read
 // and widened from the stage once more (the longest rows, whose threads have 80
-// registers). 16-bit rows are bound by instructions and by the latency of a
-// turn's sums, not by memory: 16384 x 4096 takes 103 us in bf16 when the row is
-// read twice (32 instructions an element), 83 us kept, 61 us by memory alone;
-// in Float32 129 us, 0.95 of the measured copy rate.
+// registers and spill 100 to 324 bytes: 4096 x 12288 bf16 110 us, 46 by memory).
+// 16-bit rows wait for a turn's two sums and their barriers: with 16 warps an SM
+// 47 % of the issue slots are used and 0.76 of the measured copy rate (16384 x
+// 4096 bf16: 81 us, 61 by memory; 103 when the row is read twice). Float32 rows
+// have twice the bytes to wait for: 125 us, 0.98 of that rate.
 template <class T, int E, int VW, int R, int MAXT, bool KEEP>
 __global__ void __launch_bounds__(MAXT, 1)
 ln_bwd_ring_kernel(BwdArgs p, int stages) {
@@ -584,7 +589,10 @@ constexpr int kRowWarps = 8;
 
 // R rows a turn, all their loads in flight. Lanes with more than 16 bytes of a
 // row take one row a turn and leave room for three blocks an SM (65536 x 512
-// bf16: 34 us; 44 with two rows).
+// bf16: 34 us; 44 with two rows). Lanes with three vectors of 16-bit values (rows
+// of 513 to 767) spill 120 to 136 bytes here and 200 to 236 in reverse, Float64
+// rows of 129 to 191 200 to 220 there: 16384 x 640 bf16 19 and 36 us, 6.4 and 9.6
+// by memory.
 template <class T, int E, int VW, int R>
 __global__ void __launch_bounds__(32 * kRowWarps, R == 1 ? 3 : 1)
 ln_fwd_warp_kernel(const T* __restrict__ x, const acc_t<T>* __restrict__ w,

@@ -15,8 +15,10 @@
 // in the forward shows in the gradient instead of vanishing in a code.
 //
 // Bound by memory, with the instructions close behind: gelu of 8192 x 8192 in
-// bf16 takes 68 us forward and 63 us in reverse under the profiler, 51 us each
-// by their bytes, with three quarters of the issue slots in use.
+// bf16 takes 68 us forward and 67 us in reverse, 51 us each by their bytes, with
+// three quarters of the issue slots in use; tanh in reverse 53 us. In Float32,
+// 8192 x 4096: relu, tanh and silu 0.86 to 0.98 of the measured copy rate, gelu
+// 55 us forward and 82 in reverse, 46 by their bytes (erff and expf).
 
 #include <algorithm>
 #include <initializer_list>
