@@ -35,10 +35,12 @@ __device__ int g_embed_error = 0;
 
 constexpr int kThreads = 256;
 
-// Table row of an id, negative for padding; compared before the difference, which
-// can pass 64 bits.
-__device__ __forceinline__ int64_t table_row(int64_t id, int64_t base) {
-  return id < base ? -1 : (int64_t)min((uint64_t)id - (uint64_t)base, (uint64_t)INT64_MAX);
+// Whether an id is in the table; below base it is padding, past the table an
+// error. Compared before the difference, which can pass 64 bits.
+__device__ __forceinline__ bool in_table(int64_t id, int64_t base, int64_t n_v, bool* past) {
+  const bool in = (uint64_t)id - (uint64_t)base < (uint64_t)n_v;
+  *past = id >= base && !in;
+  return id >= base && in;
 }
 
 // A warp takes kFwdRows consecutive positions: their ids first, then column by
@@ -54,14 +56,16 @@ embed_fwd_kernel(const T* __restrict__ w, const int64_t* __restrict__ ids, T* __
   const int64_t s0 = ((int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kFwdRows;
   if (s0 >= n_s) return;
   const V* row[kFwdRows];
-  bool ok[kFwdRows];
+  bool ok[kFwdRows], error = false;
 #pragma unroll
   for (int q = 0; q < kFwdRows; ++q) {
-    const int64_t v = s0 + q < n_s ? table_row(ids[s0 + q], base) : -1;
-    ok[q] = v >= 0 && v < n_v;
-    if (v >= n_v && lane == 0) g_embed_error = 1;
-    row[q] = reinterpret_cast<const V*>(w + (ok[q] ? v : 0) * n_d);
+    const int64_t id = s0 + q < n_s ? ids[s0 + q] : INT64_MIN;
+    bool past;
+    ok[q] = in_table(id, base, n_v, &past);
+    error |= past;
+    row[q] = reinterpret_cast<const V*>(w + (ok[q] ? id - base : 0) * n_d);
   }
+  if (error) g_embed_error = 1;
   const int n = (int)min((int64_t)kFwdRows, n_s - s0);
   V* out = reinterpret_cast<V*>(y + s0 * n_d);
   for (int j = lane; j < slots; j += 32) {
@@ -102,9 +106,11 @@ struct SortIn {
   int64_t base, n_v;
 };
 __device__ __forceinline__ uint32_t id_key(const SortIn& in, int64_t i) {
-  const int64_t v = table_row(in.ids[i], in.base);
-  if (v >= in.n_v) g_embed_error = 1;
-  return (uint32_t)(v >= 0 && v < in.n_v ? v : in.n_v);
+  const int64_t id = in.ids[i];
+  bool past;
+  const bool ok = in_table(id, in.base, in.n_v, &past);
+  if (past) g_embed_error = 1;
+  return (uint32_t)(ok ? id - in.base : in.n_v);
 }
 __device__ __forceinline__ uint32_t sort_key(const SortIn& in, int64_t i) {
   return in.ids ? id_key(in, i) : in.keys[i];
