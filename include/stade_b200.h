@@ -480,8 +480,8 @@ stade_status stade_heat2d_b_f64_slab(double* loss, const double* lossb,
  * Arrays may start at any multiple of their element size; 16-byte boundaries
  * are what the fast paths want. Calls that have a *_workspace query use it for
  * the length of the call: calls that can overlap on the GPU (streams with no
- * order between them) need a workspace each, since the library's cached one
- * is shared.
+ * order between them), or that several host threads make at once, need a
+ * workspace each, since the library's cached one is shared.
  * ------------------------------------------------------------------------- */
 
 /* embed: y[s] = scale w[ids[s] - base] (rows of n_d), s = 0 .. n_s - 1; base 0

@@ -11,7 +11,9 @@ The reverse sweeps add to their adjoint outputs and set the consumed seed yb
 to zero, as the generated sweeps do; `accumulate=False` stores instead of
 adding and `consume=False` leaves yb as it is. The calls are asynchronous on
 `stream` (default: torch's current stream); a `workspace` tensor of at least
-the queried bytes replaces the library's cached one.
+the queried bytes replaces the library's cached one. That one is shared: calls
+on streams with no order between them, or from several host threads, need a
+workspace each.
 """
 from __future__ import annotations
 
