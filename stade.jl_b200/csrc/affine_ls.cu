@@ -25,6 +25,10 @@ namespace stade {
 namespace {
 
 constexpr int kThreads = 512;
+// A launch's shared memory, at most. The kernel's limit is set to this whatever a
+// call needs: the limit is the kernel's, and a host thread with another size must
+// not lower it between this call's setting and its launch.
+constexpr int kMaxSmem = 200 * 1024;
 
 // Global -> shared copy with `U` loads per thread in flight before any store
 // (one memory latency for a block's whole staging instead of one per pass).
@@ -241,7 +245,7 @@ extern "C" stade_status stade_affine_ls_b_f64(double* loss, const double* lossb,
   STADE_REQUIRE(loss && lossb && w && wb && b && bb && x && xb && t && tb && y && yb,
                 "affine_ls_b: null array argument");
   const Plan p = plan(n_s, n_o, n_i);
-  STADE_REQUIRE(p.smem <= 200 * 1024, "affine_ls_b: n_o * n_i = %lld too large for one block",
+  STADE_REQUIRE(p.smem <= kMaxSmem, "affine_ls_b: n_o * n_i = %lld too large for one block",
                 (long long)(n_o * n_i));
   STADE_REQUIRE(n_s < (int64_t(1) << 31) / 2 && n_o * n_i < (int64_t(1) << 30),
                 "affine_ls_b: size overflow");
@@ -253,7 +257,7 @@ extern "C" stade_status stade_affine_ls_b_f64(double* loss, const double* lossb,
   double* part = c.take<double>((size_t)p.nblk * (size_t)(n_o * n_i + n_o + 1));
   if (p.smem > 48 * 1024)
     STADE_CUDA(cudaFuncSetAttribute(affine_ls_chunk_kernel,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem));
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
   PhaseScope ph("affine", s);
   affine_ls_chunk_kernel<<<p.nblk, kThreads, p.smem, s>>>(lossb, w, b, x, xb, t, tb, y, yb, n_s,
                                                           (int)n_o, (int)n_i, p.chunk, part);
@@ -316,7 +320,7 @@ extern "C" stade_status stade_affine_ls_b_f64_noalloc(double* loss, const double
   STADE_REQUIRE(loss && lossb && w && wb && b && bb && x && xb && t && tb && y && yb,
                 "affine_ls_b_noalloc: null array argument");
   const Plan p = plan(n_s, n_o, n_i);
-  STADE_REQUIRE(p.smem <= 200 * 1024, "affine_ls_b_noalloc: n_o * n_i = %lld too large for one block",
+  STADE_REQUIRE(p.smem <= kMaxSmem, "affine_ls_b_noalloc: n_o * n_i = %lld too large for one block",
                 (long long)(n_o * n_i));
   STADE_REQUIRE(n_s < (int64_t(1) << 31) / 2 && n_o * n_i < (int64_t(1) << 30),
                 "affine_ls_b_noalloc: size overflow");
@@ -333,7 +337,7 @@ extern "C" stade_status stade_affine_ls_b_f64_noalloc(double* loss, const double
   cudaStream_t s = stream_of(opts);
   if (p.smem > 48 * 1024)
     STADE_CUDA(cudaFuncSetAttribute(affine_ls_chunk_kernel,
-                                    cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem));
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
   PhaseScope ph("affine", s);
   // every block writes all of its partial slots, so nothing needs clearing
   affine_ls_chunk_kernel<<<p.nblk, kThreads, p.smem, s>>>(lossb, w, b, x, xb, t, tb, y, yb, n_s,

@@ -33,6 +33,10 @@ namespace {
 
 constexpr int kHeadWarps = 8;   // samples in flight per block
 constexpr int kHvHeadWarps = 16;  // the same for the Float64 HVP head (one block per SM)
+// Shared memory of the kernels that hold w2, at most. Their limits are set to
+// these whatever a call needs: a limit is the kernel's, and a host thread with
+// another size must not lower it between this call's setting and its launch.
+constexpr int kLogitsSmem = 160 * 1024, kHeadSmem = 200 * 1024, kHvHeadSmem = 220 * 1024;
 // Sum over the 32 lanes of a[0..15] (each lane its own sixteen values): four
 // halving exchanges leave each lane pair one class's sum, class
 // ((l >> 4) & 1) * 8 + ((l >> 3) & 1) * 4 + ((l >> 2) & 1) * 2 + ((l >> 1) & 1).
@@ -1273,7 +1277,7 @@ extern "C" stade_status stade_mlp2_ce_b_f32(float* loss, const float* lossb, con
     // 1. h = tanh(x W1 + b1), TMA-fed tensor cores (the logits in a pass of
     // their own when w2 fits in shared memory, else in the GEMM's epilogue)
     const size_t lsm = sizeof(float) * (size_t)H * (O <= 16 ? 16 : 32);
-    const bool own_logits = lsm <= 160 * 1024 && H % 4 == 0;
+    const bool own_logits = lsm <= kLogitsSmem && H % 4 == 0;
     {
       PhaseScope ph("fwd_gemm", s);
       st = tma_forward_tanh_logits(x, w.x_lo, w1, w.w1_lo, b1, w2, h,
@@ -1288,14 +1292,15 @@ extern "C" stade_status stade_mlp2_ce_b_f32(float* loss, const float* lossb, con
       if (own_logits && O <= 16 && H % 128 == 0 && logits_rows_enabled()) {
         if (lsm > 48 * 1024)
           STADE_CUDA(cudaFuncSetAttribute(mlp_logits_rows_kernel,
-                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)lsm));
+                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          kLogitsSmem));
         mlp_logits_rows_kernel<<<2 * tc5::sm_count(), 256, lsm, s>>>(h, w2, w.zpart, S, H, O);
         STADE_CHECK_LAUNCH();
       } else if (own_logits) {
         auto lk = O <= 16 ? mlp_logits_kernel<16> : mlp_logits_kernel<32>;
         if (lsm > 48 * 1024)
           STADE_CUDA(cudaFuncSetAttribute(lk, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          (int)lsm));
+                                          kLogitsSmem));
         lk<<<6 * tc5::sm_count(), 256, lsm, s>>>(h, w2, w.zpart, S, H, O);
         STADE_CHECK_LAUNCH();
       }
@@ -1353,11 +1358,11 @@ extern "C" stade_status stade_mlp2_ce_b_f32(float* loss, const float* lossb, con
   {
     PhaseScope ph("head", s);
     const size_t head_smem = sizeof(float) * (size_t)(n_h * n_o);
-    STADE_REQUIRE(head_smem <= 200 * 1024, "mlp2_ce_b: n_h * n_o too large");
+    STADE_REQUIRE(head_smem <= kHeadSmem, "mlp2_ce_b: n_h * n_o too large");
     auto kern = O <= 16 ? mlp_head_b_kernel<float, 16> : mlp_head_b_kernel<float, 32>;
     if (head_smem > 48 * 1024)
-      STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)head_smem));
+      STADE_CUDA(
+          cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeadSmem));
     kern<<<w.head_blocks, kHeadWarps * 32, head_smem, s>>>(lossb, y, yb, w2, b2, h, hb, z, zb, p,
                                                            pb, w.gbuf, w.s1b, S, H, O, w.loss_part);
     STADE_CHECK_LAUNCH();
@@ -1449,11 +1454,11 @@ extern "C" stade_status stade_mlp2_ce_hv_f64(
   const size_t w2_bytes = sizeof(double) * 2 * (size_t)O * (size_t)(H + 1);
   const size_t rows_bytes = sizeof(double) * kHvHeadWarps * 2 * (size_t)H;
   const int w2_smem = w2_bytes <= 160 * 1024;
-  const int rows_smem = w2_smem && w2_bytes + rows_bytes <= 220 * 1024;
+  const int rows_smem = w2_smem && w2_bytes + rows_bytes <= kHvHeadSmem;
   const size_t hsm = w2_bytes + (rows_smem ? rows_bytes : 0);
   if (w2_smem && hsm > 48 * 1024)
     STADE_CUDA(cudaFuncSetAttribute(mlp_head_hv_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    (int)hsm));
+                                    kHvHeadSmem));
   // with w2 in shared memory, one wave of the blocks the SMs hold at once
   // (each stages w2 once)
   int head_per_sm = 0;

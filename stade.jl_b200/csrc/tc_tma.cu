@@ -820,7 +820,8 @@ stade_status run(const Operand& A, const Operand& B, Geometry g, const EpiTanhLo
   if (st != STADE_OK) return st;
   const int smem = kSmemBytes + (EPI_KIND == 0 && el.w2_stride > 0 ? kW2SmemBytes : 0);
   STADE_CUDA(cudaFuncSetAttribute(tma_gemm_kernel<EPI_KIND, NO>,
-                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  std::min(232448, kSmemBytes + (EPI_KIND == 0 ? kW2SmemBytes : 0))));
   const int total = g.m_tiles * g.n_tiles * g.slices;
   const int grid = total < sm_count() ? total : sm_count();
   tma_gemm_kernel<EPI_KIND, NO><<<grid, kThreads, smem, s>>>(ah, al, bh, bl, g, el, ea, ep);
@@ -887,7 +888,10 @@ stade_status run_pair(const Operand& A, const Operand& B, Geometry g, const EpiT
   const int smem = P::kSmem + P::kStageOutBytes +
                    (EPI_KIND == 0 && el.w2_stride > 0 ? kW2SmemBytes : 0);
   auto kern = tma_gemm_pair_kernel<EPI_KIND, NO, TN>;
-  STADE_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // the kernel's limit, not the call's size: host threads share it
+  STADE_CUDA(cudaFuncSetAttribute(
+      kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      std::min(232448, P::kSmem + P::kStageOutBytes + (EPI_KIND == 0 ? kW2SmemBytes : 0))));
   const int total = g.m_tiles * g.n_tiles * g.slices;
   const int pairs = total < sm_count() / 2 ? total : sm_count() / 2;
   cudaLaunchConfig_t cfg = {};
